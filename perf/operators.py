@@ -247,7 +247,7 @@ def _own(state):
     act = 1 if case.get("gate") else 0
     if case["kind"] == "pack":
         codes, scales = ops.mxfp4_quantize(state["x"], rows=state["rows"], codes=state["codes"], scales=state["scales"])
-        return ops.mxfp4_dequantize(codes, scales, k=case["k"], out=state["out"])
+        return ops.mxfp4_dequantize(codes, scales, out=state["out"])
     if case["kind"] == "experts":
         return ops.mxfp4_grouped_gemm(state["a"], state["a_scales"], state["w"], state["w_scales"], state["offsets"], act=act, out=state["out"],
                                       workspace=state["workspace"])
