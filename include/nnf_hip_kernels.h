@@ -401,6 +401,47 @@ NNF_API int nnf_fused_mlp_wna16(nnf_stream_t stream,
                         int M, int H, int I, const nnf_quant* q_gate_up, const nnf_quant* q_down,
                         void* workspace, size_t workspace_bytes);
 
+/* ---------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (MXFP4 of the OCP microscaling formats), which gfx950's matrix cores multiply directly:
+ * quantising activations or weights, reading them back, the product, and the product grouped by expert.  The reference has
+ * neither the format nor a product over several weight matrices; the product stands where nnf_w8a8_gemm does, quantising and
+ * reading back where its Dequantize does (core/kernels/cpu/reference/kernels.cpp:601-623).
+ *   codes   u8 [rows, K/2]   two E2M1 values per byte, even k in the low nibble: sign, two exponent bits, one mantissa bit:
+ *                            +-0, 0.5, 1, 1.5, 2, 3, 4, 6
+ *   scales  u8 [rows, nnf_mxfp4_scale_bytes(K)]   byte b of a row: the values 32 b .. 32 b + 31 are times 2^(byte - 127); 255: all of
+ *                            them are NaN.  A row is padded to a multiple of 16 bytes (K a multiple of 512: none), written
+ *                            as 127 by nnf_mxfp4_quantize_f16 and read by nobody's arithmetic.
+ * K a multiple of 32 (NNF_ERR_UNSUPPORTED_SHAPE otherwise and above 2^22).  Products of two values are exact, sums are fp32 and the
+ * result is rounded once, behind bias, residual or SiLU-gate.  No function here needs synchronisation words or keeps state.
+ * ------------------------------------------------------------------------------------------- */
+NNF_API int nnf_mxfp4_scale_bytes(int K);
+
+/* x fp16 [source_rows, K] -> codes and scales of `rows` rows: row i is x's row index[i] (i32 [rows] on the device; zeros where
+ * x has no such row), or x's row i where index is NULL (then rows == source_rows).  A block's exponent is floor(log2(largest
+ * magnitude)) - 2, its values are rounded to the nearest (ties to the even code) and saturate at 6; a block of zeros has
+ * byte 127, a block with an infinity or NaN byte 255 and zero codes. */
+NNF_API int nnf_mxfp4_quantize_f16(nnf_stream_t stream, const void* x, const void* index, void* codes, void* scales,
+                           int rows, int source_rows, int K);
+/* y fp16 [rows, K]: the values, each rounded once (+-inf beyond fp16). */
+NNF_API int nnf_mxfp4_dequantize_f16(nnf_stream_t stream, const void* codes, const void* scales, void* y, int rows, int K);
+
+/* Y fp16 [M, N] = A . W^T + bias + residual, or with act == NNF_ACT_SILU_GATE (W has 2N rows: gate rows, then up rows; no bias,
+ * no residual) SiLU(gate) * up.  bias fp16 [N] and residual fp16 [M, N] may be NULL; the residual may be Y itself.  Y must not
+ * overlap the operands otherwise. */
+NNF_API size_t nnf_mxfp4_gemm_workspace_bytes(int M, int N, int K, int act);
+NNF_API int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y,
+                   int M, int N, int K, const void* bias, const void* residual, int act,
+                   void* workspace, size_t workspace_bytes);
+
+/* The product of a mixture's experts: rows of A [M, K] and Y [M, N] sorted by expert, one weight matrix each (W u8 [experts, N, K/2],
+ * 2N rows with NNF_ACT_SILU_GATE).  Group e is the rows offsets[e] .. offsets[e + 1] - 1; offsets i32 [experts + 1] on the device,
+ * not decreasing, within 0 .. M: a group may be empty, and rows before offsets[0] or from offsets[experts] on are left as they
+ * are in Y.  (Offsets that break this give undefined rows of Y, never an access outside the operands.) */
+NNF_API size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, int act);
+NNF_API int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
+                           const void* offsets, void* Y, int experts, int M, int N, int K, int act,
+                           void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

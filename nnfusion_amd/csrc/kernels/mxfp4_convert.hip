@@ -1,0 +1,150 @@
+// fp16 <-> MXFP4 (mxfp4.h): quantising rows, picked by an index or not, and reading them back.
+//
+// Both are one pass over memory: 2 bytes of fp16 and 17/32 byte of MXFP4 per value.  A wavefront takes units of 512 values of one row, eight
+// to a lane: 16 bytes of fp16, 4 bytes of codes, a block of 32 values to each four lanes, its scale byte by way of the lanes'
+// maximum.  A unit is 1 KiB, 256 bytes and 16 bytes in memory order; the row of scale bytes is padded to 16, so units never share one.
+#include "mxfp4.h"
+#include "nnf_launch.h"
+
+namespace nnf
+{
+    namespace
+    {
+        constexpr int CONVERT_THREADS = 256;
+        constexpr int CONVERT_UNITS = 4; // units of a wavefront, all their loads ahead of the first use
+
+        // the larger of two pairs of 16-bit magnitudes
+        __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b)
+        {
+            typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, a), __builtin_bit_cast(ushortx2, b)));
+        }
+
+        __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_quantize_kernel(const half_t* __restrict__ x, const int* __restrict__ index,
+                                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                                 long long units, int row_units, int source_rows, int K)
+        {
+            const int lane = threadIdx.x & (WAVE - 1);
+            const long long u0 = ((long long)blockIdx.x * (CONVERT_THREADS / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * CONVERT_UNITS;
+            uintx4 v[CONVERT_UNITS];
+            long long row[CONVERT_UNITS];
+            int unit[CONVERT_UNITS];
+#pragma unroll
+            for (int i = 0; i < CONVERT_UNITS; ++i)
+            {
+                row[i] = (u0 + i) / row_units;
+                unit[i] = (int)(u0 + i - row[i] * row_units);
+                const int k = unit[i] * 512 + lane * 8;
+                v[i] = uintx4{0, 0, 0, 0};
+                if (u0 + i < units && k < K)
+                {
+                    // (a row that is not there is a row of zeros)
+                    const long long from = index ? index[row[i]] : row[i];
+                    if (from >= 0 && from < source_rows)
+                        v[i] = *reinterpret_cast<const uintx4*>(x + from * K + k);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < CONVERT_UNITS; ++i)
+            {
+                if (u0 + i >= units)
+                    return;
+                // the largest magnitude of the block as an fp16 bit pattern: these are ordered like the numbers, infinity and NaN above
+                uint32_t top = max_u16x2(max_u16x2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), max_u16x2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
+                top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false)); // 1,0,3,2
+                top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false)); // 2,3,0,1
+                top = max(top >> 16, top & 0xFFFFu);
+                // floor(log2(top)) - 2 + 127: the exponent field of the same number in fp32, where fp16's subnormals are normal
+                const uint32_t exponent = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(half_t, (uint16_t)top)) >> 23;
+                const bool finite = top < 0x7C00u;
+                const uint32_t byte = top == 0 ? 127u : finite ? exponent - 2 : 255u;
+                const float scale = __builtin_bit_cast(float, byte << 23);
+                uint32_t code = 0;
+                // (the conversion divides by the scale's power of two, rounds to nearest even and saturates at 6)
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].x), scale, 0);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].y), scale, 1);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].z), scale, 2);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].w), scale, 3);
+                const int k = unit[i] * 512 + lane * 8;
+                if (k < K)
+                    *reinterpret_cast<uint32_t*>(codes + row[i] * (K / 2) + k / 2) = finite ? code : 0u;
+                if ((lane & 3) == 0)
+                    scales[(row[i] * row_units + unit[i]) * 16 + lane / 4] = (uint8_t)byte; // (behind the row's end: 2^0)
+            }
+        }
+
+        __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                                                   half_t* __restrict__ y, long long units, int row_units, int K)
+        {
+            const int lane = threadIdx.x & (WAVE - 1);
+            const long long u0 = ((long long)blockIdx.x * (CONVERT_THREADS / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * CONVERT_UNITS;
+            uint32_t code[CONVERT_UNITS], byte[CONVERT_UNITS];
+#pragma unroll
+            for (int i = 0; i < CONVERT_UNITS; ++i)
+            {
+                const long long row = (u0 + i) / row_units;
+                const int k = (int)(u0 + i - row * row_units) * 512 + lane * 8;
+                code[i] = 0, byte[i] = 127;
+                if (u0 + i < units && k < K)
+                {
+                    code[i] = *reinterpret_cast<const uint32_t*>(codes + row * (K / 2) + k / 2);
+                    byte[i] = scales[(u0 + i) * 16 + lane / 4];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < CONVERT_UNITS; ++i)
+            {
+                const long long row = (u0 + i) / row_units;
+                const int k = (int)(u0 + i - row * row_units) * 512 + lane * 8;
+                if (u0 + i >= units || k >= K)
+                    continue;
+                // 6 * 2^-30 and 0.5 * 2^20 are beyond fp16 as any value outside these two is (a scale of 2^-127 has no normal fp32)
+                const float scale = byte[i] == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, min(max(byte[i], 127u - 30u), 127u + 20u) << 23);
+                half8_t out;
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                {
+                    // the four-bit value exactly, then its product with the power of two, exact in fp32 and rounded once
+                    const half2_t h = p == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 0)
+                                      : p == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 1)
+                                      : p == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 2)
+                                               : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 3);
+                    out[2 * p] = (half_t)((float)h.x * scale);
+                    out[2 * p + 1] = (half_t)((float)h.y * scale);
+                }
+                *reinterpret_cast<half8_t*>(y + row * K + k) = out;
+            }
+        }
+
+        // workgroups for `units` units; 0: more than a grid holds
+        unsigned convert_grid(long long units)
+        {
+            const long long per_group = (long long)(CONVERT_THREADS / WAVE) * CONVERT_UNITS;
+            const long long groups = (units + per_group - 1) / per_group;
+            return groups > 0x7FFFFFFFLL ? 0u : (unsigned)groups;
+        }
+    } // namespace
+
+    hipError_t launch_mxfp4_quantize(hipStream_t s, const void* x, const void* index, void* codes, void* scales, int rows, int source_rows, int K)
+    {
+        const int row_units = (K + 511) / 512;
+        const long long units = (long long)rows * row_units;
+        const unsigned grid = convert_grid(units);
+        if (!grid)
+            return hipErrorInvalidConfiguration;
+        mxfp4_quantize_kernel<<<grid, CONVERT_THREADS, 0, s>>>((const half_t*)x, (const int*)index, (uint8_t*)codes, (uint8_t*)scales, units, row_units,
+                                                               source_rows, K);
+        return hipGetLastError();
+    }
+
+    hipError_t launch_mxfp4_dequantize(hipStream_t s, const void* codes, const void* scales, void* y, int rows, int K)
+    {
+        const int row_units = (K + 511) / 512;
+        const long long units = (long long)rows * row_units;
+        const unsigned grid = convert_grid(units);
+        if (!grid)
+            return hipErrorInvalidConfiguration;
+        mxfp4_dequantize_kernel<<<grid, CONVERT_THREADS, 0, s>>>((const uint8_t*)codes, (const uint8_t*)scales, (half_t*)y, units, row_units, K);
+        return hipGetLastError();
+    }
+} // namespace nnf

@@ -1,7 +1,9 @@
 // C ABI of libnnf_hip_kernels.so: argument checks, dispatch by shape, error mapping.
 // Declarations and the contract of each entry point are in include/nnf_hip_kernels.h.
 #include "nnf_hip_kernels.h"
+#include "kernels/mxfp4_launch.h"
 #include "kernels/nnf_launch.h"
+#include "nnf_mxfp4_plan.h"
 #include "nnf_workspace.h"
 
 #include <hip/hip_runtime.h>
@@ -863,6 +865,119 @@ int nnf_fused_mlp_wna16(nnf_stream_t stream, const void* x, const void* gamma, f
     if (st != NNF_OK)
         return st;
     return (int)nnf::launch_bias_residual(s, product, out, nullptr, x, M, H); // out may be x
+}
+
+} // extern "C"
+
+// ---- MXFP4 ----------------------------------------------------------------------------------------------------------------
+namespace
+{
+    // what the two products have in common; offsets == null: one weight matrix
+    int mxfp4_product(nnf_stream_t stream, const nnf::mx::Operands& o, int act)
+    {
+        if (!o.A || !o.As || !o.W || !o.Ws || !o.Y || o.M <= 0 || o.N <= 0 || o.K <= 0 || o.experts <= 0)
+            return NNF_ERR_INVALID_ARGUMENT;
+        if (act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE)
+            return NNF_ERR_INVALID_ARGUMENT;
+        if (!aligned16(o.A) || !aligned16(o.As) || !aligned16(o.W) || !aligned16(o.Ws) || !aligned16(o.Y) || !aligned16(o.bias) ||
+            !aligned16(o.residual) || !aligned16(o.offsets))
+            return NNF_ERR_INVALID_ARGUMENT;
+        const bool gate = act == NNF_ACT_SILU_GATE;
+        if (!nnf::mx::supported(o.K) || (gate && (o.bias || o.residual)) || o.N > (1 << 29) || o.M > (1 << 30))
+            return NNF_ERR_UNSUPPORTED_SHAPE;
+        const size_t y_bytes = (size_t)o.M * o.N * 2, w_rows = (size_t)o.experts * o.N * (gate ? 2 : 1);
+        const size_t row = (size_t)o.K / 2, scale_row = nnf::mx::scale_bytes(o.K);
+        // (workgroups still read when others write)
+        if (overlap(o.Y, y_bytes, o.A, o.M * row) || overlap(o.Y, y_bytes, o.As, o.M * scale_row) || overlap(o.Y, y_bytes, o.W, w_rows * row) ||
+            overlap(o.Y, y_bytes, o.Ws, w_rows * scale_row) || (o.bias && overlap(o.Y, y_bytes, o.bias, (size_t)o.N * 2)) ||
+            (o.offsets && overlap(o.Y, y_bytes, o.offsets, ((size_t)o.experts + 1) * 4)) ||
+            (o.residual && o.residual != o.Y && overlap(o.Y, y_bytes, o.residual, y_bytes)))
+            return NNF_ERR_INVALID_ARGUMENT;
+        DeviceInfo dev;
+        const int st = current_device_info(dev);
+        if (st != NNF_OK)
+            return st;
+        const nnf::mx::Plan plan = nnf::mx::plan(o.experts, o.M, o.N, o.K, gate, o.offsets != nullptr);
+        // (no tile or block has fewer than 16 columns)
+        if ((long long)plan.row_blocks * ((o.N + 15) / 16) > 0x7FFFFFFFLL)
+            return NNF_ERR_UNSUPPORTED_SHAPE;
+        return (int)(plan.tiles ? nnf::launch_mxfp4_tiles((hipStream_t)stream, o, 1 << plan.row_shift, plan.row_blocks, gate)
+                                : nnf::launch_mxfp4_rows((hipStream_t)stream, o, plan.row_shift, plan.row_blocks, gate));
+    }
+} // namespace
+
+extern "C" {
+
+int nnf_mxfp4_scale_bytes(int K)
+{
+    return K > 0 ? nnf::mx::scale_bytes(K) : 0;
+}
+
+int nnf_mxfp4_quantize_f16(nnf_stream_t stream, const void* x, const void* index, void* codes, void* scales, int rows, int source_rows, int K)
+{
+    if (!x || !codes || !scales || rows <= 0 || source_rows <= 0 || K <= 0 || (!index && rows != source_rows))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!aligned16(x) || !aligned16(index) || !aligned16(codes) || !aligned16(scales))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::mx::supported(K))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t x_bytes = (size_t)source_rows * K * 2, code_bytes = (size_t)rows * K / 2, scale_bytes = (size_t)rows * nnf::mx::scale_bytes(K);
+    if (overlap(codes, code_bytes, x, x_bytes) || overlap(scales, scale_bytes, x, x_bytes) || overlap(codes, code_bytes, scales, scale_bytes) ||
+        (index && (overlap(codes, code_bytes, index, (size_t)rows * 4) || overlap(scales, scale_bytes, index, (size_t)rows * 4))))
+        return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_mxfp4_quantize((hipStream_t)stream, x, index, codes, scales, rows, source_rows, K);
+}
+
+int nnf_mxfp4_dequantize_f16(nnf_stream_t stream, const void* codes, const void* scales, void* y, int rows, int K)
+{
+    if (!codes || !scales || !y || rows <= 0 || K <= 0 || !aligned16(codes) || !aligned16(scales) || !aligned16(y))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::mx::supported(K))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t y_bytes = (size_t)rows * K * 2;
+    if (overlap(y, y_bytes, codes, (size_t)rows * K / 2) || overlap(y, y_bytes, scales, (size_t)rows * nnf::mx::scale_bytes(K)))
+        return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_mxfp4_dequantize((hipStream_t)stream, codes, scales, y, rows, K);
+}
+
+size_t nnf_mxfp4_gemm_workspace_bytes(int M, int N, int K, int act)
+{
+    (void)M, (void)N, (void)K, (void)act;
+    return 0;
+}
+
+int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int M, int N, int K,
+                   const void* bias, const void* residual, int act, void* workspace, size_t workspace_bytes)
+{
+    (void)workspace, (void)workspace_bytes;
+    return mxfp4_product(stream, {(const uint8_t*)A, (const uint8_t*)a_scales, (const uint8_t*)W, (const uint8_t*)w_scales, (nnf::half_t*)Y,
+                                  (const nnf::half_t*)bias, (const nnf::half_t*)residual, nullptr, M, N, K, 1},
+                         act);
+}
+
+size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, int act)
+{
+    (void)experts, (void)M, (void)N, (void)K, (void)act;
+    return 0;
+}
+
+int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets, void* Y,
+                           int experts, int M, int N, int K, int act, void* workspace, size_t workspace_bytes)
+{
+    (void)workspace, (void)workspace_bytes;
+    if (!offsets)
+        return NNF_ERR_INVALID_ARGUMENT;
+    return mxfp4_product(stream, {(const uint8_t*)A, (const uint8_t*)a_scales, (const uint8_t*)W, (const uint8_t*)w_scales, (nnf::half_t*)Y, nullptr,
+                                  nullptr, (const int*)offsets, M, N, K, experts},
+                         act);
 }
 
 } // extern "C"

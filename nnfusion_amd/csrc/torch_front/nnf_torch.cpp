@@ -8,6 +8,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 
 #include "nnf_hip_kernels.h"
@@ -339,6 +340,165 @@ namespace
         return y.release();
     }
 
+    // ---- MXFP4.  These calls run on the device that holds their first tensor, whichever is current, on its current stream
+    bool is(const Tensor& t, at::ScalarType type, std::initializer_list<int64_t> sizes)
+    {
+        return t.scalar_type() == type && t.is_contiguous() && t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size());
+    }
+    void on_device(const Tensor& first, std::initializer_list<PyObject*> others)
+    {
+        require(first.is_cuda(), "tensors on a GPU");
+        for (PyObject* o : others)
+            require(o == Py_None || tensor(o).device() == first.device(), "all tensors on one device");
+    }
+    int size32(int64_t v)
+    {
+        if (v != (int)v)
+            raise(PyExc_OverflowError, "size out of range");
+        return (int)v;
+    }
+    // a new tensor of these sizes where the caller brought none; either way a reference of its own
+    PyObject* output(PyObject* given, std::initializer_list<int64_t> sizes, at::ScalarType type, const Tensor& like, const char* text)
+    {
+        if (given == Py_None)
+        {
+            PyObject* const o = THPVariable_Wrap(at::empty(at::IntArrayRef(sizes.begin(), sizes.size()), like.options().dtype(type)));
+            if (!o)
+                throw Raised();
+            return o;
+        }
+        require(is(tensor(given), type, sizes), text);
+        Py_INCREF(given);
+        return given;
+    }
+    struct Owned
+    {
+        PyObject* object;
+        explicit Owned(PyObject* o)
+            : object(o)
+        {
+        }
+        Owned(const Owned&) = delete;
+        ~Owned() { Py_XDECREF(object); }
+        void* data() const { return THPVariable_Unpack(object).data_ptr(); }
+        PyObject* release()
+        {
+            PyObject* o = object;
+            object = nullptr;
+            return o;
+        }
+    };
+    void workspace_checked(PyObject* o) { require(o == Py_None || (tensor(o).scalar_type() == at::kByte && tensor(o).is_contiguous()), "workspace: contiguous uint8"); }
+
+    // (x, rows, codes, scales) -> (codes, scales)
+    PyObject* mxfp4_quantize(Args v)
+    {
+        const Tensor& x = tensor(v[0]);
+        matrix(x);
+        require(x.scalar_type() == at::kHalf && x.is_contiguous(), "a contiguous fp16 matrix");
+        const int source = size32(x.size(0)), k = size32(x.size(1));
+        int rows = source;
+        if (v[1] != Py_None)
+        {
+            const Tensor& index = tensor(v[1]);
+            require(index.scalar_type() == at::kInt && index.dim() == 1 && index.is_contiguous(), "rows: a contiguous int32 vector");
+            rows = size32(index.size(0));
+        }
+        for (int i = 2; i < 4; ++i)
+            if (v[i] != Py_None)
+                require(is(tensor(v[i]), at::kByte, {rows, i == 2 ? k / 2 : nnf_mxfp4_scale_bytes(k)}), i == 2 ? "codes: contiguous uint8 [rows, K/2]" : "scales: contiguous uint8 [rows, mxfp4_scale_bytes(K)]");
+        on_device(x, {v[1], v[2], v[3]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+        Owned codes(output(v[2], {rows, k / 2}, at::kByte, x, "codes")), scales(output(v[3], {rows, nnf_mxfp4_scale_bytes(k)}, at::kByte, x, "scales"));
+        call("nnf_mxfp4_quantize_f16", nnf_mxfp4_quantize_f16, stream(), x.data_ptr(), address(v[1]), codes.data(), scales.data(), rows, source, k);
+        PyObject* const both = PyTuple_Pack(2, codes.object, scales.object);
+        if (!both)
+            throw Raised();
+        return both;
+    }
+
+    // (codes, scales, out)
+    PyObject* mxfp4_dequantize(Args v)
+    {
+        const Tensor &codes = tensor(v[0]), &scales = tensor(v[1]);
+        matrix(codes);
+        const int rows = size32(codes.size(0)), k = size32(codes.size(1) * 2);
+        require(is(codes, at::kByte, {rows, k / 2}), "codes: contiguous uint8 [rows, K/2]");
+        require(is(scales, at::kByte, {rows, nnf_mxfp4_scale_bytes(k)}), "scales: contiguous uint8 [rows, mxfp4_scale_bytes(K)]");
+        if (v[2] != Py_None)
+            require(is(tensor(v[2]), at::kHalf, {rows, k}), "out: contiguous fp16 [rows, K]");
+        on_device(codes, {v[1], v[2]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+        Owned y(output(v[2], {rows, k}, at::kHalf, codes, "out"));
+        call("nnf_mxfp4_dequantize_f16", nnf_mxfp4_dequantize_f16, stream(), codes.data_ptr(), scales.data_ptr(), y.data(), rows, k);
+        return y.release();
+    }
+
+    // the activations of either product: codes [M, K/2] and their scale bytes
+    void mxfp4_activations(const Tensor& a, const Tensor& as, int& m, int& k)
+    {
+        matrix(a);
+        m = size32(a.size(0)), k = size32(a.size(1) * 2);
+        require(is(a, at::kByte, {m, k / 2}), "activations: contiguous uint8 [M, K/2]");
+        require(is(as, at::kByte, {m, nnf_mxfp4_scale_bytes(k)}), "scales of the activations: contiguous uint8 [M, mxfp4_scale_bytes(K)]");
+    }
+    // columns of Y from the rows of a weight matrix
+    int mxfp4_columns(int64_t rows, int act)
+    {
+        require(act == NNF_ACT_NONE || act == NNF_ACT_SILU_GATE, "act: 0, or 1 for SiLU-gate");
+        require(act == NNF_ACT_NONE || rows % 2 == 0, "gate rows and as many up rows");
+        return size32(act == NNF_ACT_SILU_GATE ? rows / 2 : rows);
+    }
+
+    // (a, a_scales, w, w_scales, bias, residual, act, out, workspace)
+    PyObject* mxfp4_gemm(Args v)
+    {
+        const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]);
+        int m, k;
+        mxfp4_activations(a, as, m, k);
+        matrix(w);
+        const int act = integer(v[6]), n = mxfp4_columns(w.size(0), act);
+        require(is(w, at::kByte, {w.size(0), k / 2}) && is(ws, at::kByte, {w.size(0), nnf_mxfp4_scale_bytes(k)}), "weights: contiguous uint8 [N, K/2], scales [N, mxfp4_scale_bytes(K)]");
+        if (v[4] != Py_None)
+            require(is(tensor(v[4]), at::kHalf, {n}), "bias: contiguous fp16 [N]");
+        if (v[5] != Py_None)
+            require(is(tensor(v[5]), at::kHalf, {m, n}), "residual: contiguous fp16 [M, N]");
+        if (v[7] != Py_None)
+            require(is(tensor(v[7]), at::kHalf, {m, n}), "out: contiguous fp16 [M, N]");
+        workspace_checked(v[8]);
+        on_device(a, {v[1], v[2], v[3], v[4], v[5], v[7], v[8]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+        Owned y(output(v[7], {m, n}, at::kHalf, a, "out"));
+        Workspace space(v[8], a, [&] { return nnf_mxfp4_gemm_workspace_bytes(m, n, k, act); });
+        call("nnf_mxfp4_gemm", nnf_mxfp4_gemm, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data(), m, n, k, address(v[4]),
+             address(v[5]), act, space.data, space.bytes);
+        return y.release();
+    }
+
+    // (a, a_scales, w, w_scales, offsets, act, out, workspace)
+    PyObject* mxfp4_grouped_gemm(Args v)
+    {
+        const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]), &offsets = tensor(v[4]);
+        int m, k;
+        mxfp4_activations(a, as, m, k);
+        if (w.dim() != 3)
+            raise(PyExc_ValueError, "weights [experts, N, K/2] are expected");
+        const int experts = size32(w.size(0)), act = integer(v[5]), n = mxfp4_columns(w.size(1), act);
+        require(is(w, at::kByte, {experts, w.size(1), k / 2}) && is(ws, at::kByte, {experts, w.size(1), nnf_mxfp4_scale_bytes(k)}),
+                "weights: contiguous uint8 [experts, N, K/2], scales [experts, N, mxfp4_scale_bytes(K)]");
+        require(is(offsets, at::kInt, {(int64_t)experts + 1}), "offsets: contiguous int32 [experts + 1]");
+        if (v[6] != Py_None)
+            require(is(tensor(v[6]), at::kHalf, {m, n}), "out: contiguous fp16 [M, N]");
+        workspace_checked(v[7]);
+        on_device(a, {v[1], v[2], v[3], v[4], v[6], v[7]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+        Owned y(output(v[6], {m, n}, at::kHalf, a, "out"));
+        Workspace space(v[7], a, [&] { return nnf_mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act); });
+        call("nnf_mxfp4_grouped_gemm", nnf_mxfp4_grouped_gemm, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), offsets.data_ptr(),
+             y.data(), experts, m, n, k, act, space.data, space.bytes);
+        return y.release();
+    }
+
     template <PyObject* (*F)(Args), int N>
     PyObject* entry(PyObject*, Args v, Py_ssize_t n)
     {
@@ -372,7 +532,8 @@ namespace
 #define NNF_ENTRY(f, n) {#f, (PyCFunction)(void (*)(void))entry<f, n>, METH_FASTCALL, nullptr}
     PyMethodDef methods[] = {NNF_ENTRY(w4a16_gemm, 7),       NNF_ENTRY(wna16_gemm, 11),      NNF_ENTRY(w4a16_gemm_fused, 14), NNF_ENTRY(fused_mlp_w4a16, 13),
                              NNF_ENTRY(wna16_gemm_fused, 14), NNF_ENTRY(fused_mlp_wna16, 14), NNF_ENTRY(w8a8_gemm, 7),         NNF_ENTRY(w8a8_gemm_acc, 5),
-                             NNF_ENTRY(elementwise, 4),       NNF_ENTRY(rms_norm, 4),         NNF_ENTRY(dequantize, 7),        {"set_error", set_error, METH_O, nullptr},
+                             NNF_ENTRY(elementwise, 4),       NNF_ENTRY(rms_norm, 4),         NNF_ENTRY(dequantize, 7),        NNF_ENTRY(mxfp4_quantize, 4),
+                             NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 9),        NNF_ENTRY(mxfp4_grouped_gemm, 8), {"set_error", set_error, METH_O, nullptr},
                              {nullptr, nullptr, 0, nullptr}};
     PyModuleDef module = {PyModuleDef_HEAD_INIT, "nnf_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

@@ -266,3 +266,43 @@ def wna16_gemm_fused(a, wq, scales, bits=4, group=128, zp=8, zero_points=None, r
 def fused_mlp_wna16(x, gamma, wgu, sgu, wd, sd, bits=4, group=128, zp=8, zgu=None, zd=None, eps=1e-6, out=None, workspace=None):
     """The MLP block for every block parameter (zgu / zd: zero-point tensors of the two weight matrices, or None)."""
     return _native.fused_mlp_wna16(x, gamma, wgu, sgu, wd, sd, bits, group, zp, zgu, zd, eps, out, workspace)
+
+
+def mxfp4_scale_bytes(k):
+    """Bytes of a row of MXFP4 scale bytes: K / 32 rounded up to 16."""
+    return int(_lib.kernels().nnf_mxfp4_scale_bytes(k))
+
+
+def mxfp4_quantize(x, rows=None, codes=None, scales=None):
+    """fp16 [source_rows, K] -> (codes u8 [rows, K/2], scales u8 [rows, mxfp4_scale_bytes(K)]): microscaled 4-bit values in blocks of
+    32 along K.  rows: i32, the row of x that each quantised row is (tokens in the order of their experts; zeros where x has no
+    such row), or None for every row in turn."""
+    return _native.mxfp4_quantize(x, rows, codes, scales)
+
+
+def mxfp4_dequantize(codes, scales, out=None):
+    """The fp16 [rows, K] that MXFP4 codes and scale bytes stand for."""
+    return _native.mxfp4_dequantize(codes, scales, out)
+
+
+def mxfp4_gemm_workspace_bytes(m, n, k, act=0):
+    """Bytes of workspace mxfp4_gemm wants for this product (0: none)."""
+    return int(_lib.kernels().nnf_mxfp4_gemm_workspace_bytes(m, n, k, act))
+
+
+def mxfp4_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, workspace=None):
+    """Y fp16 [M,N] = A . W^T (+ bias + residual) of MXFP4 operands (see mxfp4_quantize), or with act=1 SiLU(gate) * up where w holds
+    the gate rows, then the up rows.  fp32 sums, one rounding at the end.  out may be the residual."""
+    return _native.mxfp4_gemm(a, a_scales, w, w_scales, bias, residual, act, out, workspace)
+
+
+def mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act=0):
+    """Bytes of workspace mxfp4_grouped_gemm wants for this product (0: none)."""
+    return int(_lib.kernels().nnf_mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act))
+
+
+def mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, workspace=None):
+    """The product of a mixture's experts: rows of a sorted by expert, w u8 [experts, N, K/2] (2N rows with act=1, SiLU-gate), w_scales
+    u8 [experts, N, mxfp4_scale_bytes(K)]; group e is the rows offsets[e] .. offsets[e+1] (offsets i32 [experts+1], on the device, not
+    decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here)."""
+    return _native.mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, workspace)
