@@ -433,6 +433,30 @@ NNF_API int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_sca
                    int M, int N, int K, const void* bias, const void* residual, int act,
                    void* workspace, size_t workspace_bytes);
 
+/* The kernels behind the two products as selectable variants (see nnf_w4a16_variant): activation rows x weight rows of a
+ * workgroup's tile.  Every one serves every shape; those without a form with SiLU-gate are NNF_ERR_UNSUPPORTED_SHAPE there
+ * (nnf_mxfp4_variant_supported).  NNF_MXFP4_AUTO: the one with the lowest estimated time for the shape. */
+enum nnf_mxfp4_variant
+{
+    NNF_MXFP4_AUTO = 0,
+    NNF_MXFP4_ROWS_16x16 = 1, /* operands straight into registers; no SiLU-gate */
+    NNF_MXFP4_ROWS_16x32 = 2,
+    NNF_MXFP4_TILE_8x32 = 3, /* through LDS, a range of K to each wavefront; no SiLU-gate */
+    NNF_MXFP4_TILE_16x32 = 4, /* no SiLU-gate */
+    NNF_MXFP4_TILE_16x64 = 5,
+    NNF_MXFP4_TILE_16x64_DEEP = 6,
+    NNF_MXFP4_TILE_32x64 = 7,
+    NNF_MXFP4_TILE_64x64 = 8,
+    NNF_MXFP4_TILE_64x64_DEEP = 9, /* through LDS, the wavefronts share the tile; no SiLU-gate */
+    NNF_MXFP4_TILE_128x128 = 10,
+    NNF_MXFP4_TILE_128x128_DEEP = 11,
+    NNF_MXFP4_TILE_256x256 = 12
+};
+NNF_API int nnf_mxfp4_variant_supported(int variant, int act);
+NNF_API int nnf_mxfp4_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y,
+                           int M, int N, int K, const void* bias, const void* residual, int act, int variant,
+                           void* workspace, size_t workspace_bytes);
+
 /* The product of a mixture's experts: rows of A [M, K] and Y [M, N] sorted by expert, one weight matrix each (W u8 [experts, N, K/2],
  * 2N rows with NNF_ACT_SILU_GATE).  Group e is the rows offsets[e] .. offsets[e + 1] - 1; offsets i32 [experts + 1] on the device,
  * not decreasing, within 0 .. M: a group may be empty, and rows before offsets[0] or from offsets[experts] on are left as they
@@ -441,6 +465,9 @@ NNF_API size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N,
 NNF_API int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
                            const void* offsets, void* Y, int experts, int M, int N, int K, int act,
                            void* workspace, size_t workspace_bytes);
+NNF_API int nnf_mxfp4_grouped_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
+                                   const void* offsets, void* Y, int experts, int M, int N, int K, int act, int variant,
+                                   void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

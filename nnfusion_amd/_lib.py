@@ -71,8 +71,11 @@ KERNEL_ABI = {
     "nnf_mxfp4_dequantize_f16": (_c_int, [_c_vp] * 4 + [_c_int] * 2),
     "nnf_mxfp4_gemm_workspace_bytes": (_c_sz, [_c_int] * 4),
     "nnf_mxfp4_gemm": (_c_int, [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_vp, _c_int, _c_vp, _c_sz]),
+    "nnf_mxfp4_variant_supported": (_c_int, [_c_int] * 2),
+    "nnf_mxfp4_gemm_variant": (_c_int, [_c_vp] * 6 + [_c_int] * 3 + [_c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_sz]),
     "nnf_mxfp4_grouped_gemm_workspace_bytes": (_c_sz, [_c_int] * 5),
     "nnf_mxfp4_grouped_gemm": (_c_int, [_c_vp] * 7 + [_c_int] * 5 + [_c_vp, _c_sz]),
+    "nnf_mxfp4_grouped_gemm_variant": (_c_int, [_c_vp] * 7 + [_c_int] * 6 + [_c_vp, _c_sz]),
 }
 
 

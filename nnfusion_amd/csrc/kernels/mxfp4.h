@@ -4,6 +4,7 @@
 // nibble; 32 values along K share the factor 2^(byte - 127), byte 255 standing for NaN (the OCP microscaling format).
 #pragma once
 
+#include "../nnf_mxfp4_plan.h"
 #include "nnf_device.h"
 
 namespace nnf
@@ -31,67 +32,103 @@ namespace nnf
             int experts;
         };
 
-        // `b`-th block of `1 << shift` rows: of all rows, or counted over the groups one after the other.  Every wavefront looks for
-        // itself: 64 groups a turn, their numbers of blocks added up across the lanes.  Offsets are clamped to the rows there are, so
-        // that no content of theirs leads outside the operands.  false: there is no such block.
-        struct RowBlock
+        inline long long row_blocks(const Operands& o, int rows) { return most_row_blocks(o.M, o.offsets ? o.experts : 0, rows); }
+
+        // The tile that workgroup `id` takes, of a product in blocks of `rows` rows and `col_tiles` tiles of columns: the groups one
+        // after the other; inside a group up to GROUPED row blocks of one column one after the other, then the next column, so that
+        // neighbours share their weights and the few rows of activations.  Workgroups go to the eight XCDs in turn, each of which has an
+        // L2 of its own: the order of the tiles is cut into eight runs, one an XCD.  Every wavefront looks for itself: 64 groups a turn, their
+        // numbers of blocks added up across the lanes.  Offsets are clamped to the rows there are, so that no content of theirs leads
+        // outside the operands.  false: there are no more tiles.
+        constexpr int GROUPED = 8;
+        struct TileAt
         {
-            int expert, first, end; // rows [first, end) of the group from the block's first row on
+            int expert, first, end; // rows [first, end) of the group from the tile's first row on
+            int column;             // tile of columns
         };
-        __device__ __forceinline__ bool find_rows(const Operands& o, int b, int shift, RowBlock& found)
+        __device__ __forceinline__ int xcd_order(int id, int n)
         {
+            const int xcd = id & 7, each = n >> 3, more = n & 7;
+            return xcd * each + min(xcd, more) + (id >> 3);
+        }
+        // rows [first, end) of the lane's group and its number of blocks
+        __device__ __forceinline__ int group_of_lane(const Operands& o, int e, int rows, int& first, int& end)
+        {
+            first = 0, end = 0;
+            if (e < o.experts)
+            {
+                first = min(max(o.offsets[e], 0), o.M);
+                end = min(max(o.offsets[e + 1], first), o.M);
+            }
+            return (end - first + rows - 1) / rows;
+        }
+        // sum over the lanes 0 .. own, in each lane: four shifts inside the rows of 16 lanes, then the rows' last lanes passed on
+        __device__ __forceinline__ int sum_up_to_lane(int v)
+        {
+            v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false); // row_shr:1
+            v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false); // row_shr:2
+            v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false); // row_shr:4
+            v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false); // row_shr:8
+            v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false); // row_bcast:15 into rows 1 and 3
+            v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false); // row_bcast:31 into rows 2 and 3
+            return v;
+        }
+        __device__ __forceinline__ bool find_tile(const Operands& o, int id, int rows, int col_tiles, TileAt& found)
+        {
+            int begin = 0, end = o.M, blocks = (o.M + rows - 1) / rows, expert = 0;
             if (!o.offsets)
             {
-                found = {0, b << shift, o.M};
-                return (b << shift) < o.M;
+                if (id >= blocks * col_tiles)
+                    return false;
+                id = xcd_order(id, blocks * col_tiles);
             }
-            const int lane = threadIdx.x & (WAVE - 1);
-            for (int e0 = 0; e0 < o.experts; e0 += WAVE)
+            else
             {
-                int first = 0, end = 0;
-                if (e0 + lane < o.experts)
+                const int lane = threadIdx.x & (WAVE - 1);
+                int first, last, own = group_of_lane(o, lane, rows, first, last), sum = sum_up_to_lane(own);
+                int all = __builtin_amdgcn_readlane(sum, WAVE - 1);
+                for (int e0 = WAVE; e0 < o.experts; e0 += WAVE)
                 {
-                    first = min(max(o.offsets[e0 + lane], 0), o.M);
-                    end = min(max(o.offsets[e0 + lane + 1], first), o.M);
+                    int f, l;
+                    all += __builtin_amdgcn_readlane(sum_up_to_lane(group_of_lane(o, e0 + lane, rows, f, l)), WAVE - 1);
                 }
-                const int blocks = (end - first + (1 << shift) - 1) >> shift;
-                int sum = blocks;
-#pragma unroll
-                for (int d = 1; d < WAVE; d <<= 1)
+                if (id >= all * col_tiles)
+                    return false;
+                id = xcd_order(id, all * col_tiles);
+                // the block that the tile would have if a block's columns came one after the other: it is of the same group
+                const int b = id / col_tiles;
+                int before = 0;
+                while (b >= before + __builtin_amdgcn_readlane(sum, WAVE - 1))
                 {
-                    const int v = __shfl_up(sum, d, WAVE);
-                    sum += lane >= d ? v : 0;
+                    before += __builtin_amdgcn_readlane(sum, WAVE - 1);
+                    expert += WAVE;
+                    if (expert >= o.experts)
+                        return false; // (offsets that overlap may count more blocks than an int holds)
+                    own = group_of_lane(o, expert + lane, rows, first, last);
+                    sum = sum_up_to_lane(own);
                 }
-                const uint64_t past = __ballot(sum > b);
-                if (past)
-                {
-                    const int at = __builtin_ctzll(past);
-                    found.expert = e0 + at;
-                    found.first = __builtin_amdgcn_readlane(first, at) + ((b - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(blocks, at))) << shift);
-                    found.end = __builtin_amdgcn_readlane(end, at);
-                    return true;
-                }
-                b -= __builtin_amdgcn_readlane(sum, WAVE - 1);
+                const uint64_t past = __ballot(before + sum > b);
+                const int at = past ? __builtin_ctzll(past) : 0;
+                blocks = __builtin_amdgcn_readlane(own, at);
+                id -= (before + __builtin_amdgcn_readlane(sum, at) - blocks) * col_tiles;
+                begin = __builtin_amdgcn_readlane(first, at);
+                end = __builtin_amdgcn_readlane(last, at);
+                expert += at;
+                if ((unsigned)id >= (unsigned)(blocks * col_tiles))
+                    return false;
             }
-            return false;
+            const int g = id / (GROUPED * col_tiles), of_group = min(blocks - g * GROUPED, GROUPED);
+            id -= g * (GROUPED * col_tiles);
+            const int column = id / of_group, block = g * GROUPED + id - column * of_group;
+            found = {expert, begin + block * rows, end, column};
+            return true;
         }
-
-        // bytes from one row of scale bytes to the next: K / 32 rounded up to 16, so that every row starts on 16 bytes
-        __host__ __device__ __forceinline__ constexpr int mx_scale_stride(int K) { return ((K >> 5) + 15) & ~15; }
 
         // 32 four-bit values as an operand of the scaled MFMA, which reads the first four registers of this format
         __device__ __forceinline__ intx8 operand(uintx4 v)
         {
             const intx4 i = __builtin_bit_cast(intx4, v);
             return __builtin_shufflevector(i, i, 0, 1, 2, 3, -1, -1, -1, -1);
-        }
-
-        // position `id` of a grid of `n` workgroups -> the tile it takes.  Workgroups go to the eight XCDs in turn: this way each XCD, which
-        // has an L2 of its own, works on one run of neighbouring tiles.
-        __device__ __forceinline__ int xcd_order(int id, int n)
-        {
-            const int xcd = id & 7, each = n >> 3, more = n & 7;
-            return xcd * each + min(xcd, more) + (id >> 3);
         }
 
         // bias and residual of four columns whose rows start on eight bytes
@@ -134,19 +171,47 @@ namespace nnf
                 }
         }
 
-        // Y[m, n .. n + 7], n a multiple of 8 below N
-        __device__ __forceinline__ void write_eight(const Operands& o, floatx4 y0, floatx4 y1, int m, int n)
+        // Y[row(i), n .. n + 7] for each i with a row (row(i) < 0: none), n a multiple of 8 below N
+        template <int COUNT, class Row>
+        __device__ __forceinline__ void write_rows(const Operands& o, floatx4 (&y)[COUNT][2], int n, Row row)
         {
             if (o.N & 7)
             {
-                write_four(o, y0, m, n);
-                write_four(o, y1, m, n + 4);
+#pragma unroll
+                for (int i = 0; i < COUNT; ++i)
+                    if (row(i) >= 0)
+                    {
+                        write_four(o, y[i][0], row(i), n);
+                        write_four(o, y[i][1], row(i), n + 4);
+                    }
                 return;
             }
-            add_four(o, y0, m, n);
-            add_four(o, y1, m, n + 4);
-            *reinterpret_cast<half8_t*>(o.Y + (size_t)m * o.N + n) = half8_t{(half_t)y0.x, (half_t)y0.y, (half_t)y0.z, (half_t)y0.w,
-                                                                             (half_t)y1.x, (half_t)y1.y, (half_t)y1.z, (half_t)y1.w};
+            if (o.bias)
+            {
+                const half8_t v = *reinterpret_cast<const half8_t*>(o.bias + n);
+#pragma unroll
+                for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[i][e / 4][e % 4] += (float)v[e];
+            }
+            if (o.residual)
+            {
+                half8_t v[COUNT];
+#pragma unroll
+                for (int i = 0; i < COUNT; ++i)
+                    v[i] = *reinterpret_cast<const half8_t*>(o.residual + (size_t)max(row(i), 0) * o.N + n);
+#pragma unroll
+                for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[i][e / 4][e % 4] += (float)v[i][e];
+            }
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i)
+                if (row(i) >= 0)
+                    *reinterpret_cast<half8_t*>(o.Y + (size_t)row(i) * o.N + n) = half8_t{(half_t)y[i][0].x, (half_t)y[i][0].y, (half_t)y[i][0].z, (half_t)y[i][0].w,
+                                                                                         (half_t)y[i][1].x, (half_t)y[i][1].y, (half_t)y[i][1].z, (half_t)y[i][1].w};
         }
 
         // SiLU(g) * u in fp32

@@ -11,7 +11,7 @@ namespace nnf
     namespace
     {
         constexpr int CONVERT_THREADS = 256;
-        constexpr int CONVERT_UNITS = 4; // units of a wavefront, all their loads ahead of the first use
+        constexpr int WAVES = CONVERT_THREADS / WAVE;
 
         // the larger of two pairs of 16-bit magnitudes
         __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b)
@@ -20,34 +20,53 @@ namespace nnf
             return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, a), __builtin_bit_cast(ushortx2, b)));
         }
 
+        // where the units of a wavefront lie: UNITS of them from its first on, their rows and places in them found with one division
+        template <int UNITS, class Index>
+        struct Place
+        {
+            Index first; // unit of the first
+            Index row[UNITS];
+            int unit[UNITS];
+            __device__ __forceinline__ Place(int row_units)
+            {
+                first = ((Index)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * UNITS;
+                row[0] = first / row_units;
+                unit[0] = (int)(first - row[0] * row_units);
+#pragma unroll
+                for (int i = 1; i < UNITS; ++i)
+                {
+                    const bool next = unit[i - 1] + 1 == row_units;
+                    row[i] = row[i - 1] + (next ? 1 : 0);
+                    unit[i] = next ? 0 : unit[i - 1] + 1;
+                }
+            }
+        };
+
+        template <int UNITS, class Index>
         __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_quantize_kernel(const half_t* __restrict__ x, const int* __restrict__ index,
                                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                                 long long units, int row_units, int source_rows, int K)
+                                                                                 Index units, int row_units, int source_rows, int K)
         {
             const int lane = threadIdx.x & (WAVE - 1);
-            const long long u0 = ((long long)blockIdx.x * (CONVERT_THREADS / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * CONVERT_UNITS;
-            uintx4 v[CONVERT_UNITS];
-            long long row[CONVERT_UNITS];
-            int unit[CONVERT_UNITS];
+            const Place<UNITS, Index> at(row_units);
+            uintx4 v[UNITS];
 #pragma unroll
-            for (int i = 0; i < CONVERT_UNITS; ++i)
+            for (int i = 0; i < UNITS; ++i)
             {
-                row[i] = (u0 + i) / row_units;
-                unit[i] = (int)(u0 + i - row[i] * row_units);
-                const int k = unit[i] * 512 + lane * 8;
+                const int k = at.unit[i] * 512 + lane * 8;
                 v[i] = uintx4{0, 0, 0, 0};
-                if (u0 + i < units && k < K)
+                if (at.first + i < units && k < K)
                 {
                     // (a row that is not there is a row of zeros)
-                    const long long from = index ? index[row[i]] : row[i];
+                    const long long from = index ? index[at.row[i]] : (long long)at.row[i];
                     if (from >= 0 && from < source_rows)
                         v[i] = *reinterpret_cast<const uintx4*>(x + from * K + k);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < CONVERT_UNITS; ++i)
+            for (int i = 0; i < UNITS; ++i)
             {
-                if (u0 + i >= units)
+                if (at.first + i >= units)
                     return;
                 // the largest magnitude of the block as an fp16 bit pattern: these are ordered like the numbers, infinity and NaN above
                 uint32_t top = max_u16x2(max_u16x2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), max_u16x2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
@@ -65,86 +84,86 @@ namespace nnf
                 code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].y), scale, 1);
                 code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].z), scale, 2);
                 code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(code, as_half2(v[i].w), scale, 3);
-                const int k = unit[i] * 512 + lane * 8;
+                const int k = at.unit[i] * 512 + lane * 8;
                 if (k < K)
-                    *reinterpret_cast<uint32_t*>(codes + row[i] * (K / 2) + k / 2) = finite ? code : 0u;
+                    *reinterpret_cast<uint32_t*>(codes + (size_t)at.row[i] * (K / 2) + k / 2) = finite ? code : 0u;
                 if ((lane & 3) == 0)
-                    scales[(row[i] * row_units + unit[i]) * 16 + lane / 4] = (uint8_t)byte; // (behind the row's end: 2^0)
+                    scales[(size_t)(at.first + i) * 16 + lane / 4] = (uint8_t)byte; // (behind the row's end: 2^0)
             }
         }
 
+        template <int UNITS, class Index>
         __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                                   half_t* __restrict__ y, long long units, int row_units, int K)
+                                                                                   half_t* __restrict__ y, Index units, int row_units, int K)
         {
             const int lane = threadIdx.x & (WAVE - 1);
-            const long long u0 = ((long long)blockIdx.x * (CONVERT_THREADS / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * CONVERT_UNITS;
-            uint32_t code[CONVERT_UNITS], byte[CONVERT_UNITS];
+            const Place<UNITS, Index> at(row_units);
+            uint32_t code[UNITS], byte[UNITS];
 #pragma unroll
-            for (int i = 0; i < CONVERT_UNITS; ++i)
+            for (int i = 0; i < UNITS; ++i)
             {
-                const long long row = (u0 + i) / row_units;
-                const int k = (int)(u0 + i - row * row_units) * 512 + lane * 8;
+                const int k = at.unit[i] * 512 + lane * 8;
                 code[i] = 0, byte[i] = 127;
-                if (u0 + i < units && k < K)
+                if (at.first + i < units && k < K)
                 {
-                    code[i] = *reinterpret_cast<const uint32_t*>(codes + row * (K / 2) + k / 2);
-                    byte[i] = scales[(u0 + i) * 16 + lane / 4];
+                    code[i] = *reinterpret_cast<const uint32_t*>(codes + (size_t)at.row[i] * (K / 2) + k / 2);
+                    byte[i] = scales[(size_t)(at.first + i) * 16 + lane / 4];
                 }
             }
 #pragma unroll
-            for (int i = 0; i < CONVERT_UNITS; ++i)
+            for (int i = 0; i < UNITS; ++i)
             {
-                const long long row = (u0 + i) / row_units;
-                const int k = (int)(u0 + i - row * row_units) * 512 + lane * 8;
-                if (u0 + i >= units || k >= K)
+                const int k = at.unit[i] * 512 + lane * 8;
+                if (at.first + i >= units || k >= K)
                     continue;
                 // 6 * 2^-30 and 0.5 * 2^20 are beyond fp16 as any value outside these two is (a scale of 2^-127 has no normal fp32)
                 const float scale = byte[i] == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, min(max(byte[i], 127u - 30u), 127u + 20u) << 23);
+                // the four-bit values exactly, then their products with the power of two, exact in fp32 and rounded once
+                const half2_t h[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 1),
+                                      __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 3)};
                 half8_t out;
 #pragma unroll
-                for (int p = 0; p < 4; ++p)
-                {
-                    // the four-bit value exactly, then its product with the power of two, exact in fp32 and rounded once
-                    const half2_t h = p == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 0)
-                                      : p == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 1)
-                                      : p == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 2)
-                                               : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[i], 1.0f, 3);
-                    out[2 * p] = (half_t)((float)h.x * scale);
-                    out[2 * p + 1] = (half_t)((float)h.y * scale);
-                }
-                *reinterpret_cast<half8_t*>(y + row * K + k) = out;
+                for (int p = 0; p < 8; ++p)
+                    out[p] = (half_t)((float)h[p / 2][p % 2] * scale);
+                *reinterpret_cast<half8_t*>(y + (size_t)at.row[i] * K + k) = out;
             }
         }
 
-        // workgroups for `units` units; 0: more than a grid holds
-        unsigned convert_grid(long long units)
+        // f(units, units of a wavefront as a constant, the type that counts them, workgroups): four units a wavefront, all their loads ahead
+        // of the first use, once these fill the CUs; one below, where the time is one load's latency and as many wavefronts as there are
+        // units share it
+        template <class F>
+        hipError_t over_units(int rows, int K, F f)
         {
-            const long long per_group = (long long)(CONVERT_THREADS / WAVE) * CONVERT_UNITS;
-            const long long groups = (units + per_group - 1) / per_group;
-            return groups > 0x7FFFFFFFLL ? 0u : (unsigned)groups;
+            constexpr int MANY = 4;
+            const int row_units = (K + 511) / 512;
+            const long long units = (long long)rows * row_units;
+            if (units < 256 * WAVES * MANY * 2)
+                return f((int)units, std::integral_constant<int, 1>{}, row_units, (unsigned)((units + WAVES - 1) / WAVES));
+            const long long groups = (units + WAVES * MANY - 1) / (WAVES * MANY);
+            if (groups > 0x7FFFFFFFLL)
+                return hipErrorInvalidConfiguration;
+            if (units < 0x7FFFFFFFLL - WAVES * MANY)
+                return f((int)units, std::integral_constant<int, MANY>{}, row_units, (unsigned)groups);
+            return f(units, std::integral_constant<int, MANY>{}, row_units, (unsigned)groups);
         }
     } // namespace
 
     hipError_t launch_mxfp4_quantize(hipStream_t s, const void* x, const void* index, void* codes, void* scales, int rows, int source_rows, int K)
     {
-        const int row_units = (K + 511) / 512;
-        const long long units = (long long)rows * row_units;
-        const unsigned grid = convert_grid(units);
-        if (!grid)
-            return hipErrorInvalidConfiguration;
-        mxfp4_quantize_kernel<<<grid, CONVERT_THREADS, 0, s>>>((const half_t*)x, (const int*)index, (uint8_t*)codes, (uint8_t*)scales, units, row_units,
-                                                               source_rows, K);
-        return hipGetLastError();
+        return over_units(rows, K, [&](auto units, auto many, int row_units, unsigned groups) {
+            mxfp4_quantize_kernel<many, decltype(units)><<<groups, CONVERT_THREADS, 0, s>>>((const half_t*)x, (const int*)index, (uint8_t*)codes,
+                                                                                            (uint8_t*)scales, units, row_units, source_rows, K);
+            return hipGetLastError();
+        });
     }
 
     hipError_t launch_mxfp4_dequantize(hipStream_t s, const void* codes, const void* scales, void* y, int rows, int K)
     {
-        const int row_units = (K + 511) / 512;
-        const long long units = (long long)rows * row_units;
-        const unsigned grid = convert_grid(units);
-        if (!grid)
-            return hipErrorInvalidConfiguration;
-        mxfp4_dequantize_kernel<<<grid, CONVERT_THREADS, 0, s>>>((const uint8_t*)codes, (const uint8_t*)scales, (half_t*)y, units, row_units, K);
-        return hipGetLastError();
+        return over_units(rows, K, [&](auto units, auto many, int row_units, unsigned groups) {
+            mxfp4_dequantize_kernel<many, decltype(units)><<<groups, CONVERT_THREADS, 0, s>>>((const uint8_t*)codes, (const uint8_t*)scales, (half_t*)y, units,
+                                                                                              row_units, K);
+            return hipGetLastError();
+        });
     }
 } // namespace nnf

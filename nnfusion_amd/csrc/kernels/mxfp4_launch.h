@@ -8,8 +8,7 @@ namespace nnf
     // rows == null: every row; else codes and scales of row i are those of x's row index[i], zeros where there is no such row
     hipError_t launch_mxfp4_quantize(hipStream_t s, const void* x, const void* index, void* codes, void* scales, int rows, int source_rows, int K);
     hipError_t launch_mxfp4_dequantize(hipStream_t s, const void* codes, const void* scales, void* y, int rows, int K);
-    // blocks of 1 << row_shift (4, 5, 6) rows, `row_blocks` of them
-    hipError_t launch_mxfp4_rows(hipStream_t s, const mx::Operands& o, int row_shift, int row_blocks, bool gate);
-    // tiles of `rows` rows (256 x 256, 128 x 128, 64 x 256); `row_blocks` blocks of that many rows
-    hipError_t launch_mxfp4_tiles(hipStream_t s, const mx::Operands& o, int rows, int row_blocks, bool gate);
+    // `kernel`: one of mx::Kernel that has this form (mx::choose)
+    hipError_t launch_mxfp4_rows(hipStream_t s, const mx::Operands& o, int kernel, bool gate);
+    hipError_t launch_mxfp4_tiles(hipStream_t s, const mx::Operands& o, int kernel, bool gate);
 } // namespace nnf

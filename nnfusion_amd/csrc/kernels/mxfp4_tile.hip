@@ -1,4 +1,4 @@
-// MXFP4 x MXFP4 in tiles through LDS, for more rows than the weights' own traffic pays for.
+// MXFP4 x MXFP4 in tiles through LDS.
 //
 // v_mfma_scale_f32_32x32x64: lane l holds 32 values of row l % 32, one of the step's two blocks, and their scale byte.  K goes in steps
 // of 256 values -- 128 bytes of a row, a whole line of memory -- and the lanes of the half g take the blocks 4 g .. 4 g + 3 of a step
@@ -15,22 +15,28 @@ namespace nnf
         using namespace mx;
 
         constexpr int STEP_BYTES = 128; // of a row: 256 values
-        constexpr int SCALE_BYTES = 16; // of a row's scale bytes: two steps, fetched together
+        constexpr int STEP_SCALES = 8;  // scale bytes of that
 
-        // WM x WN wavefronts, each with FM x 32 activation rows and FN x 32 weight rows.  LDS: two steps of codes, three pairs of steps of
-        // scale bytes (half of a pair is fetched with each step, a pair ahead).
-        template <int WM_, int WN_, int FM_, int FN_>
+        // WK groups of WM x WN wavefronts; a group has the whole tile over its part of K, a wavefront FM x 32 activation rows and FN x 32
+        // weight rows of it (ROWS below 32: that many rows of a fragment are fetched, the others repeat them).  LDS, a group: S steps of
+        // codes, and scale bytes twice for G steps.  The memory pipeline's time goes by the lines that a load touches: eight rows for
+        // a load of codes; the scale bytes of one step would be 8 bytes of each row and as many lines as its codes, so they are
+        // fetched for G steps together, 1024 / (8 G) rows to a load.
+        template <int WM_, int WN_, int WK_, int FM_, int FN_, int S_, int G_ = 4, int ROWS_ = WM_ * FM_ * 32>
         struct Tile
         {
-            static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_;
-            static constexpr int WAVES = WM * WN, ROWS = WM * FM * 32, COLS = WN * FN * 32;
-            static constexpr int STAGE = (ROWS + COLS) * STEP_BYTES;
-            static constexpr int SCALES = (ROWS + COLS) * SCALE_BYTES;
-            static constexpr int LOADS = (ROWS + COLS) / 8 / WAVES;           // of codes, a step and wavefront
-            static constexpr int SCALE_LOADS = (ROWS + COLS) / 64;            // a pair of steps
-            static constexpr int HALF_SCALE_LOADS = (SCALE_LOADS + 1) / 2;    // a step, one to a wavefront
-            static constexpr int LDS = 2 * STAGE + 3 * SCALES;
-            static_assert((ROWS + COLS) / 8 % WAVES == 0 && COLS % 64 == 0 && ROWS % 64 == 0 && HALF_SCALE_LOADS <= WAVES, "whole loads");
+            static constexpr int WM = WM_, WN = WN_, WK = WK_, FM = FM_, FN = FN_, S = S_, G = G_;
+            static constexpr int GROUP = WM * WN, WAVES = GROUP * WK, ROWS = ROWS_, COLS = WN * FN * 32;
+            static constexpr int LOADS = (ROWS + COLS) / 8 / GROUP;                         // of codes, a step and wavefront
+            static constexpr int SCALE_ROWS = 1024 / (STEP_SCALES * G);                     // of a load of scale bytes
+            static constexpr int ALL_SCALE_LOADS = (ROWS + COLS + SCALE_ROWS - 1) / SCALE_ROWS; // for G steps
+            static constexpr int SCALE_LOADS = (ALL_SCALE_LOADS + GROUP - 1) / GROUP;       // of a wavefront
+            static constexpr int STAGE = (ROWS + COLS) * STEP_BYTES, SCALES = ALL_SCALE_LOADS * 1024;
+            static constexpr int GROUP_LDS = S * STAGE + 2 * SCALES;
+            static constexpr int PITCH = FN * 128 + 16;                                     // fp32 results of a row of a wavefront
+            static constexpr int LDS = GROUP_LDS * WK > WAVES * 32 * PITCH ? GROUP_LDS * WK : WAVES * 32 * PITCH;
+            static_assert((ROWS == WM * FM * 32 || (ROWS < 32 && GROUP * FM == 1)) && (ROWS + COLS) / 8 % GROUP == 0, "whole loads");
+            static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && SCALE_ROWS <= 32 && S >= 2 && S <= 4 && (S - 1) * LOADS < 64, "room for them, and a count");
         };
 
         template <int OFFSET>
@@ -43,47 +49,48 @@ namespace nnf
             __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(base + offset),
                                              (void __attribute__((address_space(3)))*)lds, 16, 0, 0);
         }
+        // until at most N of this wavefront's loads are under way
+        template <int N>
+        __device__ __forceinline__ void wait_loads()
+        {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+        }
 
         template <class T, bool GATE>
         __global__ __launch_bounds__(T::WAVES* WAVE, 1) void mxfp4_tile_kernel(Operands o, int col_tiles)
         {
             extern __shared__ __align__(256) uint8_t lds[];
-            const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-            const int tile = xcd_order(blockIdx.x, gridDim.x);
-            const int block = tile / col_tiles;
-            RowBlock rows;
-            if (!find_rows(o, block, T::ROWS == 256 ? 8 : T::ROWS == 128 ? 7 : 6, rows))
+            const int lane = threadIdx.x & (WAVE - 1), wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+            const int group = wave_id / T::GROUP, wave = wave_id % T::GROUP;
+            TileAt rows;
+            if (!find_tile(o, blockIdx.x, T::ROWS, col_tiles, rows))
                 return;
             constexpr int OUT = GATE ? T::COLS / 2 : T::COLS; // columns of Y
-            const int n0 = (tile - block * col_tiles) * OUT;
-            const int row_bytes = o.K >> 1, scale_stride = mx_scale_stride(o.K);
-            const int steps = (row_bytes + STEP_BYTES - 1) / STEP_BYTES;
+            const int n0 = rows.column * OUT;
+            const int row_bytes = o.K >> 1, scale_stride = scale_bytes(o.K);
+            const int all_steps = (row_bytes + STEP_BYTES - 1) / STEP_BYTES;
+            // this group's steps: whole pairs, the same number for every group (steps behind the end add zeros)
+            const int part = T::WK == 1 ? all_steps : ((all_steps + T::WK - 1) / T::WK + 1) & ~1;
+            const int steps = min(part, all_steps), first_step = group * part;
             const size_t w_row = (size_t)rows.expert * (GATE ? 2 * o.N : o.N) + n0;
 
             // ---- what this wavefront fetches: rows of the tile in memory order, weights first, eight to a load
-            // row `i` of the tile's weight rows: with SiLU-gate a wavefront's columns are half gate rows, half their up rows
-            const auto weight_row = [&](int i, bool& up) {
-                up = false;
+            // row `i` of the tile's weight rows, counted from its first: with SiLU-gate a wavefront's columns are half gate rows, half their
+            // up rows
+            const auto weight_row = [&](int i) {
                 if constexpr (GATE)
                 {
                     constexpr int HALF = T::FN * 16;
                     const int in = i % (2 * HALF);
-                    up = in >= HALF;
-                    i = i / (2 * HALF) * HALF + in % HALF;
+                    return min(i / (2 * HALF) * HALF + in % HALF, o.N - 1 - n0) + (in >= HALF ? o.N : 0);
                 }
-                return min(i, o.N - 1 - n0);
+                else
+                    return min(i, o.N - 1 - n0);
             };
             const uint8_t* const a_base = o.A + (size_t)rows.first * row_bytes;
             const uint8_t* const w_base = o.W + w_row * row_bytes;
             uint32_t offset[T::LOADS];
-            const auto load_base = [&](int j) {
-                const int row = (wave * T::LOADS + j) * 8;
-                if (row >= T::COLS)
-                    return a_base;
-                bool up;
-                weight_row(row, up);
-                return up ? w_base + (size_t)o.N * row_bytes : w_base;
-            };
+            const auto load_base = [&](auto j) { return (wave * T::LOADS + (T::COLS % (T::LOADS * 8) == 0 ? 0 : (int)j)) * 8 >= T::COLS ? a_base : w_base; };
             // piece of a row (16 bytes) that lies at slot `lane % 8` of row `row` in LDS: XORed so that the reads of 16 rows' pieces
             // spread over all banks
             const auto piece = [&](int row) { return (lane & 7) ^ ((row >> 1) & 7); };
@@ -91,50 +98,87 @@ namespace nnf
             for (int j = 0; j < T::LOADS; ++j)
             {
                 const int row = (wave * T::LOADS + j) * 8 + (lane >> 3);
-                bool up;
-                const int at = row < T::COLS ? weight_row(row, up) : min(row - T::COLS, rows.end - rows.first - 1);
+                const int at = row < T::COLS ? weight_row(row) : min(row - T::COLS, rows.end - rows.first - 1);
                 offset[j] = (uint32_t)at * row_bytes + piece(row) * 16;
             }
-            // this wavefront's scale bytes of either half of a pair: 64 rows, one to a lane (where there are fewer loads than wavefronts,
-            // some fetch the same again)
-            const uint8_t* scale_from[2];
-            uint32_t scale_to[2];
+            // scale bytes of G steps: 16 bytes of a row to a lane, neighbouring lanes neighbouring rows (where there are fewer loads than
+            // wavefronts, some fetch the same again)
+            const uint8_t* scale_row[T::SCALE_LOADS];
+            uint32_t scale_to[T::SCALE_LOADS];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int p = 0; p < T::SCALE_LOADS; ++p)
             {
-                const int q = min(h * T::HALF_SCALE_LOADS + wave % T::HALF_SCALE_LOADS, T::SCALE_LOADS - 1);
-                const int row = q * 64 + lane;
-                if (q * 64 < T::COLS)
+                const int q = min(p * T::GROUP + wave, T::ALL_SCALE_LOADS - 1);
+                const int row = min(q * T::SCALE_ROWS + lane % T::SCALE_ROWS, T::ROWS + T::COLS - 1);
+                scale_row[p] = row < T::COLS ? o.Ws + (w_row + weight_row(row)) * scale_stride
+                                             : o.As + (size_t)(rows.first + min(row - T::COLS, rows.end - rows.first - 1)) * scale_stride;
+                scale_to[p] = q * 1024;
+            }
+            const uint32_t codes_at = lds_address(lds) + group * T::GROUP_LDS, scales_at = codes_at + T::S * T::STAGE;
+            const auto fetch_scales = [&](int step) {
+                // (behind the end of a row: its last 16 bytes, not used)
+                const int from = min((first_step + step) * STEP_SCALES + lane / T::SCALE_ROWS * 16, scale_stride - 16);
+#pragma unroll
+                for (int p = 0; p < T::SCALE_LOADS; ++p)
+                    load_to_lds(scale_row[p] + from, 0, scales_at + (step / T::G & 1) * T::SCALES + scale_to[p]);
+            };
+            // codes of a step, load by load.  FULL: the step ends within
+            // the rows; else a row's last piece stands for those behind its end, and is not used
+            const auto fetch_load = [&](auto j, int step, uint32_t stage, auto full) {
+                uint32_t from = offset[j];
+                int k0 = (first_step + step) * STEP_BYTES;
+                if constexpr (!full)
                 {
-                    bool up;
-                    const int at = weight_row(row, up);
-                    scale_from[h] = o.Ws + (w_row + at + (up ? o.N : 0)) * scale_stride;
+                    k0 = min(k0, row_bytes - 16);
+                    const int p = piece((wave * T::LOADS + j) * 8 + (lane >> 3)) * 16;
+                    from += min(p, row_bytes - 16 - k0) - p;
                 }
                 else
-                    scale_from[h] = o.As + (size_t)(rows.first + min(row - T::COLS, rows.end - rows.first - 1)) * scale_stride;
-                scale_to[h] = q * 1024;
-            }
-            const uint32_t lds0 = lds_address(lds);
-            const int last_pair = (steps - 1) >> 1;
-            const auto fetch_scales = [&](int pair, int h) {
-                load_to_lds((h ? scale_from[1] : scale_from[0]) + min(pair, last_pair) * SCALE_BYTES, 0,
-                            lds0 + 2 * T::STAGE + pair % 3 * T::SCALES + (h ? scale_to[1] : scale_to[0]));
+                    asm("" : "+v"(from)); // (or the compiler keeps a 64-bit address for each load: base + offset stays an address of two parts)
+                load_to_lds(load_base(j) + k0, from, codes_at + stage + (wave * T::LOADS + j) * 1024);
             };
-            // codes of a step, and half of the scale bytes of the pair of steps after the step's own.  LAST: the step may end behind the
-            // rows' end: a row's last piece stands for those that are not there, and is not used
-            const auto fetch = [&](int step, auto last) {
-                const int k0 = step * STEP_BYTES;
-                const uint32_t stage = lds0 + (step & 1) * T::STAGE;
+            const auto fetch = [&](int step, uint32_t stage) {
+                unroll_for<0, T::LOADS>([&](auto j) { fetch_load(j, step, stage, std::false_type{}); });
+            };
+            // a step that does not end within the rows, landed: what this wavefront has fetched from behind their end becomes zeros, of the
+            // weights, times 2^0 of both operands
+            const auto cut = [&](int step, uint32_t stage) {
+                const int blocks = (row_bytes >> 4) - (first_step + step) * 8;
                 unroll_for<0, T::LOADS>([&](auto j) {
-                    uint32_t from = offset[j];
-                    if constexpr (last)
-                    {
-                        const int p = piece((wave * T::LOADS + j) * 8 + (lane >> 3)) * 16;
-                        from += min(p, row_bytes - 16 - k0) - p;
-                    }
-                    load_to_lds(load_base(j) + k0, from, stage + (wave * T::LOADS + j) * 1024);
+                    const int row = (wave * T::LOADS + j) * 8;
+                    if (row < T::COLS && piece(row + (lane >> 3)) >= blocks)
+                        *reinterpret_cast<uintx4*>(lds + group * T::GROUP_LDS + stage + row * STEP_BYTES + lane * 16) = uintx4{0, 0, 0, 0};
                 });
-                fetch_scales((step >> 1) + 1, step & 1);
+#pragma unroll
+                for (int p = 0; p < T::SCALE_LOADS; ++p)
+                {
+                    // bytes of the step that this lane's 16 hold, if any: those behind the end
+                    const int first = step % T::G * STEP_SCALES - lane / T::SCALE_ROWS * 16;
+                    if (first < 0 || first >= 16)
+                        continue;
+                    uint32_t* const at = reinterpret_cast<uint32_t*>(lds + group * T::GROUP_LDS + T::S * T::STAGE + (step / T::G & 1) * T::SCALES + scale_to[p] + lane * 16 + first);
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+                    {
+                        const int there = min(max(blocks - 4 * d, 0), 4);
+                        const uint32_t mask = there == 4 ? ~0u : (1u << (8 * there)) - 1;
+                        at[d] = (at[d] & mask) | (ONES & ~mask);
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            };
+            const auto ends_outside = [&](int step) { return (first_step + step + 1) * STEP_BYTES > row_bytes; };
+            constexpr int STEP_LOADS = T::LOADS;
+            // until no more than `steps` steps' loads are under way (scale bytes asked for since then make it wait for more, never for less)
+            const auto landed_but = [&](int steps) {
+                if (T::S > 3 && steps >= 3)
+                    wait_loads<(T::S > 3 ? 3 : 0) * STEP_LOADS>();
+                else if (T::S > 2 && steps == 2)
+                    wait_loads<(T::S > 2 ? 2 : 0) * STEP_LOADS>();
+                else if (steps == 1)
+                    wait_loads<STEP_LOADS>();
+                else
+                    wait_loads<0>();
             };
 
             // ---- what it reads from LDS
@@ -144,21 +188,22 @@ namespace nnf
 #pragma unroll
             for (int s = 0; s < 4; ++s)
             {
-                const uint32_t in_row = r * STEP_BYTES + (((4 * g + s) ^ ((r >> 1) & 7)) << 4);
-                w_at[s] = lds0 + wave_n * T::FN * 32 * STEP_BYTES + in_row;
-                a_at[s] = lds0 + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES + in_row;
+                const auto in_row = [&](int row) { return row * STEP_BYTES + (((4 * g + s) ^ ((row >> 1) & 7)) << 4); };
+                w_at[s] = codes_at + wave_n * T::FN * 32 * STEP_BYTES + in_row(r);
+                a_at[s] = codes_at + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES + in_row(r % T::ROWS);
             }
-            const uint32_t ws_at = lds0 + 2 * T::STAGE + (wave_n * T::FN * 32 + r) * SCALE_BYTES + 4 * g;
-            const uint32_t as_at = lds0 + 2 * T::STAGE + (T::COLS + wave_m * T::FM * 32 + r) * SCALE_BYTES + 4 * g;
+            const auto scale_at = [&](int row) { return scales_at + row / T::SCALE_ROWS * 1024 + row % T::SCALE_ROWS * 16 + 4 * g; };
+            const uint32_t ws_at = scale_at(wave_n * T::FN * 32 + r), as_at = scale_at(T::COLS + wave_m * T::FM * 32 + r % T::ROWS);
+            constexpr int FRAGMENT_SCALES = 32 / T::SCALE_ROWS * 1024; // from one fragment's scale bytes to the next one's
 
             floatx16 sum[T::FN][T::FM] = {};
             uintx4 wf[2][T::FN], af[2][T::FM]; // fragments of an MFMA step and of the next
             uint32_t ws[T::FN], as[T::FM], ws_next[T::FN], as_next[T::FM];
 
             const auto read_scales = [&](int step) {
-                const uint32_t from = (step >> 1) % 3 * T::SCALES + (step & 1) * 8;
-                unroll_for<0, T::FN>([&](auto f) { lds_read_b32_nowait<f * 32 * SCALE_BYTES>(ws_next[f], ws_at + from); });
-                unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * 32 * SCALE_BYTES>(as_next[f], as_at + from); });
+                const uint32_t from = (step / T::G & 1) * T::SCALES + step % T::G / 2 * (T::SCALE_ROWS * 16) + (step & 1) * 8;
+                unroll_for<0, T::FN>([&](auto f) { lds_read_b32_nowait<f * FRAGMENT_SCALES>(ws_next[f], ws_at + from); });
+                unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * FRAGMENT_SCALES>(as_next[f], as_at + from); });
             };
             // fragment f of an MFMA step: weights, then activations
             const auto read_fragment = [&](auto f, auto set, int s, uint32_t stage) {
@@ -177,56 +222,73 @@ namespace nnf
                 unroll_for<0, T::FN>([&](auto f) { lds_wait_also(ws_next[f]); ws[f] = ws_next[f]; });
                 unroll_for<0, T::FM>([&](auto f) { lds_wait_also(as_next[f]); as[f] = as_next[f]; });
             };
-            using Zero = std::integral_constant<int, 0>;
-            using Yes = std::true_type;
-            using No = std::false_type;
 
-            // one step; the next one's first fragments and scale bytes are read during its last MFMAs.  FETCH: ask for the codes of the
-            // step after the next; LAST: that one is the last; END: this one is
-            const auto body = [&](int step, auto do_fetch, auto last, auto end) {
-                const uint32_t stage = (step & 1) * T::STAGE;
-                const int blocks = (row_bytes - step * STEP_BYTES) >> 4; // of this step and behind it
-                if constexpr (end)
-                {
-                    // blocks behind the rows' end: 2^0 times zeros, whatever lies there
-                    const int there = min(max(blocks - 4 * g, 0), 4);
-                    const uint32_t mask = there == 4 ? ~0u : (1u << (8 * there)) - 1;
+            fetch_scales(0);
 #pragma unroll
-                    for (int f = 0; f < T::FN; ++f)
-                        ws[f] = (ws[f] & mask) | (ONES & ~mask);
-#pragma unroll
-                    for (int f = 0; f < T::FM; ++f)
-                        as[f] = (as[f] & mask) | (ONES & ~mask);
-                }
+            for (int i = 0; i < T::S; ++i)
+                if (i < steps)
+                    fetch(i, i * T::STAGE);
+            if (ends_outside(0))
+            {
+                wait_loads<0>();
+                cut(0, 0);
+            }
+            else
+                landed_but(min(T::S, steps) - 1);
+            if constexpr (T::GROUP > 1)
+                asm volatile("s_barrier" ::: "memory");
+            read_scales(0);
+            unroll_for<0, T::FN + T::FM>([&](auto f) { read_fragment(f, std::integral_constant<int, 0>{}, 0, 0); });
+            landed(std::integral_constant<int, 0>{});
+            take_scales();
+            uint32_t stage = 0;
+            // a step; the next one's first fragments and scale bytes are read during its last MFMAs, and what comes S steps later is asked
+            // for where this one's last reads have left room.  FULL: that one ends within the rows, and its loads go out between the MFMAs
+            const auto body = [&](int step, auto full) {
+                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
                 unroll_for<0, 4>([&](auto s) {
                     constexpr int SET = s & 1;
                     using Next = std::integral_constant<int, 1 - SET>;
-                    constexpr bool READS = s < 3 || !end;
-                    if constexpr (end)
+                    if constexpr (s == 3)
                     {
-#pragma unroll
-                        for (int f = 0; f < T::FN; ++f)
-                            wf[SET][f] = 4 * g + s < blocks ? wf[SET][f] : uintx4{0, 0, 0, 0};
-                    }
-                    if constexpr (s == 3 && READS)
-                    {
-                        // every wavefront has read all of this step, all of the next has landed
-                        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-                        if constexpr (do_fetch)
-                            fetch(step + 2, last);
+                        // every wavefront of the group has read all of this step, all of the next has landed
+                        if constexpr (full)
+                            wait_loads<(T::S - 2) * STEP_LOADS>();
+                        else if (step + 1 < steps && ends_outside(step + 1))
+                        {
+                            wait_loads<0>();
+                            cut(step + 1, next_stage);
+                        }
+                        else
+                            landed_but(min(T::S - 2, steps - 2 - step));
+                        if constexpr (T::GROUP > 1)
+                            asm volatile("s_barrier" ::: "memory");
+                        if (step % T::G == 0 && step + T::G < steps)
+                            fetch_scales(step + T::G);
+                        if (!full && step + T::S < steps)
+                            fetch(step + T::S, stage);
                         read_scales(step + 1);
                     }
-                    unroll_for<0, T::FN * T::FM>([&](auto i) {
+                    // (behind the last step: what lies in LDS, not used)
+                    constexpr int MFMAS = T::FN * T::FM;
+                    unroll_for<0, MFMAS>([&](auto i) {
                         constexpr int fn = i / T::FM, fm = i % T::FM;
-                        if constexpr (READS && i < T::FN + T::FM)
-                            read_fragment(i, Next{}, (s + 1) & 3, s < 3 ? stage : T::STAGE - stage);
+                        constexpr int READS = (T::FN + T::FM + MFMAS - 1) / MFMAS, FETCHES = (T::LOADS + MFMAS - 1) / MFMAS; // ahead of each MFMA
+                        unroll_for<0, READS>([&](auto q) {
+                            if constexpr (i * READS + q < T::FN + T::FM)
+                                read_fragment(std::integral_constant<int, i * READS + q>{}, Next{}, (s + 1) & 3, s < 3 ? stage : next_stage);
+                        });
+                        if constexpr (s == 3 && full)
+                            unroll_for<0, FETCHES>([&](auto q) {
+                                if constexpr (i * FETCHES + q < T::LOADS)
+                                    fetch_load(std::integral_constant<int, i * FETCHES + q>{}, step + T::S, stage, std::true_type{});
+                            });
                         sum[fn][fm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf[SET][fn]), operand(af[SET][fm]), sum[fn][fm], FP4, FP4,
                                                                                       s, (int)ws[fn], s, (int)as[fm]);
                         __builtin_amdgcn_sched_barrier(0);
                     });
-                    if constexpr (READS)
-                        landed(Next{});
-                    if constexpr (s == 3 && READS)
+                    landed(Next{});
+                    if constexpr (s == 3)
                         take_scales();
 #pragma unroll
                     for (int fn = 0; fn < T::FN; ++fn)
@@ -234,85 +296,107 @@ namespace nnf
                         for (int fm = 0; fm < T::FM; ++fm)
                             asm volatile("" : "+a"(sum[fn][fm])); // the MFMAs stay where they are written, their sums in AGPRs
                 });
+                stage = next_stage;
             };
-
-            fetch_scales(0, 0);
-            fetch_scales(0, 1);
-            fetch(0, Yes{});
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-            if (steps > 1)
-                fetch(1, Yes{});
-            read_scales(0);
-            unroll_for<0, T::FN>([&](auto f) { read_fragment(f, Zero{}, 0, 0); });
-            unroll_for<T::FN, T::FN + T::FM>([&](auto f) { read_fragment(f, Zero{}, 0, 0); });
-            landed(Zero{});
-            take_scales();
             int step = 0;
-            for (; step < steps - 3; ++step)
-                body(step, Yes{}, No{}, No{});
-            if (steps >= 3)
-                body(step++, Yes{}, Yes{}, No{});
-            if (steps >= 2)
-                body(step++, No{}, No{}, No{});
-            body(step, No{}, No{}, Yes{});
+            const int whole = min(steps, max(row_bytes / STEP_BYTES - first_step, 0)); // steps that end within the rows
+#pragma unroll 1
+            for (; step + T::S < whole; ++step)
+                body(step, std::true_type{});
+#pragma unroll 1
+            for (; step < steps; ++step)
+                body(step, std::false_type{});
 
             // ---- Y: lane l of a fragment has columns 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32.  A block of 32 rows at a time goes through
-            // LDS in fp32 (a part of the wavefront's own) and leaves as whole rows, 16 bytes a lane
+            // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane
             constexpr int FO = GATE ? T::FN / 2 : T::FN; // fragments of columns of Y
-            constexpr int PITCH = FO * 128 + 16, LANES = FO * 4, PASSES = 32 * LANES / WAVE;
-            static_assert(T::WAVES * 32 * PITCH <= T::LDS && WAVE % LANES == 0, "room for the results");
-            uint8_t* const mine = lds + wave * (32 * PITCH);
+            constexpr int LANES = FO * 4, PASSES = 32 * LANES / WAVE, MINE = (PASSES + T::WK - 1) / T::WK;
+            static_assert(32 * LANES % WAVE == 0, "whole passes");
             const int n = n0 + wave_n * FO * 32 + lane % LANES * 8;
+            uint8_t* const block = lds + wave * (32 * T::PITCH); // the first group's; the others' behind it
+            constexpr int PART = T::GROUP * 32 * T::PITCH;
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
             for (int fm = 0; fm < T::FM; ++fm)
             {
+                if (T::WK > 1 && fm > 0)
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-                for (int fn = 0; fn < FO; ++fn)
+                for (int fn = 0; fn < T::FN; ++fn)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                    {
-                        floatx4 y;
+                        *reinterpret_cast<floatx4*>(block + group * PART + r * T::PITCH + fn * 128 + q * 32 + g * 16) =
+                            floatx4{sum[fn][fm][q * 4], sum[fn][fm][q * 4 + 1], sum[fn][fm][q * 4 + 2], sum[fn][fm][q * 4 + 3]};
+                if constexpr (T::WK > 1)
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                floatx4 y[MINE][2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                        {
-                            y[i] = sum[fn][fm][q * 4 + i];
-                            if constexpr (GATE)
-                                y[i] = silu_gate(y[i], sum[fn + FO][fm][q * 4 + i]);
-                        }
-                        *reinterpret_cast<floatx4*>(mine + r * PITCH + fn * 128 + q * 32 + g * 16) = y;
-                    }
-#pragma unroll 1
-                for (int i = 0; i < PASSES; ++i)
+                for (int i = 0; i < MINE; ++i)
                 {
-                    const int row = i * (WAVE / LANES) + lane / LANES, m = rows.first + (wave_m * T::FM + fm) * 32 + row;
-                    const floatx4* const y = reinterpret_cast<const floatx4*>(mine + row * PITCH + lane % LANES * 32);
-                    if (m < rows.end && n < o.N)
-                        write_eight(o, y[0], y[1], m, n);
+                    const uint8_t* const at = block + ((i * T::WK + group) % PASSES * (WAVE / LANES) + lane / LANES) * T::PITCH + lane % LANES * 32;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        y[i][h] = *reinterpret_cast<const floatx4*>(at + h * 16);
+#pragma unroll
+                        for (int k = 1; k < T::WK; ++k)
+                            y[i][h] += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16);
+                        if constexpr (GATE)
+                        {
+                            floatx4 up = *reinterpret_cast<const floatx4*>(at + h * 16 + FO * 128);
+#pragma unroll
+                            for (int k = 1; k < T::WK; ++k)
+                                up += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16 + FO * 128);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[i][h][e] = silu_gate(y[i][h][e], up[e]);
+                        }
+                    }
                 }
+                const int first = rows.first + (wave_m * T::FM + fm) * 32 + lane / LANES;
+                if (n < o.N)
+                    write_rows<MINE>(o, y, n, [&](int i) {
+                        const int pass = i * T::WK + group, m = first + pass * (WAVE / LANES);
+                        return pass < PASSES && m < rows.end && (T::ROWS >= 32 || m < rows.first + T::ROWS) ? m : -1;
+                    });
             }
         }
 
         template <class T, bool GATE>
-        hipError_t launch(hipStream_t s, const Operands& o, int row_blocks)
+        hipError_t launch(hipStream_t s, const Operands& o)
         {
             static LdsGrant granted;
             const hipError_t e = allow_dynamic_lds((const void*)mxfp4_tile_kernel<T, GATE>, granted, T::LDS);
             if (e != hipSuccess)
                 return e;
-            constexpr int OUT = GATE ? T::COLS / 2 : T::COLS;
-            const int col_tiles = (o.N + OUT - 1) / OUT;
-            mxfp4_tile_kernel<T, GATE><<<(unsigned)row_blocks * col_tiles, T::WAVES * WAVE, T::LDS, s>>>(o, col_tiles);
+            const int col_tiles = column_tiles(o.N, T::COLS, GATE);
+            mxfp4_tile_kernel<T, GATE><<<(unsigned)(row_blocks(o, T::ROWS) * col_tiles), T::WAVES * WAVE, T::LDS, s>>>(o, col_tiles);
             return hipGetLastError();
+        }
+        template <class T>
+        hipError_t launch_either(hipStream_t s, const Operands& o, bool gate)
+        {
+            if constexpr (T::FN % 2 == 0)
+                if (gate)
+                    return launch<T, true>(s, o);
+            return gate ? hipErrorInvalidValue : launch<T, false>(s, o);
         }
     } // namespace
 
-    hipError_t launch_mxfp4_tiles(hipStream_t s, const mx::Operands& o, int rows, int row_blocks, bool gate)
+    hipError_t launch_mxfp4_tiles(hipStream_t s, const mx::Operands& o, int kernel, bool gate)
     {
-        if (rows == 256)
-            return gate ? launch<Tile<2, 2, 4, 4>, true>(s, o, row_blocks) : launch<Tile<2, 2, 4, 4>, false>(s, o, row_blocks);
-        if (rows == 128)
-            return gate ? launch<Tile<2, 2, 2, 2>, true>(s, o, row_blocks) : launch<Tile<2, 2, 2, 2>, false>(s, o, row_blocks);
-        return gate ? launch<Tile<1, 4, 2, 2>, true>(s, o, row_blocks) : launch<Tile<1, 4, 2, 2>, false>(s, o, row_blocks);
+        switch (kernel)
+        {
+        case mx::TILE_8x32: return launch_either<Tile<1, 1, 4, 1, 1, 3, 4, 8>>(s, o, gate);
+        case mx::TILE_16x32: return launch_either<Tile<1, 1, 8, 1, 1, 2, 4, 16>>(s, o, gate);
+        case mx::TILE_16x64: return launch_either<Tile<1, 1, 2, 1, 2, 3, 8, 16>>(s, o, gate);
+        case mx::TILE_16x64_DEEP: return launch_either<Tile<1, 1, 1, 1, 2, 4, 16, 16>>(s, o, gate);
+        case mx::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2>>(s, o, gate);
+        case mx::TILE_64x64: return launch_either<Tile<1, 1, 4, 2, 2, 2>>(s, o, gate);
+        case mx::TILE_64x64_DEEP: return launch_either<Tile<2, 2, 1, 1, 1, 4>>(s, o, gate);
+        case mx::TILE_128x128: return launch_either<Tile<2, 2, 1, 2, 2, 2>>(s, o, gate);
+        case mx::TILE_128x128_DEEP: return launch_either<Tile<2, 2, 1, 2, 2, 4>>(s, o, gate);
+        default: return launch_either<Tile<2, 4, 1, 4, 2, 2>>(s, o, gate);
+        }
     }
 } // namespace nnf

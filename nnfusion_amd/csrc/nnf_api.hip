@@ -873,17 +873,18 @@ int nnf_fused_mlp_wna16(nnf_stream_t stream, const void* x, const void* gamma, f
 namespace
 {
     // what the two products have in common; offsets == null: one weight matrix
-    int mxfp4_product(nnf_stream_t stream, const nnf::mx::Operands& o, int act)
+    int mxfp4_product(nnf_stream_t stream, const nnf::mx::Operands& o, int act, int variant)
     {
         if (!o.A || !o.As || !o.W || !o.Ws || !o.Y || o.M <= 0 || o.N <= 0 || o.K <= 0 || o.experts <= 0)
             return NNF_ERR_INVALID_ARGUMENT;
-        if (act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE)
+        if ((act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE) || variant < 0 || variant > nnf::mx::KERNELS)
             return NNF_ERR_INVALID_ARGUMENT;
         if (!aligned16(o.A) || !aligned16(o.As) || !aligned16(o.W) || !aligned16(o.Ws) || !aligned16(o.Y) || !aligned16(o.bias) ||
             !aligned16(o.residual) || !aligned16(o.offsets))
             return NNF_ERR_INVALID_ARGUMENT;
         const bool gate = act == NNF_ACT_SILU_GATE;
-        if (!nnf::mx::supported(o.K) || (gate && (o.bias || o.residual)) || o.N > (1 << 29) || o.M > (1 << 30))
+        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::supported(o.K) || (gate && (o.bias || o.residual)) || o.N > (1 << 29) || o.M > (1 << 30) ||
+            (gate && (size_t)o.N * o.K >= (size_t)1 << 32)) // (byte offsets from a gate row to its up row: 32 bits)
             return NNF_ERR_UNSUPPORTED_SHAPE;
         const size_t y_bytes = (size_t)o.M * o.N * 2, w_rows = (size_t)o.experts * o.N * (gate ? 2 : 1);
         const size_t row = (size_t)o.K / 2, scale_row = nnf::mx::scale_bytes(o.K);
@@ -897,12 +898,12 @@ namespace
         const int st = current_device_info(dev);
         if (st != NNF_OK)
             return st;
-        const nnf::mx::Plan plan = nnf::mx::plan(o.experts, o.M, o.N, o.K, gate, o.offsets != nullptr);
-        // (no tile or block has fewer than 16 columns)
-        if ((long long)plan.row_blocks * ((o.N + 15) / 16) > 0x7FFFFFFFLL)
-            return NNF_ERR_UNSUPPORTED_SHAPE;
-        return (int)(plan.tiles ? nnf::launch_mxfp4_tiles((hipStream_t)stream, o, 1 << plan.row_shift, plan.row_blocks, gate)
-                                : nnf::launch_mxfp4_rows((hipStream_t)stream, o, plan.row_shift, plan.row_blocks, gate));
+        const int kernel = variant != NNF_MXFP4_AUTO ? variant - 1 : nnf::mx::choose(o.M, o.N, o.K, gate, o.offsets ? o.experts : 0, dev.num_cu);
+        const nnf::mx::KernelFacts& facts = nnf::mx::FACTS[kernel];
+        if (nnf::mx::row_blocks(o, facts.rows) * nnf::mx::column_tiles(o.N, facts.cols, gate) > 0x7FFFFFFFLL)
+            return NNF_ERR_UNSUPPORTED_SHAPE; // more workgroups than a grid holds
+        return (int)(kernel <= nnf::mx::ROWS_16x32 ? nnf::launch_mxfp4_rows((hipStream_t)stream, o, kernel, gate)
+                                                   : nnf::launch_mxfp4_tiles((hipStream_t)stream, o, kernel, gate));
     }
 } // namespace
 
@@ -954,13 +955,27 @@ size_t nnf_mxfp4_gemm_workspace_bytes(int M, int N, int K, int act)
     return 0;
 }
 
-int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int M, int N, int K,
-                   const void* bias, const void* residual, int act, void* workspace, size_t workspace_bytes)
+int nnf_mxfp4_variant_supported(int variant, int act)
+{
+    static_assert(NNF_MXFP4_TILE_256x256 == nnf::mx::KERNELS, "variants and kernels in one order, automatic choice first");
+    if (variant < 0 || variant > nnf::mx::KERNELS || (act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE))
+        return 0;
+    return variant == NNF_MXFP4_AUTO || act == NNF_ACT_NONE || nnf::mx::FACTS[variant - 1].gate;
+}
+
+int nnf_mxfp4_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int M, int N, int K,
+                           const void* bias, const void* residual, int act, int variant, void* workspace, size_t workspace_bytes)
 {
     (void)workspace, (void)workspace_bytes;
     return mxfp4_product(stream, {(const uint8_t*)A, (const uint8_t*)a_scales, (const uint8_t*)W, (const uint8_t*)w_scales, (nnf::half_t*)Y,
                                   (const nnf::half_t*)bias, (const nnf::half_t*)residual, nullptr, M, N, K, 1},
-                         act);
+                         act, variant);
+}
+
+int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int M, int N, int K,
+                   const void* bias, const void* residual, int act, void* workspace, size_t workspace_bytes)
+{
+    return nnf_mxfp4_gemm_variant(stream, A, a_scales, W, w_scales, Y, M, N, K, bias, residual, act, NNF_MXFP4_AUTO, workspace, workspace_bytes);
 }
 
 size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, int act)
@@ -969,15 +984,21 @@ size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, 
     return 0;
 }
 
-int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets, void* Y,
-                           int experts, int M, int N, int K, int act, void* workspace, size_t workspace_bytes)
+int nnf_mxfp4_grouped_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets,
+                                   void* Y, int experts, int M, int N, int K, int act, int variant, void* workspace, size_t workspace_bytes)
 {
     (void)workspace, (void)workspace_bytes;
     if (!offsets)
         return NNF_ERR_INVALID_ARGUMENT;
     return mxfp4_product(stream, {(const uint8_t*)A, (const uint8_t*)a_scales, (const uint8_t*)W, (const uint8_t*)w_scales, (nnf::half_t*)Y, nullptr,
                                   nullptr, (const int*)offsets, M, N, K, experts},
-                         act);
+                         act, variant);
+}
+
+int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets, void* Y,
+                           int experts, int M, int N, int K, int act, void* workspace, size_t workspace_bytes)
+{
+    return nnf_mxfp4_grouped_gemm_variant(stream, A, a_scales, W, w_scales, offsets, Y, experts, M, N, K, act, NNF_MXFP4_AUTO, workspace, workspace_bytes);
 }
 
 } // extern "C"

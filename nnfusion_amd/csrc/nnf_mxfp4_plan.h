@@ -1,4 +1,4 @@
-// Which kernel serves an MXFP4 product and what it needs: shared by the library and the emitters (host arithmetic only).
+// Which kernel serves an MXFP4 product: shared by the library and the emitters (host arithmetic only).
 #pragma once
 
 #include <stddef.h>
@@ -8,28 +8,99 @@ namespace nnf
     namespace mx
     {
         constexpr int MAX_K = 1 << 22; // byte offsets inside a tile of 256 rows stay below 2^31
+        // bytes from one row of scale bytes to the next: K / 32 rounded up to 16, so that every row starts on 16 bytes
         constexpr int scale_bytes(int K) { return ((K >> 5) + 15) & ~15; }
         constexpr bool supported(int K) { return K > 0 && K % 32 == 0 && K <= MAX_K; }
 
-        struct Plan
+        // blocks of `rows` rows that there are at most, of M rows in `experts` groups (0: one product): every group may end in a block of its
+        // own, which has a row at least
+        constexpr long long most_row_blocks(int M, int experts, int rows)
         {
-            bool tiles;     // the kernel through LDS (else: the one for a few rows)
-            int row_shift;  // log2 of the rows of a block
-            int row_blocks; // that there are at most
+            const long long groups = experts == 0 ? 1 : experts < M ? experts : M;
+            return (M + groups * (rows - 1)) / rows;
+        }
+        // tiles of columns of Y, `cols` weight rows each
+        constexpr int column_tiles(int N, int cols, bool gate) { return (int)(((long long)N + (gate ? cols / 2 : cols) - 1) / (gate ? cols / 2 : cols)); }
+
+        // activation rows x weight rows of a workgroup's tile.  DEEP: more steps of K under way, fewer wavefronts or workgroups a CU
+        enum Kernel
+        {
+            ROWS_16x16, // operands straight into registers, eight ranges of K
+            ROWS_16x32, // four
+            TILE_8x32,  // through LDS, a wavefront for each range of K: four
+            TILE_16x32, // eight
+            TILE_16x64, // two
+            TILE_16x64_DEEP, // one
+            TILE_32x64, // four
+            TILE_64x64, // four
+            TILE_64x64_DEEP, // through LDS, the wavefronts share the tile and all of K
+            TILE_128x128,
+            TILE_128x128_DEEP,
+            TILE_256x256,
+            KERNELS
         };
 
-        inline Plan plan(int experts, int M, int N, int K, bool gate, bool grouped)
+        // What is known of a kernel: its tile, ranges of K, workgroups that a CU holds at once, values of a step of K, whether it has a
+        // form with SiLU-gate, and the constants of its time in us,
+        //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps, wait * rounds * steps) * (1 + off)
+        // with the rounds of workgroups that a CU runs and `off` where rows of codes do not start on lines of memory (K no multiple of
+        // 256).  Fitted to 1900 timings on one MI355X (12 weight matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192, read from HBM, 1 to
+        // 2048 rows): each within 5 .. 16 % (rms); what they choose takes 1.02 times as long as the best of the twelve kernels, on average.
+        struct KernelFacts
         {
-            (void)N, (void)K, (void)gate;
-            const long long mean = grouped ? ((long long)M + experts - 1) / experts : M;
-            Plan p = {};
-            p.tiles = mean > 64;
-            p.row_shift = p.tiles ? (mean > 1024 ? 8 : mean > 64 ? 7 : 6) : mean > 32 ? 6 : mean > 16 ? 5 : 4;
-            // every group may end in a block of its own, which has a row at least
-            const long long rows = 1LL << p.row_shift;
-            const long long blocks = grouped ? (M + (long long)(experts < M ? experts : M) * (rows - 1)) / rows : (M + rows - 1) / rows;
-            p.row_blocks = (int)blocks;
-            return p;
+            int rows, cols, ranges, per_cu, step_values;
+            bool gate;
+            float start, turn, step, wait, off;
+        };
+        constexpr KernelFacts FACTS[KERNELS] = {
+            {16, 16, 8, 3, 128, false, 2.47f, 0.94f, 0.815f, 0.845f, 0.20f},  {16, 32, 4, 5, 128, true, 2.42f, 0.00f, 0.689f, 0.704f, 0.30f},
+            {8, 32, 4, 2, 256, false, 3.53f, 0.60f, 0.418f, 0.470f, 0.50f},   {16, 32, 8, 1, 256, false, 3.31f, 1.80f, 0.780f, 1.162f, 0.24f},
+            {16, 64, 2, 2, 256, true, 3.58f, 0.25f, 0.420f, 0.447f, 0.71f},   {16, 64, 1, 2, 256, true, 3.69f, 2.20f, 0.208f, 0.354f, 0.40f},
+            {32, 64, 4, 1, 256, true, 3.15f, 1.69f, 0.605f, 1.031f, 0.32f},   {64, 64, 4, 1, 256, true, 4.09f, 2.65f, 0.631f, 1.177f, 0.32f},
+            {64, 64, 1, 2, 256, false, 3.69f, 0.34f, 0.308f, 0.315f, 0.50f},  {128, 128, 1, 2, 256, true, 3.63f, 2.33f, 0.685f, 0.829f, 0.42f},
+            {128, 128, 1, 1, 256, true, 4.58f, 4.57f, 0.618f, 0.636f, 0.62f}, {256, 256, 1, 1, 256, true, 5.70f, 13.56f, 1.414f, 0.848f, 0.54f},
+        };
+
+        // estimated time; experts == 0: one product, else M rows in that many groups, whose sizes are not known here
+        inline float estimate(const KernelFacts& k, int M, int N, int K, bool gate, int experts, int num_cu)
+        {
+            // blocks of rows: a group ends in a block that is half full on average, and groups are of about one size
+            double blocks = (double)((M + k.rows - 1) / k.rows);
+            if (experts > 0)
+            {
+                const int groups = experts < M ? experts : M;
+                blocks = groups * ((double)M / groups / k.rows + 0.5);
+                if (blocks < groups)
+                    blocks = groups;
+            }
+            const int all_steps = (K + k.step_values - 1) / k.step_values;
+            int steps = (all_steps + k.ranges - 1) / k.ranges;
+            if (k.step_values == 256 && k.ranges > 1)
+            {
+                steps = (steps + 1) & ~1;
+                if (steps > all_steps)
+                    steps = all_steps;
+            }
+            const double a_cu = blocks * column_tiles(N, k.cols, gate) / num_cu;
+            const double most = (double)(long long)(a_cu + 0.999999), rounds = (double)(long long)((most + k.per_cu - 1) / k.per_cu);
+            const double work = most * steps * k.step, wait = rounds * steps * k.wait;
+            return (float)(k.start + k.turn * (rounds - 1) + (work > wait ? work : wait) * (K % 256 ? 1 + k.off : 1));
+        }
+
+        // the kernel with the lowest estimate
+        inline Kernel choose(int M, int N, int K, bool gate, int experts, int num_cu)
+        {
+            int best = -1;
+            float time = 0;
+            for (int k = 0; k < KERNELS; ++k)
+            {
+                if (gate && !FACTS[k].gate)
+                    continue;
+                const float t = estimate(FACTS[k], M, N, K, gate, experts, num_cu);
+                if (best < 0 || t < time)
+                    best = k, time = t;
+            }
+            return (Kernel)best;
         }
     } // namespace mx
 } // namespace nnf

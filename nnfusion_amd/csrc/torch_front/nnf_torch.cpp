@@ -450,7 +450,7 @@ namespace
         return size32(act == NNF_ACT_SILU_GATE ? rows / 2 : rows);
     }
 
-    // (a, a_scales, w, w_scales, bias, residual, act, out, workspace)
+    // (a, a_scales, w, w_scales, bias, residual, act, out, workspace, variant)
     PyObject* mxfp4_gemm(Args v)
     {
         const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]);
@@ -470,12 +470,12 @@ namespace
         const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
         Owned y(output(v[7], {m, n}, at::kHalf, a, "out"));
         Workspace space(v[8], a, [&] { return nnf_mxfp4_gemm_workspace_bytes(m, n, k, act); });
-        call("nnf_mxfp4_gemm", nnf_mxfp4_gemm, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data(), m, n, k, address(v[4]),
-             address(v[5]), act, space.data, space.bytes);
+        call("nnf_mxfp4_gemm", nnf_mxfp4_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data(), m, n, k, address(v[4]),
+             address(v[5]), act, integer(v[9]), space.data, space.bytes);
         return y.release();
     }
 
-    // (a, a_scales, w, w_scales, offsets, act, out, workspace)
+    // (a, a_scales, w, w_scales, offsets, act, out, workspace, variant)
     PyObject* mxfp4_grouped_gemm(Args v)
     {
         const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]), &offsets = tensor(v[4]);
@@ -494,8 +494,8 @@ namespace
         const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
         Owned y(output(v[6], {m, n}, at::kHalf, a, "out"));
         Workspace space(v[7], a, [&] { return nnf_mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act); });
-        call("nnf_mxfp4_grouped_gemm", nnf_mxfp4_grouped_gemm, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), offsets.data_ptr(),
-             y.data(), experts, m, n, k, act, space.data, space.bytes);
+        call("nnf_mxfp4_grouped_gemm", nnf_mxfp4_grouped_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), offsets.data_ptr(),
+             y.data(), experts, m, n, k, act, integer(v[8]), space.data, space.bytes);
         return y.release();
     }
 
@@ -533,7 +533,7 @@ namespace
     PyMethodDef methods[] = {NNF_ENTRY(w4a16_gemm, 7),       NNF_ENTRY(wna16_gemm, 11),      NNF_ENTRY(w4a16_gemm_fused, 14), NNF_ENTRY(fused_mlp_w4a16, 13),
                              NNF_ENTRY(wna16_gemm_fused, 14), NNF_ENTRY(fused_mlp_wna16, 14), NNF_ENTRY(w8a8_gemm, 7),         NNF_ENTRY(w8a8_gemm_acc, 5),
                              NNF_ENTRY(elementwise, 4),       NNF_ENTRY(rms_norm, 4),         NNF_ENTRY(dequantize, 7),        NNF_ENTRY(mxfp4_quantize, 4),
-                             NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 9),        NNF_ENTRY(mxfp4_grouped_gemm, 8), {"set_error", set_error, METH_O, nullptr},
+                             NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 10),        NNF_ENTRY(mxfp4_grouped_gemm, 9), {"set_error", set_error, METH_O, nullptr},
                              {nullptr, nullptr, 0, nullptr}};
     PyModuleDef module = {PyModuleDef_HEAD_INIT, "nnf_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

@@ -285,15 +285,25 @@ def mxfp4_dequantize(codes, scales, out=None):
     return _native.mxfp4_dequantize(codes, scales, out)
 
 
+MXFP4_VARIANTS = {name: i for i, name in enumerate((
+    "auto", "rows_16x16", "rows_16x32", "tile_8x32", "tile_16x32", "tile_16x64", "tile_16x64_deep", "tile_32x64", "tile_64x64", "tile_64x64_deep",
+    "tile_128x128", "tile_128x128_deep", "tile_256x256"))}
+
+
+def mxfp4_variant_supported(variant, act=0):
+    return bool(_lib.kernels().nnf_mxfp4_variant_supported(MXFP4_VARIANTS[variant], act))
+
+
 def mxfp4_gemm_workspace_bytes(m, n, k, act=0):
     """Bytes of workspace mxfp4_gemm wants for this product (0: none)."""
     return int(_lib.kernels().nnf_mxfp4_gemm_workspace_bytes(m, n, k, act))
 
 
-def mxfp4_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, workspace=None):
+def mxfp4_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, workspace=None, variant="auto"):
     """Y fp16 [M,N] = A . W^T (+ bias + residual) of MXFP4 operands (see mxfp4_quantize), or with act=1 SiLU(gate) * up where w holds
-    the gate rows, then the up rows.  fp32 sums, one rounding at the end.  out may be the residual."""
-    return _native.mxfp4_gemm(a, a_scales, w, w_scales, bias, residual, act, out, workspace)
+    the gate rows, then the up rows.  fp32 sums, one rounding at the end.  out may be the residual.  variant: one kernel
+    (a key of MXFP4_VARIANTS) instead of the library's choice."""
+    return _native.mxfp4_gemm(a, a_scales, w, w_scales, bias, residual, act, out, workspace, MXFP4_VARIANTS[variant])
 
 
 def mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act=0):
@@ -301,8 +311,8 @@ def mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act=0):
     return int(_lib.kernels().nnf_mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act))
 
 
-def mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, workspace=None):
+def mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, workspace=None, variant="auto"):
     """The product of a mixture's experts: rows of a sorted by expert, w u8 [experts, N, K/2] (2N rows with act=1, SiLU-gate), w_scales
     u8 [experts, N, mxfp4_scale_bytes(K)]; group e is the rows offsets[e] .. offsets[e+1] (offsets i32 [experts+1], on the device, not
     decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here)."""
-    return _native.mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, workspace)
+    return _native.mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, workspace, MXFP4_VARIANTS[variant])

@@ -126,7 +126,7 @@ def _check(y, want, tol):
     assert not over.any(), (int(over.sum()), over.nonzero()[:5].tolist(), float(((y - want).abs() / tol).max()))
 
 
-def _product_case(gpu, gen, m, n, k, bias=False, residual=False, gate=False):
+def _product_case(gpu, gen, m, n, k, bias=False, residual=False, gate=False, variant="auto"):
     a, a_s = _codes(gen, m, k)
     w, w_s = _codes(gen, n * (2 if gate else 1), k, 112, 124)
     b = _normal(gen, n) if bias else None
@@ -134,7 +134,7 @@ def _product_case(gpu, gen, m, n, k, bias=False, residual=False, gate=False):
     room = torch.full((m + 2, n), 9.0, dtype=torch.float16, device=gpu) if n % 8 == 0 else None
     out = room[1 : m + 1] if room is not None else None
     ga, gas, gw, gws, gb, gr = _gpu(gpu, a, a_s, w, w_s, b, r)
-    y = ops.mxfp4_gemm(ga, gas, gw, gws, bias=gb, residual=gr, act=1 if gate else 0, out=out)
+    y = ops.mxfp4_gemm(ga, gas, gw, gws, bias=gb, residual=gr, act=1 if gate else 0, out=out, variant=variant)
     va, vw = ref.values(a, a_s), ref.values(w, w_s)
     if gate:
         (g, gm), (u, um) = ref.product(va, vw[:n]), ref.product(va, vw[n:])
@@ -264,10 +264,65 @@ def test_same_call_same_bits(gpu, m, n, k):
         assert _equal_bits(first, ops.mxfp4_gemm(*operands))
 
 
+VARIANTS = [v for v in ops.MXFP4_VARIANTS if v != "auto"]
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_every_kernel_on_shapes_of_any_size(gpu, variant):
+    """Each kernel behind the product: one row and more rows than its tile, columns and K that end inside a tile, a step, a
+    pair of steps, a range of K, K shorter than the ranges."""
+    for m, n, k in ((1, 1, 32), (7, 40, 64), (9, 33, 96), (16, 64, 256), (17, 70, 288), (33, 130, 512), (65, 129, 544), (130, 260, 1024), (260, 300, 736),
+                    (20, 24, 1248), (40, 72, 2080), (3, 56, 4096), (300, 264, 2336), (12, 16, 11008), (8, 104, 8160)):
+        _product_case(gpu, _gen(m * 7 + n), m, n, k, bias=n % 2 == 0, residual=m % 2 == 1, variant=variant)
+        if ops.mxfp4_variant_supported(variant, 1):
+            _product_case(gpu, _gen(m * 7 + n + 1), m, n, k, gate=True, variant=variant)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_every_kernel_exactly_and_with_what_is_not_a_number(gpu, variant):
+    gen = _gen(31)
+    m, n, k = 70, 150, 1056
+    pick = torch.tensor([0, 2, 4, 10, 12, 0, 0, 0], dtype=torch.uint8)
+
+    def matrix(rows):
+        c = pick[torch.randint(0, 8, (rows, k // 2, 2), generator=gen)]
+        scales = torch.full((rows, ref.scale_bytes(k)), 255, dtype=torch.uint8)
+        scales[:, : k // 32] = 127
+        return c[..., 0] | c[..., 1] << 4, scales
+
+    a, w = matrix(m), matrix(n)
+    y = ops.mxfp4_gemm(*_gpu(gpu, *a, *w), variant=variant).cpu().double()
+    want = ref.values(*a) @ ref.values(*w).T
+    assert want.abs().max() < 2048 and torch.equal(y, want)
+    a[1][13, 32] = 255  # the last block
+    w[1][149, 0] = 255
+    w[1][64, 17] = 255
+    y = torch.isnan(ops.mxfp4_gemm(*_gpu(gpu, *a, *w), variant=variant).cpu())
+    want = torch.zeros((m, n), dtype=torch.bool)
+    want[13], want[:, 149], want[:, 64] = True, True, True
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_every_kernel_grouped(gpu, variant):
+    for sizes, n, k in (([1, 0, 3], 40, 96), ([20, 0, 0, 17, 1], 70, 544), ([130, 5, 0, 260], 136, 768), ([0, 0, 9], 33, 2080), ([2] * 70, 24, 256)):
+        _grouped_case(gpu, _gen(n), sizes, n, k, first=3, behind=9, variant=variant)
+        if ops.mxfp4_variant_supported(variant, 1):
+            _grouped_case(gpu, _gen(n + 1), sizes, n, k, gate=True, first=1, behind=70, variant=variant)
+
+
+@pytest.mark.parametrize("variant", [v for v in ops.MXFP4_VARIANTS if not ops.mxfp4_variant_supported(v, 1)])
+def test_kernels_without_a_gate_refuse_it(gpu, variant):
+    a, w = _codes(_gen(1), 4, 64), _codes(_gen(2), 32, 64)
+    with pytest.raises(ops.NnfError) as e:
+        ops.mxfp4_gemm(*_gpu(gpu, *a, *w), act=1, variant=variant)
+    assert e.value.status == -2
+
+
 # ---- grouped by expert -------------------------------------------------------------------------------------------------------------
 
 
-def _grouped_case(gpu, gen, sizes, n, k, gate=False, first=0, behind=0):
+def _grouped_case(gpu, gen, sizes, n, k, gate=False, first=0, behind=0, variant="auto"):
     experts, rows = len(sizes), n * (2 if gate else 1)
     m = first + sum(sizes) + behind
     a, a_s = _codes(gen, m, k)
@@ -277,7 +332,7 @@ def _grouped_case(gpu, gen, sizes, n, k, gate=False, first=0, behind=0):
     for s in sizes:
         at.append(at[-1] + s)
     out = torch.full((m, n), 5.0, dtype=torch.float16, device=gpu)
-    y = ops.mxfp4_grouped_gemm(*_gpu(gpu, a, a_s, w, w_s, torch.tensor(at, dtype=torch.int32)), act=1 if gate else 0, out=out)
+    y = ops.mxfp4_grouped_gemm(*_gpu(gpu, a, a_s, w, w_s, torch.tensor(at, dtype=torch.int32)), act=1 if gate else 0, out=out, variant=variant)
     assert y.data_ptr() == out.data_ptr()
     y = y.cpu()
     assert (y[:first] == 5).all() and (y[at[-1] :] == 5).all()
@@ -329,14 +384,15 @@ def test_no_rows_in_any_group(gpu, rows):
     assert (out == 5).all()
 
 
+@pytest.mark.parametrize("variant", list(ops.MXFP4_VARIANTS))
 @pytest.mark.parametrize("offsets", [[-7, 3, 900, 5], [9, 4, 2, 1], [0, 2**31 - 1, -(2**31), 3], [50, 60, 70, 80], [-5, -4, -3, -2]])
-def test_offsets_out_of_order_stay_inside_the_operands(gpu, offsets):
+def test_offsets_out_of_order_stay_inside_the_operands(gpu, offsets, variant):
     """What comes out is undefined; rows of Y's neighbours are not touched and the call ends."""
     gen = _gen(1)
     a, a_s = _codes(gen, 20, 64)
     w, w_s = _codes(gen, 3 * 32, 64)
     room = torch.full((60, 32), 5.0, dtype=torch.float16, device=gpu)
-    ops.mxfp4_grouped_gemm(*_gpu(gpu, a, a_s, w.view(3, 32, 32), w_s.view(3, 32, 16), torch.tensor(offsets, dtype=torch.int32)), out=room[20:40])
+    ops.mxfp4_grouped_gemm(*_gpu(gpu, a, a_s, w.view(3, 32, 32), w_s.view(3, 32, 16), torch.tensor(offsets, dtype=torch.int32)), out=room[20:40], variant=variant)
     torch.cuda.synchronize()
     assert (room[:20] == 5).all() and (room[40:] == 5).all()
 
