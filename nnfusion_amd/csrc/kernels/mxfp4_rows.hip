@@ -4,7 +4,7 @@
 // wavefronts cut K into as many ranges, each with the whole tile's sums in registers, which meet in LDS at the end.
 // v_mfma_scale_f32_16x16x128: lane l holds 32 values of row l % 16, the (l / 16)-th block of the step's four, so a load of 16 bytes a
 // lane covers 64 contiguous bytes of each of 16 rows; the row's four scale bytes of the step are one word, from which each lane takes
-// its own.  The weights are the A operand: a lane then has four consecutive columns of one row of Y.
+// its own (the memory pipeline's time goes by the lines that a load touches: the words of four steps are one load).  The weights are the A operand: a lane then has four consecutive columns of one row of Y.
 #include "mxfp4.h"
 #include "mxfp4_launch.h"
 #include "nnf_launch.h"
@@ -54,23 +54,33 @@ namespace nnf
             // and the weights count as zeros, times 2^0 of both operands
             const auto batch = [&](int step, auto count, auto last) {
                 constexpr int C = count;
-                uintx4 wv[TW][C], av[C];
-                uint32_t wsv[TW][C], asv[C];
-                const int outside = last ? g * 16 : 0; // bytes back to the first block
+                uintx4 wv[TW][C], av[C], wsv[TW], asv;
                 const bool there = (step + C - 1) * 64 + g * 16 < row_bytes;
+                const uint32_t back = last && !there ? g * 16 : 0; // bytes back to the first block
+                // the scale bytes of the batch are one load of 16 bytes a row, as far as the row's (padded) end lets it begin there: `skip` words
+                // of it belong to the steps before
+                const int scale_from = min(step * 4, scale_stride - 16), skip = step - scale_from / 4;
+#pragma unroll
+                for (int t = 0; t < TW; ++t)
+                    wsv[t] = *reinterpret_cast<const uintx4*>(ws_base + scale_from + ws[t]);
+                asv = *reinterpret_cast<const uintx4*>(as_base + scale_from + as);
 #pragma unroll
                 for (int s = 0; s < C; ++s)
                 {
-                    const int at = (step + s) * 64;
-                    const uint32_t back = last && s == C - 1 && !there ? outside : 0;
 #pragma unroll
                     for (int t = 0; t < TW; ++t)
-                    {
-                        wv[t][s] = *reinterpret_cast<const uintx4*>(w_base + at + (w[t] - back));
-                        wsv[t][s] = *reinterpret_cast<const uint32_t*>(ws_base + (at >> 4) + ws[t]);
-                    }
-                    av[s] = *reinterpret_cast<const uintx4*>(a_base + at + (a - back));
-                    asv[s] = *reinterpret_cast<const uint32_t*>(as_base + (at >> 4) + as);
+                        wv[t][s] = *reinterpret_cast<const uintx4*>(w_base + (step + s) * 64 + (w[t] - (s == C - 1 ? back : 0)));
+                    av[s] = *reinterpret_cast<const uintx4*>(a_base + (step + s) * 64 + (a - (s == C - 1 ? back : 0)));
+                }
+                if (skip)
+                {
+                    const auto moved = [&](uintx4 v) {
+                        return skip == 1 ? uintx4{v.y, v.z, v.w, ONES} : skip == 2 ? uintx4{v.z, v.w, ONES, ONES} : uintx4{v.w, ONES, ONES, ONES};
+                    };
+#pragma unroll
+                    for (int t = 0; t < TW; ++t)
+                        wsv[t] = moved(wsv[t]);
+                    asv = moved(asv);
                 }
                 if constexpr (last)
                 {

@@ -44,8 +44,10 @@ namespace nnf
         // form with SiLU-gate, and the constants of its time in us,
         //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps, wait * rounds * steps) * (1 + off)
         // with the rounds of workgroups that a CU runs and `off` where rows of codes do not start on lines of memory (K no multiple of
-        // 256).  Fitted to 1900 timings on one MI355X (12 weight matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192, read from HBM, 1 to
-        // 2048 rows): each within 5 .. 16 % (rms); what they choose takes 1.02 times as long as the best of the twelve kernels, on average.
+        // 256).  Fitted to 6700 timings on one MI355X (weights read from HBM: 16 matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192
+        // with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and uneven, each with and without SiLU-gate): 15 .. 24 %
+        // (rms) from each; what they choose takes 1.02 (one matrix) and 1.03 (a mixture) times as long as the best of the kernels on
+        // average, at most 1.5 times (12288 x 1056 with 24 .. 64 rows).
         struct KernelFacts
         {
             int rows, cols, ranges, per_cu, step_values;
@@ -53,12 +55,18 @@ namespace nnf
             float start, turn, step, wait, off;
         };
         constexpr KernelFacts FACTS[KERNELS] = {
-            {16, 16, 8, 3, 128, false, 2.47f, 0.94f, 0.815f, 0.845f, 0.20f},  {16, 32, 4, 5, 128, true, 2.42f, 0.00f, 0.689f, 0.704f, 0.30f},
-            {8, 32, 4, 2, 256, false, 3.53f, 0.60f, 0.418f, 0.470f, 0.50f},   {16, 32, 8, 1, 256, false, 3.31f, 1.80f, 0.780f, 1.162f, 0.24f},
-            {16, 64, 2, 2, 256, true, 3.58f, 0.25f, 0.420f, 0.447f, 0.71f},   {16, 64, 1, 2, 256, true, 3.69f, 2.20f, 0.208f, 0.354f, 0.40f},
-            {32, 64, 4, 1, 256, true, 3.15f, 1.69f, 0.605f, 1.031f, 0.32f},   {64, 64, 4, 1, 256, true, 4.09f, 2.65f, 0.631f, 1.177f, 0.32f},
-            {64, 64, 1, 2, 256, false, 3.69f, 0.34f, 0.308f, 0.315f, 0.50f},  {128, 128, 1, 2, 256, true, 3.63f, 2.33f, 0.685f, 0.829f, 0.42f},
-            {128, 128, 1, 1, 256, true, 4.58f, 4.57f, 0.618f, 0.636f, 0.62f}, {256, 256, 1, 1, 256, true, 5.70f, 13.56f, 1.414f, 0.848f, 0.54f},
+            {16, 16, 8, 3, 128, false, 2.80f, 1.11f, 0.465f, 0.607f, 0.00f},
+            {16, 32, 4, 5, 128, true, 2.82f, 0.87f, 0.388f, 0.331f, 0.00f},
+            {8, 32, 4, 2, 256, false, 3.83f, 1.64f, 0.404f, 0.422f, 0.22f},
+            {16, 32, 8, 1, 256, false, 3.49f, 2.02f, 1.117f, 1.137f, 0.07f},
+            {16, 64, 2, 2, 256, true, 4.14f, 2.14f, 0.404f, 0.424f, 0.27f},
+            {16, 64, 1, 2, 256, true, 4.06f, 2.64f, 0.226f, 0.355f, 0.18f},
+            {32, 64, 4, 1, 256, true, 3.69f, 2.46f, 0.293f, 1.012f, 0.13f},
+            {64, 64, 4, 1, 256, true, 4.71f, 3.33f, 0.732f, 1.143f, 0.18f},
+            {64, 64, 1, 2, 256, false, 3.95f, 1.98f, 0.291f, 0.305f, 0.16f},
+            {128, 128, 1, 2, 256, true, 4.58f, 4.87f, 0.678f, 0.808f, 0.12f},
+            {128, 128, 1, 1, 256, true, 5.22f, 5.03f, 0.566f, 0.637f, 0.21f},
+            {256, 256, 1, 1, 256, true, 7.57f, 14.47f, 0.148f, 1.449f, 0.13f},
         };
 
         // estimated time; experts == 0: one product, else M rows in that many groups, whose sizes are not known here

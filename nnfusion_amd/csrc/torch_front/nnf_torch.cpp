@@ -388,6 +388,8 @@ namespace
             return o;
         }
     };
+    // (no MXFP4 kernel needs a workspace: none is allocated for a caller that brings none)
+    size_t bytes_of(PyObject* o) { return o == Py_None ? 0 : (size_t)tensor(o).nbytes(); }
     void workspace_checked(PyObject* o) { require(o == Py_None || (tensor(o).scalar_type() == at::kByte && tensor(o).is_contiguous()), "workspace: contiguous uint8"); }
 
     // (x, rows, codes, scales) -> (codes, scales)
@@ -469,9 +471,8 @@ namespace
         on_device(a, {v[1], v[2], v[3], v[4], v[5], v[7], v[8]});
         const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
         Owned y(output(v[7], {m, n}, at::kHalf, a, "out"));
-        Workspace space(v[8], a, [&] { return nnf_mxfp4_gemm_workspace_bytes(m, n, k, act); });
         call("nnf_mxfp4_gemm", nnf_mxfp4_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data(), m, n, k, address(v[4]),
-             address(v[5]), act, integer(v[9]), space.data, space.bytes);
+             address(v[5]), act, integer(v[9]), address(v[8]), bytes_of(v[8]));
         return y.release();
     }
 
@@ -493,9 +494,8 @@ namespace
         on_device(a, {v[1], v[2], v[3], v[4], v[6], v[7]});
         const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
         Owned y(output(v[6], {m, n}, at::kHalf, a, "out"));
-        Workspace space(v[7], a, [&] { return nnf_mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act); });
         call("nnf_mxfp4_grouped_gemm", nnf_mxfp4_grouped_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), offsets.data_ptr(),
-             y.data(), experts, m, n, k, act, integer(v[8]), space.data, space.bytes);
+             y.data(), experts, m, n, k, act, integer(v[8]), address(v[7]), bytes_of(v[7]));
         return y.release();
     }
 
