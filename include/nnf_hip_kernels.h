@@ -411,15 +411,18 @@ NNF_API int nnf_fused_mlp_wna16(nnf_stream_t stream,
  *   scales  u8 [rows, nnf_mxfp4_scale_bytes(K)]   byte b of a row: the values 32 b .. 32 b + 31 are times 2^(byte - 127); 255: all of
  *                            them are NaN.  A row is padded to a multiple of 16 bytes (K a multiple of 512: none), written
  *                            as 127 by nnf_mxfp4_quantize_f16 and read by nobody's arithmetic.
- * K a multiple of 32 (NNF_ERR_UNSUPPORTED_SHAPE otherwise and above 2^22).  Products of two values are exact, sums are fp32 and the
- * result is rounded once, behind bias, residual or SiLU-gate.  No function here needs synchronisation words or keeps state.
+ * K a multiple of 32 (NNF_ERR_UNSUPPORTED_SHAPE otherwise and above 2^22).  Products of two values and sums are fp32 (scales so far
+ * from 1 that a product of two values leaves fp32's range give 0 or an infinity there) and the result is rounded once, behind
+ * bias, residual or SiLU-gate.  Every size is at least 1.  No function here needs synchronisation words or keeps state, the same
+ * call gives the same bits, and what belongs to one row or column of a product does not touch another.
  * ------------------------------------------------------------------------------------------- */
 NNF_API int nnf_mxfp4_scale_bytes(int K);
 
 /* x fp16 [source_rows, K] -> codes and scales of `rows` rows: row i is x's row index[i] (i32 [rows] on the device; zeros where
  * x has no such row), or x's row i where index is NULL (then rows == source_rows).  A block's exponent is floor(log2(largest
  * magnitude)) - 2, its values are rounded to the nearest (ties to the even code) and saturate at 6; a block of zeros has
- * byte 127, a block with an infinity or NaN byte 255 and zero codes. */
+ * byte 127, a block with an infinity or NaN byte 255 and zero codes.  The results must not overlap each other, x or index;
+ * rows * ceil(K / 512) up to 2^28 - 16 (NNF_ERR_UNSUPPORTED_SHAPE above; nnf_mxfp4_dequantize_f16 likewise). */
 NNF_API int nnf_mxfp4_quantize_f16(nnf_stream_t stream, const void* x, const void* index, void* codes, void* scales,
                            int rows, int source_rows, int K);
 /* y fp16 [rows, K]: the values, each rounded once (+-inf beyond fp16). */
@@ -427,7 +430,8 @@ NNF_API int nnf_mxfp4_dequantize_f16(nnf_stream_t stream, const void* codes, con
 
 /* Y fp16 [M, N] = A . W^T + bias + residual, or with act == NNF_ACT_SILU_GATE (W has 2N rows: gate rows, then up rows; no bias,
  * no residual) SiLU(gate) * up.  bias fp16 [N] and residual fp16 [M, N] may be NULL; the residual may be Y itself.  Y must not
- * overlap the operands otherwise. */
+ * overlap the operands otherwise.  NNF_ERR_UNSUPPORTED_SHAPE: N above 2^29, M above 2^30, N * K of 2^32 or more with SiLU-gate,
+ * more tiles than a grid holds (2^23 of the kernel's; the automatic choice passes over kernels with too small tiles). */
 NNF_API size_t nnf_mxfp4_gemm_workspace_bytes(int M, int N, int K, int act);
 NNF_API int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y,
                    int M, int N, int K, const void* bias, const void* residual, int act,

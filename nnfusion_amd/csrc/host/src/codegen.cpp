@@ -603,7 +603,7 @@ namespace nnfusion
             NNFUSION_CHECK(unserved.empty())
                 << "no " << get_device_str(ROCM_GPU) << " kernel for: " << unserved
                 << "; the quantized fusion passes did not absorb these operators, and only QuantDot, QuantDotW8A8, "
-                   "FusedQuantMLP and Slice have emitters";
+                   "FusedQuantMLP, Slice and the Mx operators have emitters";
         }
         auto tu = visit_graph(graph);
         auto ctx = std::make_shared<InterpreterContext>();

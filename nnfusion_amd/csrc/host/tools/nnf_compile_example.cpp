@@ -13,11 +13,14 @@
 //                                                         Swish, Multiply, Add; the fusion pass folds it into one node)
 //   nnf_compile_example qkv_graph <out_dir> M N K       (RMSNorm feeding three QuantDots of N rows each; merged
 //                                                         into one 3N-row QuantDot + three Slices; three results)
+//   nnf_compile_example mx_experts <out_dir> M H I       (a mixture of four experts on MXFP4: rows picked by an index are quantised,
+//                                                         gate | up with SiLU-gate, quantised, down; x, index, offsets are inputs)
 // every form: [include_dir lib_dir [kernel_profiling_dir [prepare]]] at the end; a kernel_profiling_dir switches
 // profiling-based kernel selection on (every candidate kernel of a QuantDot node is timed on the GPU)
 //   nnf_compile_example onnx      <out_dir> <model.onnx> [include_dir lib_dir]
 //                                                        (an ONNX model of the quantized path: MatMulNBits,
 //                                                         SimplifiedLayerNormalization, Sigmoid, Mul, Add)
+#include "../../nnf_mxfp4_plan.h"
 #include "../nnf_datagen.h"
 #include "nnfusion/core/operators/generic_op/generic_op.hpp"
 #include "nnfusion/engine/pass/codegen/base_codegen_pass.hpp"
@@ -33,7 +36,7 @@ namespace
     // stream ids shared with nnfusion_amd/datagen.py
     enum
     {
-        S_ACT = 1, S_WQ, S_SCALE, S_GAMMA, S_A8, S_W8, S_STOK, S_SCH, S_WQ2, S_SCALE2
+        S_ACT = 1, S_WQ, S_SCALE, S_GAMMA, S_A8, S_W8, S_STOK, S_SCH, S_WQ2, S_SCALE2, S_BIAS, S_RES, S_ZP, S_MXS, S_MXS2
     };
 
     std::shared_ptr<graph::GNode> constant_u4(graph::Graph& g, uint64_t stream, size_t n, size_t k)
@@ -48,6 +51,18 @@ namespace
         nnf_gen_uniform_f16(0, stream, 0.005, 0.02, data.data(), data.size());
         return g.add_node_and_edge(std::make_shared<op::Constant>(element::f16, Shape{n, groups}, data.data()), graph::GNodeVector{});
     }
+    // the codes and scale bytes (2^-9 .. 2^-3) of `experts` matrices
+    std::pair<std::shared_ptr<graph::GNode>, std::shared_ptr<graph::GNode>> constant_mx(graph::Graph& g, uint64_t codes, uint64_t scales, size_t experts,
+                                                                                        size_t n, size_t k)
+    {
+        std::vector<uint8_t> data(experts * n * k / 2);
+        nnf_gen_uniform_u4_packed(0, codes, data.data(), experts * n * k);
+        const size_t stride = (size_t)nnf::mx::scale_bytes((int)k);
+        std::vector<int8_t> bytes(experts * n * stride);
+        nnf_gen_uniform_i8(0, scales, 118, 124, bytes.data(), bytes.size());
+        return {g.add_node_and_edge(std::make_shared<op::Constant>(element::u8, Shape{experts, n, k / 2}, data.data()), graph::GNodeVector{}),
+                g.add_node_and_edge(std::make_shared<op::Constant>(element::u8, Shape{experts, n, stride}, bytes.data()), graph::GNodeVector{})};
+    }
 } // namespace
 
 int main(int argc, char** argv)
@@ -55,7 +70,7 @@ int main(int argc, char** argv)
     const bool from_onnx = argc >= 4 && std::string(argv[1]) == "onnx";
     if (argc < 6 && !(from_onnx && argc >= 4))
     {
-        fprintf(stderr, "usage: %s <quant_dot|w8a8|mlp|mlp_nodes|mlp_graph|qkv_graph> <out_dir> <d0> <d1> <d2> [include_dir lib_dir]\n"
+        fprintf(stderr, "usage: %s <quant_dot|w8a8|mlp|mlp_nodes|mlp_graph|qkv_graph|mx_experts> <out_dir> <d0> <d1> <d2> [include_dir lib_dir]\n"
                         "       %s onnx <out_dir> <model.onnx> [include_dir lib_dir]\n", argv[0], argv[0]);
         return 2;
     }
@@ -152,6 +167,23 @@ int main(int argc, char** argv)
             auto down = g->add_node_and_edge(std::make_shared<op::GenericOp>("down", "QuantDot", any), {h, wd, sd});
             auto out = g->add_node_and_edge(std::make_shared<op::GenericOp>("out", "Add", any), {x, down});
             g->add_node_and_edge(std::make_shared<op::Result>(), {out});
+        }
+        else if (kind == "mx_experts")
+        {
+            const size_t M = d0, H = d1, I = d2, E = 4;
+            auto x = g->add_node_and_edge(std::make_shared<op::Parameter>(element::f16, Shape{M, H}), graph::GNodeVector{});
+            auto index = g->add_node_and_edge(std::make_shared<op::Parameter>(element::i32, Shape{2 * M}), graph::GNodeVector{});
+            auto offsets = g->add_node_and_edge(std::make_shared<op::Parameter>(element::i32, Shape{E + 1}), graph::GNodeVector{});
+            auto up = constant_mx(*g, S_WQ, S_MXS, E, 2 * I, H), down = constant_mx(*g, S_WQ2, S_MXS2, E, H, I);
+            using Inputs = std::vector<std::pair<std::shared_ptr<graph::GNode>, int>>;
+            auto a = g->add_node_and_edge(std::make_shared<op::GenericOp>("quantize", "MxQuantize", op::OpConfig::any::parse("{\"has_index\": true}")),
+                                          Inputs{{x, 0}, {index, 0}});
+            auto h = g->add_node_and_edge(std::make_shared<op::GenericOp>("gate_up", "MxGroupedDot", op::OpConfig::any::parse("{\"act\": \"silu_gate\"}")),
+                                          Inputs{{a, 0}, {a, 1}, {up.first, 0}, {up.second, 0}, {offsets, 0}});
+            auto b = g->add_node_and_edge(std::make_shared<op::GenericOp>("quantize_h", "MxQuantize", op::OpConfig::any()), Inputs{{h, 0}});
+            auto y = g->add_node_and_edge(std::make_shared<op::GenericOp>("down", "MxGroupedDot", op::OpConfig::any()),
+                                          Inputs{{b, 0}, {b, 1}, {down.first, 0}, {down.second, 0}, {offsets, 0}});
+            g->add_node_and_edge(std::make_shared<op::Result>(), {y});
         }
         else if (kind == "qkv_graph")
         {

@@ -3,6 +3,9 @@
 // Both are one pass over memory: 2 bytes of fp16 and 17/32 byte of MXFP4 per value.  A wavefront takes units of 512 values of one row, eight
 // to a lane: 16 bytes of fp16, 4 bytes of codes, a block of 32 values to each four lanes, its scale byte by way of the lanes'
 // maximum.  A unit is 1 KiB, 256 bytes and 16 bytes in memory order; the row of scale bytes is padded to 16, so units never share one.
+// The hardware's conversion does the division by the power of two, the rounding and the saturation of a pair of values at once.
+//
+// Measured: @CONVERT@
 #include "mxfp4.h"
 #include "nnf_launch.h"
 
@@ -10,6 +13,8 @@ namespace nnf
 {
     namespace
     {
+        using namespace mx;
+
         constexpr int CONVERT_THREADS = 256;
         constexpr int WAVES = CONVERT_THREADS / WAVE;
 
@@ -21,17 +26,17 @@ namespace nnf
         }
 
         // where the units of a wavefront lie: UNITS of them from its first on, their rows and places in them found with one division
-        template <int UNITS, class Index>
+        template <int UNITS>
         struct Place
         {
-            Index first; // unit of the first
-            Index row[UNITS];
+            int first; // unit of the first
+            int row[UNITS];
             int unit[UNITS];
             __device__ __forceinline__ Place(int row_units)
             {
-                first = ((Index)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * UNITS;
+                first = ((int)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * UNITS;
                 row[0] = first / row_units;
-                unit[0] = (int)(first - row[0] * row_units);
+                unit[0] = first - row[0] * row_units;
 #pragma unroll
                 for (int i = 1; i < UNITS; ++i)
                 {
@@ -42,13 +47,13 @@ namespace nnf
             }
         };
 
-        template <int UNITS, class Index>
+        template <int UNITS>
         __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_quantize_kernel(const half_t* __restrict__ x, const int* __restrict__ index,
                                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                                 Index units, int row_units, int source_rows, int K)
+                                                                                 int units, int row_units, int source_rows, int K)
         {
             const int lane = threadIdx.x & (WAVE - 1);
-            const Place<UNITS, Index> at(row_units);
+            const Place<UNITS> at(row_units);
             uintx4 v[UNITS];
 #pragma unroll
             for (int i = 0; i < UNITS; ++i)
@@ -92,12 +97,12 @@ namespace nnf
             }
         }
 
-        template <int UNITS, class Index>
+        template <int UNITS>
         __global__ __launch_bounds__(CONVERT_THREADS) void mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                                   half_t* __restrict__ y, Index units, int row_units, int K)
+                                                                                   half_t* __restrict__ y, int units, int row_units, int K)
         {
             const int lane = threadIdx.x & (WAVE - 1);
-            const Place<UNITS, Index> at(row_units);
+            const Place<UNITS> at(row_units);
             uint32_t code[UNITS], byte[UNITS];
 #pragma unroll
             for (int i = 0; i < UNITS; ++i)
@@ -129,30 +134,24 @@ namespace nnf
             }
         }
 
-        // f(units, units of a wavefront as a constant, the type that counts them, workgroups): four units a wavefront, all their loads ahead
-        // of the first use, once these fill the CUs; one below, where the time is one load's latency and as many wavefronts as there are
-        // units share it
+        // f(units, units of a wavefront as a constant, units of a row, workgroups): four units a wavefront, all their loads ahead of the
+        // first use, once these fill the CUs; one below, where the time is one load's latency and as many wavefronts as there are units
+        // share it
         template <class F>
         hipError_t over_units(int rows, int K, F f)
         {
             constexpr int MANY = 4;
-            const int row_units = (K + 511) / 512;
-            const long long units = (long long)rows * row_units;
+            const int units = rows * row_units(K);
             if (units < 256 * WAVES * MANY * 2)
-                return f((int)units, std::integral_constant<int, 1>{}, row_units, (unsigned)((units + WAVES - 1) / WAVES));
-            const long long groups = (units + WAVES * MANY - 1) / (WAVES * MANY);
-            if (groups > 0x7FFFFFFFLL)
-                return hipErrorInvalidConfiguration;
-            if (units < 0x7FFFFFFFLL - WAVES * MANY)
-                return f((int)units, std::integral_constant<int, MANY>{}, row_units, (unsigned)groups);
-            return f(units, std::integral_constant<int, MANY>{}, row_units, (unsigned)groups);
+                return f(units, std::integral_constant<int, 1>{}, row_units(K), (units + WAVES - 1) / WAVES);
+            return f(units, std::integral_constant<int, MANY>{}, row_units(K), (units + WAVES * MANY - 1) / (WAVES * MANY));
         }
     } // namespace
 
     hipError_t launch_mxfp4_quantize(hipStream_t s, const void* x, const void* index, void* codes, void* scales, int rows, int source_rows, int K)
     {
-        return over_units(rows, K, [&](auto units, auto many, int row_units, unsigned groups) {
-            mxfp4_quantize_kernel<many, decltype(units)><<<groups, CONVERT_THREADS, 0, s>>>((const half_t*)x, (const int*)index, (uint8_t*)codes,
+        return over_units(rows, K, [&](int units, auto many, int row_units, int groups) {
+            mxfp4_quantize_kernel<many><<<groups, CONVERT_THREADS, 0, s>>>((const half_t*)x, (const int*)index, (uint8_t*)codes,
                                                                                             (uint8_t*)scales, units, row_units, source_rows, K);
             return hipGetLastError();
         });
@@ -160,8 +159,8 @@ namespace nnf
 
     hipError_t launch_mxfp4_dequantize(hipStream_t s, const void* codes, const void* scales, void* y, int rows, int K)
     {
-        return over_units(rows, K, [&](auto units, auto many, int row_units, unsigned groups) {
-            mxfp4_dequantize_kernel<many, decltype(units)><<<groups, CONVERT_THREADS, 0, s>>>((const uint8_t*)codes, (const uint8_t*)scales, (half_t*)y, units,
+        return over_units(rows, K, [&](int units, auto many, int row_units, int groups) {
+            mxfp4_dequantize_kernel<many><<<groups, CONVERT_THREADS, 0, s>>>((const uint8_t*)codes, (const uint8_t*)scales, (half_t*)y, units,
                                                                                               row_units, K);
             return hipGetLastError();
         });

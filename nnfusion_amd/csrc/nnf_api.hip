@@ -898,10 +898,10 @@ namespace
         const int st = current_device_info(dev);
         if (st != NNF_OK)
             return st;
-        const int kernel = variant != NNF_MXFP4_AUTO ? variant - 1 : nnf::mx::choose(o.M, o.N, o.K, gate, o.offsets ? o.experts : 0, dev.num_cu);
-        const nnf::mx::KernelFacts& facts = nnf::mx::FACTS[kernel];
-        if (nnf::mx::row_blocks(o, facts.rows) * nnf::mx::column_tiles(o.N, facts.cols, gate) > 0x7FFFFFFFLL)
-            return NNF_ERR_UNSUPPORTED_SHAPE; // more workgroups than a grid holds
+        const int experts = o.offsets ? o.experts : 0;
+        const int kernel = variant != NNF_MXFP4_AUTO ? variant - 1 : nnf::mx::choose(o.M, o.N, o.K, gate, experts, dev.num_cu);
+        if (kernel == nnf::mx::KERNELS || !nnf::mx::fits(nnf::mx::FACTS[kernel], o.M, o.N, gate, experts))
+            return NNF_ERR_UNSUPPORTED_SHAPE;
         return (int)(kernel <= nnf::mx::ROWS_16x32 ? nnf::launch_mxfp4_rows((hipStream_t)stream, o, kernel, gate)
                                                    : nnf::launch_mxfp4_tiles((hipStream_t)stream, o, kernel, gate));
     }
@@ -920,7 +920,7 @@ int nnf_mxfp4_quantize_f16(nnf_stream_t stream, const void* x, const void* index
         return NNF_ERR_INVALID_ARGUMENT;
     if (!aligned16(x) || !aligned16(index) || !aligned16(codes) || !aligned16(scales))
         return NNF_ERR_INVALID_ARGUMENT;
-    if (!nnf::mx::supported(K))
+    if (!nnf::mx::supported(K) || !nnf::mx::convertible(rows, K))
         return NNF_ERR_UNSUPPORTED_SHAPE;
     const size_t x_bytes = (size_t)source_rows * K * 2, code_bytes = (size_t)rows * K / 2, scale_bytes = (size_t)rows * nnf::mx::scale_bytes(K);
     if (overlap(codes, code_bytes, x, x_bytes) || overlap(scales, scale_bytes, x, x_bytes) || overlap(codes, code_bytes, scales, scale_bytes) ||
@@ -937,7 +937,7 @@ int nnf_mxfp4_dequantize_f16(nnf_stream_t stream, const void* codes, const void*
 {
     if (!codes || !scales || !y || rows <= 0 || K <= 0 || !aligned16(codes) || !aligned16(scales) || !aligned16(y))
         return NNF_ERR_INVALID_ARGUMENT;
-    if (!nnf::mx::supported(K))
+    if (!nnf::mx::supported(K) || !nnf::mx::convertible(rows, K))
         return NNF_ERR_UNSUPPORTED_SHAPE;
     const size_t y_bytes = (size_t)rows * K * 2;
     if (overlap(y, y_bytes, codes, (size_t)rows * K / 2) || overlap(y, y_bytes, scales, (size_t)rows * nnf::mx::scale_bytes(K)))

@@ -22,6 +22,12 @@ namespace nnf
         // tiles of columns of Y, `cols` weight rows each
         constexpr int column_tiles(int N, int cols, bool gate) { return (int)(((long long)N + (gate ? cols / 2 : cols) - 1) / (gate ? cols / 2 : cols)); }
 
+        // a grid has fewer than 2^32 threads.  Of the products' kernels none has more than 512 in a workgroup
+        constexpr long long MAX_WORKGROUPS = (1 << 23) - 1;
+        // quantising and reading back take units of 512 values of a row, 16 of them to a workgroup of 256 threads
+        constexpr int row_units(int K) { return (K + 511) / 512; }
+        constexpr bool convertible(int rows, int K) { return (long long)rows * row_units(K) <= (1 << 28) - 16; }
+
         // activation rows x weight rows of a workgroup's tile.  DEEP: more steps of K under way, fewer wavefronts or workgroups a CU
         enum Kernel
         {
@@ -55,18 +61,19 @@ namespace nnf
             float start, turn, step, wait, off;
         };
         constexpr KernelFacts FACTS[KERNELS] = {
-            {16, 16, 8, 3, 128, false, 2.80f, 1.11f, 0.465f, 0.607f, 0.00f},
-            {16, 32, 4, 5, 128, true, 2.82f, 0.87f, 0.388f, 0.331f, 0.00f},
-            {8, 32, 4, 2, 256, false, 3.83f, 1.64f, 0.404f, 0.422f, 0.22f},
-            {16, 32, 8, 1, 256, false, 3.49f, 2.02f, 1.117f, 1.137f, 0.07f},
-            {16, 64, 2, 2, 256, true, 4.14f, 2.14f, 0.404f, 0.424f, 0.27f},
-            {16, 64, 1, 2, 256, true, 4.06f, 2.64f, 0.226f, 0.355f, 0.18f},
-            {32, 64, 4, 1, 256, true, 3.69f, 2.46f, 0.293f, 1.012f, 0.13f},
-            {64, 64, 4, 1, 256, true, 4.71f, 3.33f, 0.732f, 1.143f, 0.18f},
-            {64, 64, 1, 2, 256, false, 3.95f, 1.98f, 0.291f, 0.305f, 0.16f},
-            {128, 128, 1, 2, 256, true, 4.58f, 4.87f, 0.678f, 0.808f, 0.12f},
-            {128, 128, 1, 1, 256, true, 5.22f, 5.03f, 0.566f, 0.637f, 0.21f},
-            {256, 256, 1, 1, 256, true, 7.57f, 14.47f, 0.148f, 1.449f, 0.13f},
+            // (behind each: a product at which it is the fastest, its time and that of the next)
+            {16, 16, 8, 3, 128, false, 2.80f, 1.11f, 0.465f, 0.607f, 0.00f},   // ROWS_16x16: 1 row by 4096 x 11008 in 8.2 us, the next best 10.5
+            {16, 32, 4, 5, 128, true, 2.82f, 0.87f, 0.388f, 0.331f, 0.00f},    // ROWS_16x32: 64 rows, 60 experts of 2050 x 1376: 15.6 us, 20.9
+            {8, 32, 4, 2, 256, false, 3.83f, 1.64f, 0.404f, 0.422f, 0.22f},    // TILE_8x32: 8 rows by 8192 x 8192: 9.8 us, 10.7
+            {16, 32, 8, 1, 256, false, 3.49f, 2.02f, 1.117f, 1.137f, 0.07f},   // TILE_16x32: 128 rows by 1024 x 8192: 6.7 us, 8.6
+            {16, 64, 2, 2, 256, true, 4.14f, 2.14f, 0.404f, 0.424f, 0.27f},    // TILE_16x64: 64 rows by 4096 x 11008: 13.9 us, 17.2
+            {16, 64, 1, 2, 256, true, 4.06f, 2.64f, 0.226f, 0.355f, 0.18f},    // TILE_16x64_DEEP: 16 rows by 22016 x 4096: 12.6 us, 13.7
+            {32, 64, 4, 1, 256, true, 3.69f, 2.46f, 0.293f, 1.012f, 0.13f},    // TILE_32x64: 64 rows by 8192 x 8192: 13.2 us, 16.3
+            {64, 64, 4, 1, 256, true, 4.71f, 3.33f, 0.732f, 1.143f, 0.18f},    // TILE_64x64: 512 rows by 1024 x 8192: 11.3 us, 13.2
+            {64, 64, 1, 2, 256, false, 3.95f, 1.98f, 0.291f, 0.305f, 0.16f},   // TILE_64x64_DEEP: 512 rows by 2050 x 2080: 11.2 us, 15.0
+            {128, 128, 1, 2, 256, true, 4.58f, 4.87f, 0.678f, 0.808f, 0.12f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376: 43.6 us, 55.4
+            {128, 128, 1, 1, 256, true, 5.22f, 5.03f, 0.566f, 0.637f, 0.21f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 36.7 us, 48.5
+            {256, 256, 1, 1, 256, true, 7.57f, 14.47f, 0.148f, 1.449f, 0.13f}, // TILE_256x256: 2048 rows by 8192 x 8192: 68.8 us, 93.6
         };
 
         // estimated time; experts == 0: one product, else M rows in that many groups, whose sizes are not known here
@@ -95,17 +102,23 @@ namespace nnf
             return (float)(k.start + k.turn * (rounds - 1) + (work > wait ? work : wait) * (K % 256 ? 1 + k.off : 1));
         }
 
-        // the kernel with the lowest estimate
+        // whether a kernel has this form, in a grid that there can be
+        constexpr bool fits(const KernelFacts& k, int M, int N, bool gate, int experts)
+        {
+            return (!gate || k.gate) && most_row_blocks(M, experts, k.rows) * column_tiles(N, k.cols, gate) <= MAX_WORKGROUPS;
+        }
+
+        // the kernel with the lowest estimate of those that fit; KERNELS: none does
         inline Kernel choose(int M, int N, int K, bool gate, int experts, int num_cu)
         {
-            int best = -1;
+            int best = KERNELS;
             float time = 0;
             for (int k = 0; k < KERNELS; ++k)
             {
-                if (gate && !FACTS[k].gate)
+                if (!fits(FACTS[k], M, N, gate, experts))
                     continue;
                 const float t = estimate(FACTS[k], M, N, K, gate, experts, num_cu);
-                if (best < 0 || t < time)
+                if (best == KERNELS || t < time)
                     best = k, time = t;
             }
             return (Kernel)best;

@@ -10,7 +10,7 @@ import numpy as np
 from . import _lib
 
 # stream ids
-S_ACT, S_WQ, S_SCALE, S_GAMMA, S_A8, S_W8, S_STOK, S_SCH, S_WQ2, S_SCALE2, S_BIAS, S_RES, S_ZP = range(1, 14)
+S_ACT, S_WQ, S_SCALE, S_GAMMA, S_A8, S_W8, S_STOK, S_SCH, S_WQ2, S_SCALE2, S_BIAS, S_RES, S_ZP, S_MXS, S_MXS2 = range(1, 16)
 
 
 def _ptr(a):

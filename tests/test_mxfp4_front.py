@@ -143,6 +143,8 @@ def test_conversions_refuse_bad_arguments():
                  (A, None, A, WS, 4, 4, 64), (A, None, W, A, 4, 4, 64), (A, None, W, W, 4, 4, 64), (A, X, X, WS, 4, 4, 64)):
         assert quantize(None, *args) == INVALID, args
     assert quantize(None, A, None, W, WS, 4, 4, 40) == UNSUPPORTED
+    assert quantize(None, A, X, W, WS, 1 << 28, 4, 32) == UNSUPPORTED  # more threads than a grid has
     for args in ((None, WS, Y, 4, 64), (W, None, Y, 4, 64), (W, WS, None, 4, 64), (W, WS, Y, 0, 64), (W, WS, Y, 4, -32), (W, WS, _off(Y, 8), 4, 64), (W, WS, W, 4, 64), (W, WS, WS, 4, 64)):
         assert dequantize(None, *args) == INVALID, args
     assert dequantize(None, W, WS, Y, 4, 24) == UNSUPPORTED
+    assert dequantize(None, W, WS, Y, 1 << 27, 1024) == UNSUPPORTED
