@@ -33,10 +33,14 @@ namespace nnf
             static constexpr int SCALE_LOADS = (ALL_SCALE_LOADS + GROUP - 1) / GROUP;       // of a wavefront
             static constexpr int STAGE = (ROWS + COLS) * STEP_BYTES, SCALES = ALL_SCALE_LOADS * 1024;
             static constexpr int GROUP_LDS = S * STAGE + 2 * SCALES;
+            // a wavefront's fragments of a whole step are read together where it has few MFMAs to hide the latency of LDS behind: a step's four
+            // reads one after the other took 0.26 us of 64 x 64 x 256, together 0.22 (512 x 1024 x 8192 in 12.8 and 11.3 us; with four
+            // MFMAs to a read, 128 x 128, no difference: 27.2 and 27.9 us for 2048 x 4096 x 4096)
+            static constexpr bool WHOLE = FM * FN <= 2;
             static constexpr int PITCH = FN * 128 + 16;                                     // fp32 results of a row of a wavefront
             static constexpr int LDS = GROUP_LDS * WK > WAVES * 32 * PITCH ? GROUP_LDS * WK : WAVES * 32 * PITCH;
             static_assert((ROWS == WM * FM * 32 || (ROWS < 32 && GROUP * FM == 1)) && (ROWS + COLS) / 8 % GROUP == 0, "whole loads");
-            static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && SCALE_ROWS <= 32 && S >= 2 && S <= 4 && (S - 1) * LOADS < 64, "room for them, and a count");
+            static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && SCALE_ROWS <= 32 && S >= 2 && (S - 1) * LOADS < 64, "room for them, and a count");
         };
 
         template <int OFFSET>
@@ -171,13 +175,11 @@ namespace nnf
             constexpr int STEP_LOADS = T::LOADS;
             // until no more than `steps` steps' loads are under way (scale bytes asked for since then make it wait for more, never for less)
             const auto landed_but = [&](int steps) {
-                if (T::S > 3 && steps >= 3)
-                    wait_loads<(T::S > 3 ? 3 : 0) * STEP_LOADS>();
-                else if (T::S > 2 && steps == 2)
-                    wait_loads<(T::S > 2 ? 2 : 0) * STEP_LOADS>();
-                else if (steps == 1)
-                    wait_loads<STEP_LOADS>();
-                else
+                unroll_for<1, T::S>([&](auto n) {
+                    if (steps == n)
+                        wait_loads<n * STEP_LOADS>();
+                });
+                if (steps <= 0)
                     wait_loads<0>();
             };
 
@@ -197,7 +199,8 @@ namespace nnf
             constexpr int FRAGMENT_SCALES = 32 / T::SCALE_ROWS * 1024; // from one fragment's scale bytes to the next one's
 
             floatx16 sum[T::FN][T::FM] = {};
-            uintx4 wf[2][T::FN], af[2][T::FM]; // fragments of an MFMA step and of the next
+            constexpr int U = T::WHOLE ? 4 : 1;
+            uintx4 wf[2][U][T::FN], af[2][U][T::FM]; // fragments of an MFMA step (a whole step) and of the next
             uint32_t ws[T::FN], as[T::FM], ws_next[T::FN], as_next[T::FM];
 
             const auto read_scales = [&](int step) {
@@ -206,17 +209,23 @@ namespace nnf
                 unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * FRAGMENT_SCALES>(as_next[f], as_at + from); });
             };
             // fragment f of an MFMA step: weights, then activations
-            const auto read_fragment = [&](auto f, auto set, int s, uint32_t stage) {
+            const auto read_fragment = [&](auto f, auto set, auto s, uint32_t stage) {
+                constexpr int u = s % U;
                 if constexpr (f < T::FN)
-                    lds_read_b128_nowait<f * 32 * STEP_BYTES>(wf[set][f], w_at[s] + stage);
+                    lds_read_b128_nowait<f * 32 * STEP_BYTES>(wf[set][u][f], w_at[s] + stage);
                 else
-                    lds_read_b128_nowait<(f - T::FN) * 32 * STEP_BYTES>(af[set][f - T::FN], a_at[s] + stage);
+                    lds_read_b128_nowait<(f - T::FN) * 32 * STEP_BYTES>(af[set][u][f - T::FN], a_at[s] + stage);
+            };
+            const auto read_steps = [&](auto set, uint32_t stage) {
+                unroll_for<0, U>([&](auto s) { unroll_for<0, T::FN + T::FM>([&](auto f) { read_fragment(f, set, s, stage); }); });
             };
             // nothing read without a wait stays in flight past the straight line of code that asked for it
             const auto landed = [&](auto set) {
-                lds_wait<0>(wf[set][0]);
-                unroll_for<1, T::FN>([&](auto f) { lds_wait_also(wf[set][f]); });
-                unroll_for<0, T::FM>([&](auto f) { lds_wait_also(af[set][f]); });
+                lds_wait<0>(wf[set][0][0]);
+                unroll_for<0, U>([&](auto u) {
+                    unroll_for<0, T::FN>([&](auto f) { lds_wait_also(wf[set][u][f]); });
+                    unroll_for<0, T::FM>([&](auto f) { lds_wait_also(af[set][u][f]); });
+                });
             };
             const auto take_scales = [&] {
                 unroll_for<0, T::FN>([&](auto f) { lds_wait_also(ws_next[f]); ws[f] = ws_next[f]; });
@@ -238,7 +247,7 @@ namespace nnf
             if constexpr (T::GROUP > 1)
                 asm volatile("s_barrier" ::: "memory");
             read_scales(0);
-            unroll_for<0, T::FN + T::FM>([&](auto f) { read_fragment(f, std::integral_constant<int, 0>{}, 0, 0); });
+            read_steps(std::integral_constant<int, 0>{}, 0);
             landed(std::integral_constant<int, 0>{});
             take_scales();
             uint32_t stage = 0;
@@ -276,14 +285,14 @@ namespace nnf
                         constexpr int READS = (T::FN + T::FM + MFMAS - 1) / MFMAS, FETCHES = (T::LOADS + MFMAS - 1) / MFMAS; // ahead of each MFMA
                         unroll_for<0, READS>([&](auto q) {
                             if constexpr (i * READS + q < T::FN + T::FM)
-                                read_fragment(std::integral_constant<int, i * READS + q>{}, Next{}, (s + 1) & 3, s < 3 ? stage : next_stage);
+                                read_fragment(std::integral_constant<int, i * READS + q>{}, Next{}, std::integral_constant<int, (s + 1) & 3>{}, s < 3 ? stage : next_stage);
                         });
                         if constexpr (s == 3 && full)
                             unroll_for<0, FETCHES>([&](auto q) {
                                 if constexpr (i * FETCHES + q < T::LOADS)
                                     fetch_load(std::integral_constant<int, i * FETCHES + q>{}, step + T::S, stage, std::true_type{});
                             });
-                        sum[fn][fm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf[SET][fn]), operand(af[SET][fm]), sum[fn][fm], FP4, FP4,
+                        sum[fn][fm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf[SET][0][fn]), operand(af[SET][0][fm]), sum[fn][fm], FP4, FP4,
                                                                                       s, (int)ws[fn], s, (int)as[fm]);
                         __builtin_amdgcn_sched_barrier(0);
                     });
@@ -298,14 +307,100 @@ namespace nnf
                 });
                 stage = next_stage;
             };
+            // the same with a whole step's fragments in registers: once every wavefront of the group has its own, the step's place in LDS is
+            // free and the next step's fragments are read, all of them, ahead of this one's MFMAs
+            const auto whole_body = [&](int step, auto set, auto full) {
+                using Next = std::integral_constant<int, 1 - set>;
+                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                if constexpr (full)
+                    wait_loads<(T::S - 2) * STEP_LOADS>();
+                else if (step + 1 < steps && ends_outside(step + 1))
+                {
+                    wait_loads<0>();
+                    cut(step + 1, next_stage);
+                }
+                else
+                    landed_but(min(T::S - 2, steps - 2 - step));
+                if constexpr (T::GROUP > 1)
+                    asm volatile("s_barrier" ::: "memory");
+                if (step % T::G == 0 && step + T::G < steps)
+                    fetch_scales(step + T::G);
+                if constexpr (full)
+                    unroll_for<0, T::LOADS>([&](auto j) { fetch_load(j, step + T::S, stage, std::true_type{}); });
+                else if (step + T::S < steps)
+                    fetch(step + T::S, stage);
+                read_scales(step + 1);
+                read_steps(Next{}, next_stage);
+                unroll_for<0, U>([&](auto s) {
+                    unroll_for<0, T::FN * T::FM>([&](auto i) {
+                        constexpr int fn = i / T::FM, fm = i % T::FM;
+                        sum[fn][fm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf[set][s][fn]), operand(af[set][s][fm]), sum[fn][fm], FP4, FP4,
+                                                                                      s, (int)ws[fn], s, (int)as[fm]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                });
+                landed(Next{});
+                take_scales();
+#pragma unroll
+                for (int fn = 0; fn < T::FN; ++fn)
+#pragma unroll
+                    for (int fm = 0; fm < T::FM; ++fm)
+                        asm volatile("" : "+a"(sum[fn][fm]));
+                stage = next_stage;
+            };
             int step = 0;
             const int whole = min(steps, max(row_bytes / STEP_BYTES - first_step, 0)); // steps that end within the rows
+            // wavefronts whose rows all lie behind the group's end (a block of few rows in a tall tile) fetch for the others, no more: the
+            // matrix cores are left to the other wavefronts of the CU
+            const bool idle = T::WM > 1 && wave_m * T::FM * 32 >= rows.end - rows.first;
+            if (idle)
+            {
 #pragma unroll 1
-            for (; step + T::S < whole; ++step)
-                body(step, std::true_type{});
+                for (; step < steps; ++step)
+                {
+                    const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                    if (step + 1 < steps && ends_outside(step + 1))
+                    {
+                        wait_loads<0>();
+                        cut(step + 1, next_stage);
+                    }
+                    else
+                        landed_but(min(T::S - 2, steps - 2 - step));
+                    asm volatile("s_barrier" ::: "memory");
+                    if (step % T::G == 0 && step + T::G < steps)
+                        fetch_scales(step + T::G);
+                    if (step + T::S < steps)
+                        fetch(step + T::S, stage);
+                    stage = next_stage;
+                }
+            }
+            if constexpr (T::WHOLE)
+            {
+                using Even = std::integral_constant<int, 0>;
+                using Odd = std::integral_constant<int, 1>;
 #pragma unroll 1
-            for (; step < steps; ++step)
-                body(step, std::false_type{});
+                for (; step + 1 + T::S < whole; step += 2)
+                {
+                    whole_body(step, Even{}, std::true_type{});
+                    whole_body(step + 1, Odd{}, std::true_type{});
+                }
+#pragma unroll 1
+                for (; step < steps; step += 2)
+                {
+                    whole_body(step, Even{}, std::false_type{});
+                    if (step + 1 < steps)
+                        whole_body(step + 1, Odd{}, std::false_type{});
+                }
+            }
+            else
+            {
+#pragma unroll 1
+                for (; step + T::S < whole; ++step)
+                    body(step, std::true_type{});
+#pragma unroll 1
+                for (; step < steps; ++step)
+                    body(step, std::false_type{});
+            }
 
             // ---- Y: lane l of a fragment has columns 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32.  A block of 32 rows at a time goes through
             // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane

@@ -80,11 +80,11 @@ namespace nnf
         inline float estimate(const KernelFacts& k, int M, int N, int K, bool gate, int experts, int num_cu)
         {
             // blocks of rows: a group ends in a block that is half full on average, and groups are of about one size
-            double blocks = (double)((M + k.rows - 1) / k.rows);
+            float blocks = (float)((M + k.rows - 1) / k.rows);
             if (experts > 0)
             {
                 const int groups = experts < M ? experts : M;
-                blocks = groups * ((double)M / groups / k.rows + 0.5);
+                blocks = groups * ((float)M / groups / k.rows + 0.5f);
                 if (blocks < groups)
                     blocks = groups;
             }
@@ -96,9 +96,9 @@ namespace nnf
                 if (steps > all_steps)
                     steps = all_steps;
             }
-            const double a_cu = blocks * column_tiles(N, k.cols, gate) / num_cu;
-            const double most = (double)(long long)(a_cu + 0.999999), rounds = (double)(long long)((most + k.per_cu - 1) / k.per_cu);
-            const double work = most * steps * k.step, wait = rounds * steps * k.wait;
+            const float a_cu = blocks * column_tiles(N, k.cols, gate) / num_cu;
+            const float most = (float)(int)(a_cu + 0.99999f), rounds = (float)(int)((most + k.per_cu - 1) / k.per_cu);
+            const float work = most * steps * k.step, wait = rounds * steps * k.wait;
             return (float)(k.start + k.turn * (rounds - 1) + (work > wait ? work : wait) * (K % 256 ? 1 + k.off : 1));
         }
 
