@@ -451,10 +451,13 @@ enum nnf_mxfp4_variant
     NNF_MXFP4_TILE_16x64_DEEP = 6,
     NNF_MXFP4_TILE_32x64 = 7,
     NNF_MXFP4_TILE_64x64 = 8,
-    NNF_MXFP4_TILE_64x64_DEEP = 9, /* through LDS, the wavefronts share the tile; no SiLU-gate */
-    NNF_MXFP4_TILE_128x128 = 10,
-    NNF_MXFP4_TILE_128x128_DEEP = 11,
-    NNF_MXFP4_TILE_256x256 = 12
+    NNF_MXFP4_TILE_32x128 = 9, /* through LDS, the wavefronts share the tile; no SiLU-gate */
+    NNF_MXFP4_TILE_64x64_DEEP = 10, /* no SiLU-gate */
+    NNF_MXFP4_TILE_64x128 = 11,
+    NNF_MXFP4_TILE_64x128_DEEP = 12,
+    NNF_MXFP4_TILE_128x128 = 13,
+    NNF_MXFP4_TILE_128x128_DEEP = 14,
+    NNF_MXFP4_TILE_256x256 = 15
 };
 NNF_API int nnf_mxfp4_variant_supported(int variant, int act);
 NNF_API int nnf_mxfp4_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y,

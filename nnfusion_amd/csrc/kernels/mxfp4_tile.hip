@@ -488,7 +488,10 @@ namespace nnf
         case mx::TILE_16x64_DEEP: return launch_either<Tile<1, 1, 1, 1, 2, 4, 16, 16>>(s, o, gate);
         case mx::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2>>(s, o, gate);
         case mx::TILE_64x64: return launch_either<Tile<1, 1, 4, 2, 2, 2>>(s, o, gate);
+        case mx::TILE_32x128: return launch_either<Tile<1, 4, 1, 1, 1, 3>>(s, o, gate);
         case mx::TILE_64x64_DEEP: return launch_either<Tile<2, 2, 1, 1, 1, 4>>(s, o, gate);
+        case mx::TILE_64x128: return launch_either<Tile<2, 2, 1, 1, 2, 2>>(s, o, gate);
+        case mx::TILE_64x128_DEEP: return launch_either<Tile<2, 2, 1, 1, 2, 4>>(s, o, gate);
         case mx::TILE_128x128: return launch_either<Tile<2, 2, 1, 2, 2, 2>>(s, o, gate);
         case mx::TILE_128x128_DEEP: return launch_either<Tile<2, 2, 1, 2, 2, 4>>(s, o, gate);
         default: return launch_either<Tile<2, 4, 1, 4, 2, 2>>(s, o, gate);

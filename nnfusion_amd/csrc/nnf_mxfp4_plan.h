@@ -39,7 +39,10 @@ namespace nnf
             TILE_16x64_DEEP, // one
             TILE_32x64, // four
             TILE_64x64, // four
-            TILE_64x64_DEEP, // through LDS, the wavefronts share the tile and all of K
+            TILE_32x128, // through LDS, the wavefronts share the tile and all of K
+            TILE_64x64_DEEP,
+            TILE_64x128,
+            TILE_64x128_DEEP,
             TILE_128x128,
             TILE_128x128_DEEP,
             TILE_256x256,
@@ -50,10 +53,11 @@ namespace nnf
         // form with SiLU-gate, and the constants of its time in us,
         //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps, wait * rounds * steps) * (1 + off)
         // with the rounds of workgroups that a CU runs and `off` where rows of codes do not start on lines of memory (K no multiple of
-        // 256).  Fitted to 6700 timings on one MI355X (weights read from HBM: 16 matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192
-        // with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and uneven, each with and without SiLU-gate): 15 .. 24 %
-        // (rms) from each; what they choose takes 1.02 (one matrix) and 1.03 (a mixture) times as long as the best of the kernels on
-        // average, at most 1.5 times (12288 x 1056 with 24 .. 64 rows).
+        // 256).  Fitted to 9800 timings on one MI355X (weights read from HBM: 16 matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192
+        // with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and uneven, each with and without SiLU-gate), those
+        // of the kernels near the fastest with more weight: 15 .. 24 % (rms) from each; what they choose takes 1.02 times as long as the best of
+        // the kernels on average (matrices that the fit has not seen: 1.02, mixtures 1.03), at most 1.45 times (64 rows in 4 uneven
+        // groups by 4096 x 11008).
         struct KernelFacts
         {
             int rows, cols, ranges, per_cu, step_values;
@@ -62,18 +66,21 @@ namespace nnf
         };
         constexpr KernelFacts FACTS[KERNELS] = {
             // (behind each: a product at which it is the fastest, its time and that of the next)
-            {16, 16, 8, 3, 128, false, 2.80f, 1.11f, 0.465f, 0.607f, 0.00f},   // ROWS_16x16: 1 row by 4096 x 11008 in 8.2 us, the next best 10.5
-            {16, 32, 4, 5, 128, true, 2.82f, 0.87f, 0.388f, 0.331f, 0.00f},    // ROWS_16x32: 64 rows, 60 experts of 2050 x 1376: 15.6 us, 20.9
-            {8, 32, 4, 2, 256, false, 3.83f, 1.64f, 0.404f, 0.422f, 0.22f},    // TILE_8x32: 8 rows by 8192 x 8192: 9.8 us, 10.7
-            {16, 32, 8, 1, 256, false, 3.49f, 2.02f, 1.117f, 1.137f, 0.07f},   // TILE_16x32: 128 rows by 1024 x 8192: 6.7 us, 8.6
-            {16, 64, 2, 2, 256, true, 4.14f, 2.14f, 0.404f, 0.424f, 0.27f},    // TILE_16x64: 64 rows by 4096 x 11008: 13.9 us, 17.2
-            {16, 64, 1, 2, 256, true, 4.06f, 2.64f, 0.226f, 0.355f, 0.18f},    // TILE_16x64_DEEP: 16 rows by 22016 x 4096: 12.6 us, 13.7
-            {32, 64, 4, 1, 256, true, 3.69f, 2.46f, 0.293f, 1.012f, 0.13f},    // TILE_32x64: 64 rows by 8192 x 8192: 13.2 us, 16.3
-            {64, 64, 4, 1, 256, true, 4.71f, 3.33f, 0.732f, 1.143f, 0.18f},    // TILE_64x64: 512 rows by 1024 x 8192: 11.3 us, 13.2
-            {64, 64, 1, 2, 256, false, 3.95f, 1.98f, 0.291f, 0.305f, 0.16f},   // TILE_64x64_DEEP: 512 rows by 2050 x 2080: 11.2 us, 15.0
-            {128, 128, 1, 2, 256, true, 4.58f, 4.87f, 0.678f, 0.808f, 0.12f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376: 43.6 us, 55.4
-            {128, 128, 1, 1, 256, true, 5.22f, 5.03f, 0.566f, 0.637f, 0.21f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 36.7 us, 48.5
-            {256, 256, 1, 1, 256, true, 7.57f, 14.47f, 0.148f, 1.449f, 0.13f}, // TILE_256x256: 2048 rows by 8192 x 8192: 68.8 us, 93.6
+            {16, 16, 8, 3, 128, false, 2.80f, 0.02f, 0.476f, 0.408f, 0.00f},   // ROWS_16x16: 1 row by 4096 x 11008 in 8.0 us, the next best 10.4
+            {16, 32, 4, 5, 128, true, 2.64f, 0.01f, 0.334f, 0.414f, 0.00f},    // ROWS_16x32: 16 rows by 2050 x 2080, SiLU-gate: 4.4 us, 7.8
+            {8, 32, 4, 2, 256, false, 3.42f, 1.23f, 0.453f, 0.357f, 0.31f},    // TILE_8x32: 8 rows by 8192 x 8192: 9.7 us, 10.7
+            {16, 32, 8, 1, 256, false, 3.40f, 1.91f, 0.898f, 1.101f, 0.15f},   // TILE_16x32: 128 rows by 1024 x 8192: 6.4 us, 8.2
+            {16, 64, 2, 2, 256, true, 4.02f, 1.86f, 0.411f, 0.336f, 0.30f},    // TILE_16x64: 48 rows by 4096 x 11008: 13.6 us, 16.5
+            {16, 64, 1, 2, 256, true, 4.20f, 2.47f, 0.231f, 0.318f, 0.13f},    // TILE_16x64_DEEP: 64 rows, 4 experts of 4096 x 11008, SiLU-gate: 26.4 us, 28.2
+            {32, 64, 4, 1, 256, true, 3.20f, 1.84f, 0.464f, 1.110f, 0.28f},    // TILE_32x64: 128 rows by 4096 x 4096, SiLU-gate: 6.9 us, 8.9
+            {64, 64, 4, 1, 256, true, 4.49f, 2.59f, 0.884f, 1.290f, 0.22f},    // TILE_64x64: 128 rows by 8192 x 8192, SiLU-gate: 16.5 us, 22.0
+            {32, 128, 1, 2, 256, false, 3.21f, 2.64f, 0.418f, 0.381f, 0.36f},  // TILE_32x128: 256 rows, 8 experts of 2048 x 4096: 10.1 us, 11.5
+            {64, 64, 1, 2, 256, false, 3.90f, 1.78f, 0.296f, 0.277f, 0.31f},   // TILE_64x64_DEEP: 64 rows, 4 experts of 4096 x 11008: 22.7 us, 26.2
+            {64, 128, 1, 2, 256, true, 3.42f, 3.60f, 0.545f, 0.706f, 0.13f},   // TILE_64x128: 1024 rows, 32 experts of 1024 x 1024, SiLU-gate: 8.4 us, 10.8
+            {64, 128, 1, 1, 256, true, 4.72f, 3.83f, 0.467f, 0.467f, 0.14f},   // TILE_64x128_DEEP: 384 rows by 4096 x 11008, SiLU-gate: 27.0 us, 34.9
+            {128, 128, 1, 2, 256, true, 4.75f, 5.28f, 0.620f, 0.827f, 0.17f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376, SiLU-gate: 40.6 us, 50.5
+            {128, 128, 1, 1, 256, true, 5.31f, 4.68f, 0.593f, 0.640f, 0.27f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 37.0 us, 48.1
+            {256, 256, 1, 1, 256, true, 7.30f, 12.58f, 1.145f, 1.538f, 0.19f}, // TILE_256x256: 2048 rows by 8192 x 8192: 66.7 us, 89.2
         };
 
         // estimated time; experts == 0: one product, else M rows in that many groups, whose sizes are not known here
@@ -113,6 +120,8 @@ namespace nnf
         {
             int best = KERNELS;
             float time = 0;
+            // (unrolled: divisions by constants, 0.12 us in place of 0.33)
+#pragma GCC unroll 16
             for (int k = 0; k < KERNELS; ++k)
             {
                 if (!fits(FACTS[k], M, N, gate, experts))
