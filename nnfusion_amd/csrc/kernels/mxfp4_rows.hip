@@ -4,7 +4,14 @@
 // wavefronts cut K into as many ranges, each with the whole tile's sums in registers, which meet in LDS at the end.
 // v_mfma_scale_f32_16x16x128: lane l holds 32 values of row l % 16, the (l / 16)-th block of the step's four, so a load of 16 bytes a
 // lane covers 64 contiguous bytes of each of 16 rows; the row's four scale bytes of the step are one word, from which each lane takes
-// its own (the memory pipeline's time goes by the lines that a load touches: the words of four steps are one load).  The weights are the A operand: a lane then has four consecutive columns of one row of Y.
+// its own (the memory pipeline's time goes by the lines that a load touches: the words of four steps are one load).  The weights are the
+// A operand: a lane then has four consecutive columns of one row of Y.
+//
+// Bound by the latency of a batch of loads where few workgroups have few batches (one row by 4096 x 4096, 8.9 MB: 4.3 us), then by the half
+// lines that its loads take (16 rows by 11008 x 4096, 24 MB: 10.7 us; the tile kernel, which loads whole lines into LDS, 8.3).  It is the
+// fastest where a row of K is a few steps or does not start on a line: 333 rows in 60 groups by 2050 x 1376, 57 MB, in 14 us, 19.7
+// where the weights come from HBM (tiles through LDS: 22 and more).  92 registers instead of 104, for a fifth wavefront on a SIMD, changed
+// nothing.
 #include "mxfp4.h"
 #include "mxfp4_launch.h"
 #include "nnf_launch.h"

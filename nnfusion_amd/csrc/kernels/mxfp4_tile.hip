@@ -4,6 +4,19 @@
 // of 256 values -- 128 bytes of a row, a whole line of memory -- and the lanes of the half g take the blocks 4 g .. 4 g + 3 of a step
 // one MFMA after the other (which values meet in an MFMA is free as long as both operands agree): the four scale bytes that a lane
 // needs for a step are then one aligned word, read once, its byte chosen by the instruction.
+//
+// What bounds the tiles (MI355X; weights read from HBM):
+//   8 .. 64 rows      HBM and the way into LDS: 16 rows by 22016 x 4096, 49 MB, in 13.0 us; 64 rows in 32 groups by 4096 x 4096 with
+//                     SiLU-gate, 233 MB, in 42 us (5.5 TB/s).
+//   64 .. 512 rows    a step's latencies one after the other -- a barrier, LDS, the loads into it at 64 bytes a cycle and CU --: 256 rows by
+//                     4096 x 11008 on 64 x 64 in 16 .. 20 us.  More steps under way (6, 8) or twice the wavefronts on half of K each: no change.
+//   128 x 128         at two workgroups a CU LDS is as busy as the matrix cores would be: four reads of 32 rows for four MFMAs and
+//                     what the loads write.  1024 rows in 8 groups by 22016 x 4096 with SiLU-gate, 408 MB, in 118 us.
+//   256 x 256         power: 4096 rows by 8192 x 8192 in 130 us (4.2 PFLOP/s, matrix cores busy 55 % of the cycles at 1.9 GHz), 92 us with
+//                     zero codes, the same cycles at 2.4 GHz; MFMAs alone reach 6.6 PFLOP/s on drawn data, 9.5 on constant data.  Short K:
+//                     every CU loads, multiplies and stores at the same time (16000 rows in 64 groups by 4096 x 2048 in 129 us).
+// Measured and not kept: lines touched ahead into L2; fragments read two MFMA steps ahead; 256 x 256 by four wavefronts of 128 x 128 (143 us,
+// 134 by eight); 256 x 128 and 128 x 256 (181 us, 130 by 256 x 256); MFMAs at a higher wave priority (no change).
 #include "mxfp4.h"
 #include "mxfp4_launch.h"
 #include "nnf_launch.h"
