@@ -14,6 +14,8 @@ namespace nnfusion
     {
         namespace hip
         {
+            namespace mx = nnf::mx;
+
             class MxEmitter : public HipLibEmitter
             {
             public:
@@ -53,6 +55,8 @@ namespace nnfusion
                     auto gop = generic();
                     if (!gop || !sized())
                         return nullptr;
+                    if (!mx::convertible((int)m_context->outputs[0]->get_shape()[0], (int)input(0)[1]))
+                        return nullptr;
                     const bool has_index = gop->localOpConfig.getRoot()["has_index"].get<bool>();
                     std::ostringstream ss;
                     ss << "input0, " << (has_index ? "input1" : "nullptr") << ", output0, output1, " << m_context->outputs[0]->get_shape()[0] << ", "
@@ -70,7 +74,7 @@ namespace nnfusion
                 }
                 LanguageUnit_p emit_function_body() override
                 {
-                    if (!generic() || !sized())
+                    if (!generic() || !sized() || !mx::convertible((int)input(0)[0], 2 * (int)input(0)[1]))
                         return nullptr;
                     std::ostringstream ss;
                     ss << "input0, input1, output0, " << input(0)[0] << ", " << 2 * input(0)[1];
@@ -93,9 +97,10 @@ namespace nnfusion
                     auto& cfg = gop->localOpConfig.getRoot();
                     const bool bias = cfg["has_bias"].get<bool>(), residual = cfg["has_residual"].get<bool>();
                     const bool gate = cfg["act"].get<std::string>() == "silu_gate";
-                    if (gate && (bias || residual)) // what the launcher declines
-                        return nullptr;
                     const Shape& y = m_context->outputs[0]->get_shape();
+                    // what the launcher declines
+                    if ((gate && (bias || residual)) || !mx::product_supported((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate))
+                        return nullptr;
                     std::ostringstream ss;
                     ss << "input0, input1, input2, input3, output0, " << y[0] << ", " << y[1] << ", " << 2 * input(0)[1] << ", "
                        << (bias ? "input4" : "nullptr") << ", " << (residual ? (bias ? "input5" : "input4") : "nullptr") << ", " << act_enum(gate)
@@ -118,6 +123,8 @@ namespace nnfusion
                         return nullptr;
                     const bool gate = gop->localOpConfig.getRoot()["act"].get<std::string>() == "silu_gate";
                     const Shape& y = m_context->outputs[0]->get_shape();
+                    if (!mx::product_supported((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate))
+                        return nullptr;
                     std::ostringstream ss;
                     ss << "input0, input1, input2, input3, input4, output0, " << input(2)[0] << ", " << y[0] << ", " << y[1] << ", " << 2 * input(0)[1]
                        << ", " << act_enum(gate) << ", nullptr, 0";

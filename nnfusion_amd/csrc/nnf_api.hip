@@ -883,8 +883,7 @@ namespace
             !aligned16(o.residual) || !aligned16(o.offsets))
             return NNF_ERR_INVALID_ARGUMENT;
         const bool gate = act == NNF_ACT_SILU_GATE;
-        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::supported(o.K) || (gate && (o.bias || o.residual)) || o.N > (1 << 29) || o.M > (1 << 30) ||
-            (gate && (size_t)o.N * o.K >= (size_t)1 << 32)) // (byte offsets from a gate row to its up row: 32 bits)
+        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::product_supported(o.M, o.N, o.K, gate) || (gate && (o.bias || o.residual)))
             return NNF_ERR_UNSUPPORTED_SHAPE;
         const size_t y_bytes = (size_t)o.M * o.N * 2, w_rows = (size_t)o.experts * o.N * (gate ? 2 : 1);
         const size_t row = (size_t)o.K / 2, scale_row = nnf::mx::scale_bytes(o.K);

@@ -118,6 +118,14 @@ int main()
         EXPECT(gate->get_output_shape(0) == (Shape{7, 48}) && emitted(gate).find("output0, 7, 48, 512, nullptr, nullptr, NNF_ACT_SILU_GATE") != std::string::npos);
         // the launcher has no gate with a bias: the node is declined, not miscompiled
         EXPECT(emitted(add(g, "MxDot", {a, as, w, ws, param(g, element::f16, Shape{48})}, "{\"act\": \"silu_gate\", \"has_bias\": true}")).empty());
+        // nor sizes beyond its own: N * K of 2^32 with SiLU-gate, 2^30 rows of results and more
+        const size_t rows = 1 << 17, k = 1 << 15;
+        auto la = param(g, element::u8, Shape{4, k / 2}), las = param(g, element::u8, Shape{4, k / 32});
+        auto lw = param(g, element::u8, Shape{2 * rows, k / 2}), lws = param(g, element::u8, Shape{2 * rows, k / 32});
+        EXPECT(!emitted(add(g, "MxDot", {la, las, lw, lws})).empty() && emitted(add(g, "MxDot", {la, las, lw, lws}, "{\"act\": \"silu_gate\"}")).empty());
+        EXPECT(emitted(add(g, "MxDot", {param(g, element::u8, Shape{(1 << 30) + 1, 16}), param(g, element::u8, Shape{(1 << 30) + 1, 16}),
+                                        param(g, element::u8, Shape{8, 16}), param(g, element::u8, Shape{8, 16})})).empty());
+        EXPECT(emitted(add(g, "MxQuantize", {param(g, element::f16, Shape{1 << 28, 32})})).empty());
         EXPECT(refused([&] { add(g, "MxDot", {a, as, param(g, element::u8, Shape{96, 128}), param(g, element::u8, Shape{96, 16})}); }));
         EXPECT(refused([&] { add(g, "MxDot", {a, as, w, ws, param(g, element::f16, Shape{95})}, "{\"has_bias\": true}"); }));
         EXPECT(refused([&] { add(g, "MxDot", {a, as, w, ws, param(g, element::f16, Shape{96, 7})}, "{\"has_residual\": true}"); }));
