@@ -438,23 +438,23 @@ NNF_API int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_sca
                    void* workspace, size_t workspace_bytes);
 
 /* The kernels behind the two products as selectable variants (see nnf_w4a16_variant): activation rows x weight rows of a
- * workgroup's tile.  Every one serves every shape; those without a form with SiLU-gate are NNF_ERR_UNSUPPORTED_SHAPE there
+ * workgroup's tile.  Every one serves every shape; the one without a form with SiLU-gate is NNF_ERR_UNSUPPORTED_SHAPE there
  * (nnf_mxfp4_variant_supported).  NNF_MXFP4_AUTO: the one with the lowest estimated time for the shape. */
 enum nnf_mxfp4_variant
 {
     NNF_MXFP4_AUTO = 0,
     NNF_MXFP4_ROWS_16x16 = 1, /* operands straight into registers; no SiLU-gate */
     NNF_MXFP4_ROWS_16x32 = 2,
-    NNF_MXFP4_TILE_8x32 = 3, /* through LDS, a range of K to each wavefront; no SiLU-gate */
-    NNF_MXFP4_TILE_16x32 = 4, /* no SiLU-gate */
-    NNF_MXFP4_TILE_16x64 = 5,
-    NNF_MXFP4_TILE_16x64_DEEP = 6,
-    NNF_MXFP4_TILE_32x64 = 7,
-    NNF_MXFP4_TILE_64x64 = 8,
-    NNF_MXFP4_TILE_32x128 = 9, /* through LDS, the wavefronts share the tile; no SiLU-gate */
-    NNF_MXFP4_TILE_64x64_DEEP = 10, /* no SiLU-gate */
+    NNF_MXFP4_TILE_8x32 = 3, /* through LDS, a range of K to each wavefront: two */
+    NNF_MXFP4_TILE_16x32 = 4, /* one, two, four */
+    NNF_MXFP4_TILE_16x32_2 = 5,
+    NNF_MXFP4_TILE_16x32_4 = 6,
+    NNF_MXFP4_TILE_16x64 = 7,
+    NNF_MXFP4_TILE_32x64 = 8,
+    NNF_MXFP4_TILE_32x128 = 9, /* through LDS, the wavefronts share the tile */
+    NNF_MXFP4_TILE_64x64 = 10,
     NNF_MXFP4_TILE_64x128 = 11,
-    NNF_MXFP4_TILE_64x128_DEEP = 12,
+    NNF_MXFP4_TILE_64x128_DEEP = 12, /* more steps of K under way, one workgroup a CU */
     NNF_MXFP4_TILE_128x128 = 13,
     NNF_MXFP4_TILE_128x128_DEEP = 14,
     NNF_MXFP4_TILE_256x256 = 15

@@ -417,10 +417,10 @@ namespace nnf
 
             // ---- Y: lane l of a fragment has columns 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32.  A block of 32 rows at a time goes through
             // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane
-            constexpr int FO = GATE ? T::FN / 2 : T::FN; // fragments of columns of Y
-            constexpr int LANES = FO * 4, PASSES = 32 * LANES / WAVE, MINE = (PASSES + T::WK - 1) / T::WK;
+            constexpr int MY_COLS = T::FN * (GATE ? 16 : 32); // columns of Y of a wavefront
+            constexpr int LANES = MY_COLS / 8, PASSES = 32 * LANES / WAVE, MINE = (PASSES + T::WK - 1) / T::WK;
             static_assert(32 * LANES % WAVE == 0, "whole passes");
-            const int n = n0 + wave_n * FO * 32 + lane % LANES * 8;
+            const int n = n0 + wave_n * MY_COLS + lane % LANES * 8;
             uint8_t* const block = lds + wave * (32 * T::PITCH); // the first group's; the others' behind it
             constexpr int PART = T::GROUP * 32 * T::PITCH;
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -451,10 +451,10 @@ namespace nnf
                             y[i][h] += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16);
                         if constexpr (GATE)
                         {
-                            floatx4 up = *reinterpret_cast<const floatx4*>(at + h * 16 + FO * 128);
+                            floatx4 up = *reinterpret_cast<const floatx4*>(at + h * 16 + MY_COLS * 4);
 #pragma unroll
                             for (int k = 1; k < T::WK; ++k)
-                                up += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16 + FO * 128);
+                                up += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16 + MY_COLS * 4);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 y[i][h][e] = silu_gate(y[i][h][e], up[e]);
@@ -484,10 +484,7 @@ namespace nnf
         template <class T>
         hipError_t launch_either(hipStream_t s, const Operands& o, bool gate)
         {
-            if constexpr (T::FN % 2 == 0)
-                if (gate)
-                    return launch<T, true>(s, o);
-            return gate ? hipErrorInvalidValue : launch<T, false>(s, o);
+            return gate ? launch<T, true>(s, o) : launch<T, false>(s, o);
         }
     } // namespace
 
@@ -495,14 +492,14 @@ namespace nnf
     {
         switch (kernel)
         {
-        case mx::TILE_8x32: return launch_either<Tile<1, 1, 4, 1, 1, 3, 4, 8>>(s, o, gate);
-        case mx::TILE_16x32: return launch_either<Tile<1, 1, 8, 1, 1, 2, 4, 16>>(s, o, gate);
+        case mx::TILE_8x32: return launch_either<Tile<1, 1, 2, 1, 1, 3, 8, 8>>(s, o, gate);
+        case mx::TILE_16x32: return launch_either<Tile<1, 1, 1, 1, 1, 4, 16, 16>>(s, o, gate);
+        case mx::TILE_16x32_2: return launch_either<Tile<1, 1, 2, 1, 1, 4, 8, 16>>(s, o, gate);
+        case mx::TILE_16x32_4: return launch_either<Tile<1, 1, 4, 1, 1, 3, 4, 16>>(s, o, gate);
         case mx::TILE_16x64: return launch_either<Tile<1, 1, 2, 1, 2, 3, 8, 16>>(s, o, gate);
-        case mx::TILE_16x64_DEEP: return launch_either<Tile<1, 1, 1, 1, 2, 4, 16, 16>>(s, o, gate);
         case mx::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2>>(s, o, gate);
-        case mx::TILE_64x64: return launch_either<Tile<1, 1, 4, 2, 2, 2>>(s, o, gate);
         case mx::TILE_32x128: return launch_either<Tile<1, 4, 1, 1, 1, 3>>(s, o, gate);
-        case mx::TILE_64x64_DEEP: return launch_either<Tile<2, 2, 1, 1, 1, 4>>(s, o, gate);
+        case mx::TILE_64x64: return launch_either<Tile<2, 2, 1, 1, 1, 4>>(s, o, gate);
         case mx::TILE_64x128: return launch_either<Tile<2, 2, 1, 1, 2, 2>>(s, o, gate);
         case mx::TILE_64x128_DEEP: return launch_either<Tile<2, 2, 1, 1, 2, 4>>(s, o, gate);
         case mx::TILE_128x128: return launch_either<Tile<2, 2, 1, 2, 2, 2>>(s, o, gate);

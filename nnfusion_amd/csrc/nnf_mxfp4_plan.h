@@ -39,14 +39,14 @@ namespace nnf
         {
             ROWS_16x16, // operands straight into registers, eight ranges of K
             ROWS_16x32, // four
-            TILE_8x32,  // through LDS, a wavefront for each range of K: four
-            TILE_16x32, // eight
+            TILE_8x32,  // through LDS, a wavefront for each range of K: two
+            TILE_16x32, // one
+            TILE_16x32_2, // two
+            TILE_16x32_4, // four
             TILE_16x64, // two
-            TILE_16x64_DEEP, // one
             TILE_32x64, // four
-            TILE_64x64, // four
             TILE_32x128, // through LDS, the wavefronts share the tile and all of K
-            TILE_64x64_DEEP,
+            TILE_64x64,
             TILE_64x128,
             TILE_64x128_DEEP,
             TILE_128x128,
@@ -57,40 +57,46 @@ namespace nnf
 
         // What is known of a kernel: its tile, ranges of K, workgroups that a CU holds at once, values of a step of K, whether it has a
         // form with SiLU-gate, and the constants of its time in us,
-        //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps, wait * rounds * steps) * (1 + off)
-        // with the rounds of workgroups that a CU runs and `off` where rows of codes do not start on lines of memory (K no multiple of
-        // 256).  Fitted to 9800 timings on one MI355X (weights read from HBM: 16 matrices from 512 x 2048 to 22016 x 4096 and 8192 x 8192
-        // with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and uneven, each with and without SiLU-gate), those
-        // of the kernels near the fastest with more weight: 15 .. 24 % (rms) from each; what they choose takes 1.02 times as long as the best of
-        // the kernels on average (matrices that the fit has not seen: 1.02, mixtures 1.03), at most 1.45 times (64 rows in 4 uneven
-        // groups by 4096 x 11008).
+        //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps * (1 + off), wait * rounds * steps * (1 + off), bytes / rate)
+        // with the rounds of workgroups that a CU runs, `off` where rows of codes do not start on lines of memory (K no multiple of
+        // 256), and the bytes of weights, activations and results at TB/s.  Fitted to 12700 timings on one MI355X (weights read from
+        // HBM: 19 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and
+        // uneven, each with and without SiLU-gate), those of the kernels near the fastest with more weight: 17 .. 23 % (rms) from each; what
+        // they choose takes 1.02 times as long as the best of the kernels on average (matrices and mixtures that the fit has not
+        // seen: 1.03), at most 1.34 times (64 rows in 60 groups by 2050 x 1376).
         struct KernelFacts
         {
             int rows, cols, ranges, per_cu, step_values;
             bool gate;
-            float start, turn, step, wait, off;
+            float start, turn, step, wait, off, rate;
         };
         constexpr KernelFacts FACTS[KERNELS] = {
             // (behind each: a product at which it is the fastest, its time and that of the next)
-            {16, 16, 8, 3, 128, false, 2.80f, 0.02f, 0.476f, 0.408f, 0.00f},   // ROWS_16x16: 1 row by 4096 x 11008 in 8.0 us, the next best 10.4
-            {16, 32, 4, 5, 128, true, 2.64f, 0.01f, 0.334f, 0.414f, 0.00f},    // ROWS_16x32: 16 rows by 2050 x 2080, SiLU-gate: 4.4 us, 7.8
-            {8, 32, 4, 2, 256, false, 3.42f, 1.23f, 0.453f, 0.357f, 0.31f},    // TILE_8x32: 8 rows by 8192 x 8192: 9.7 us, 10.7
-            {16, 32, 8, 1, 256, false, 3.40f, 1.91f, 0.898f, 1.101f, 0.15f},   // TILE_16x32: 128 rows by 1024 x 8192: 6.4 us, 8.2
-            {16, 64, 2, 2, 256, true, 4.02f, 1.86f, 0.411f, 0.336f, 0.30f},    // TILE_16x64: 48 rows by 4096 x 11008: 13.6 us, 16.5
-            {16, 64, 1, 2, 256, true, 4.20f, 2.47f, 0.231f, 0.318f, 0.13f},    // TILE_16x64_DEEP: 64 rows, 4 experts of 4096 x 11008, SiLU-gate: 26.4 us, 28.2
-            {32, 64, 4, 1, 256, true, 3.20f, 1.84f, 0.464f, 1.110f, 0.28f},    // TILE_32x64: 128 rows by 4096 x 4096, SiLU-gate: 6.9 us, 8.9
-            {64, 64, 4, 1, 256, true, 4.49f, 2.59f, 0.884f, 1.290f, 0.22f},    // TILE_64x64: 128 rows by 8192 x 8192, SiLU-gate: 16.5 us, 22.0
-            {32, 128, 1, 2, 256, false, 3.21f, 2.64f, 0.418f, 0.381f, 0.36f},  // TILE_32x128: 256 rows, 8 experts of 2048 x 4096: 10.1 us, 11.5
-            {64, 64, 1, 2, 256, false, 3.90f, 1.78f, 0.296f, 0.277f, 0.31f},   // TILE_64x64_DEEP: 64 rows, 4 experts of 4096 x 11008: 22.7 us, 26.2
-            {64, 128, 1, 2, 256, true, 3.42f, 3.60f, 0.545f, 0.706f, 0.13f},   // TILE_64x128: 1024 rows, 32 experts of 1024 x 1024, SiLU-gate: 8.4 us, 10.8
-            {64, 128, 1, 1, 256, true, 4.72f, 3.83f, 0.467f, 0.467f, 0.14f},   // TILE_64x128_DEEP: 384 rows by 4096 x 11008, SiLU-gate: 27.0 us, 34.9
-            {128, 128, 1, 2, 256, true, 4.75f, 5.28f, 0.620f, 0.827f, 0.17f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376, SiLU-gate: 40.6 us, 50.5
-            {128, 128, 1, 1, 256, true, 5.31f, 4.68f, 0.593f, 0.640f, 0.27f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 37.0 us, 48.1
-            {256, 256, 1, 1, 256, true, 7.30f, 12.58f, 1.145f, 1.538f, 0.19f}, // TILE_256x256: 2048 rows by 8192 x 8192: 66.7 us, 89.2
+            {16, 16, 8, 3, 128, false, 2.76f, 0.15f, 0.452f, 0.437f, 0.00f, 4.71f},   // ROWS_16x16: 2 rows by 4096 x 11008 in 7.9 us, the next best 9.8
+            {16, 32, 4, 5, 128, true, 2.62f, 0.03f, 0.328f, 0.393f, 0.00f, 5.52f},    // ROWS_16x32: 24 rows by 2050 x 2080, SiLU-gate: 4.4 us, 6.5
+            {8, 32, 2, 3, 256, true, 3.88f, 1.36f, 0.200f, 0.307f, 0.19f, 9.41f},     // TILE_8x32: 1 row by 11008 x 4096: 7.5 us, 8.2
+            {16, 32, 1, 4, 256, true, 3.72f, 1.47f, 0.108f, 0.240f, 0.37f, 7.86f},    // TILE_16x32: 16 rows by 22016 x 4096, SiLU-gate: 11.4 us, 13.0
+            {16, 32, 2, 2, 256, true, 4.02f, 1.28f, 0.239f, 0.230f, 0.41f, 7.80f},    // TILE_16x32_2: 32 rows by 4096 x 11008, SiLU-gate: 10.7 us, 12.1
+            {16, 32, 4, 1, 256, true, 3.30f, 1.65f, 0.496f, 0.367f, 0.61f, 5.94f},    // TILE_16x32_4: 96 rows by 1024 x 8192, SiLU-gate: 6.7 us, 7.4
+            {16, 64, 2, 2, 256, true, 4.03f, 1.31f, 0.372f, 0.343f, 0.44f, 7.41f},    // TILE_16x64: 16 rows by 28672 x 8192, SiLU-gate: 25.2 us, 27.9
+            {32, 64, 4, 1, 256, true, 3.33f, 1.67f, 0.917f, 0.852f, 0.48f, 5.55f},    // TILE_32x64: 384 rows by 1024 x 8192: 8.8 us, 11.1
+            {32, 128, 1, 2, 256, true, 3.19f, 1.76f, 0.412f, 0.495f, 0.13f, 8.96f},   // TILE_32x128: 256 rows, 8 experts of 2048 x 4096: 10.2 us, 11.6
+            {64, 64, 1, 2, 256, true, 4.02f, 1.42f, 0.293f, 0.260f, 0.29f, 6.49f},    // TILE_64x64: 1024 rows by 1000 x 5504, SiLU-gate: 11.5 us, 13.3
+            {64, 128, 1, 2, 256, true, 3.46f, 3.59f, 0.482f, 0.760f, 0.07f, 6.14f},   // TILE_64x128: 4096 rows, 60 uneven experts of 2050 x 1376: 52.7 us, 61.6
+            {64, 128, 1, 1, 256, true, 4.18f, 2.85f, 0.208f, 0.481f, 0.22f, 6.35f},   // TILE_64x128_DEEP: 128 rows by 12288 x 4096: 13.3 us, 15.0
+            {128, 128, 1, 2, 256, true, 4.61f, 4.64f, 0.620f, 0.860f, 0.17f, 6.82f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376, SiLU-gate: 40.1 us, 50.4
+            {128, 128, 1, 1, 256, true, 5.21f, 4.34f, 0.564f, 0.652f, 0.24f, 6.84f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 35.5 us, 47.1
+            {256, 256, 1, 1, 256, true, 6.44f, 10.18f, 1.554f, 1.554f, 0.29f, 5.25f}, // TILE_256x256: 4096 rows by 12288 x 4096: 106 us, 145
         };
 
+        // bytes of weights (every group's), activations and results
+        inline float bytes_of(int M, int N, int K, bool gate, int experts)
+        {
+            const float matrices = (float)(experts > 0 ? experts < M ? experts : M : 1);
+            return (matrices * N * (gate ? 2 : 1) + M) * K * (17 / 32.f) + (float)M * N * 2;
+        }
         // estimated time; experts == 0: one product, else M rows in that many groups, whose sizes are not known here
-        inline float estimate(const KernelFacts& k, int M, int N, int K, bool gate, int experts, int num_cu)
+        inline float estimate(const KernelFacts& k, int M, int N, int K, bool gate, int experts, int num_cu, float bytes)
         {
             // blocks of rows: a group ends in a block that is half full on average, and groups are of about one size
             float blocks = (float)((M + k.rows - 1) / k.rows);
@@ -99,7 +105,7 @@ namespace nnf
                 const int groups = experts < M ? experts : M;
                 blocks = groups * ((float)M / groups / k.rows + 0.5f);
                 if (blocks < groups)
-                    blocks = groups;
+                    blocks = (float)groups;
             }
             const int all_steps = (K + k.step_values - 1) / k.step_values;
             int steps = (all_steps + k.ranges - 1) / k.ranges;
@@ -109,10 +115,11 @@ namespace nnf
                 if (steps > all_steps)
                     steps = all_steps;
             }
-            const float a_cu = blocks * column_tiles(N, k.cols, gate) / num_cu;
-            const float most = (float)(int)(a_cu + 0.99999f), rounds = (float)(int)((most + k.per_cu - 1) / k.per_cu);
-            const float work = most * steps * k.step, wait = rounds * steps * k.wait;
-            return (float)(k.start + k.turn * (rounds - 1) + (work > wait ? work : wait) * (K % 256 ? 1 + k.off : 1));
+            const float most = (float)(int)(blocks * column_tiles(N, k.cols, gate) / num_cu + 0.99999f); // workgroups of a CU
+            const float rounds = (float)(((int)most + k.per_cu - 1) / k.per_cu);
+            const float work = most * steps * k.step, wait = rounds * steps * k.wait, stream = bytes * 1e-6f / k.rate;
+            const float steady = (work > wait ? work : wait) * (K % 256 ? 1 + k.off : 1);
+            return k.start + k.turn * (rounds - 1) + (steady > stream ? steady : stream);
         }
 
         // whether a kernel has this form, in a grid that there can be
@@ -124,15 +131,16 @@ namespace nnf
         // the kernel with the lowest estimate of those that fit; KERNELS: none does
         inline Kernel choose(int M, int N, int K, bool gate, int experts, int num_cu)
         {
+            const float bytes = bytes_of(M, N, K, gate, experts);
             int best = KERNELS;
             float time = 0;
-            // (unrolled: divisions by constants, 0.12 us in place of 0.33)
+            // (unrolled: divisions by constants, 0.13 us in place of 0.38)
 #pragma GCC unroll 16
             for (int k = 0; k < KERNELS; ++k)
             {
                 if (!fits(FACTS[k], M, N, gate, experts))
                     continue;
-                const float t = estimate(FACTS[k], M, N, K, gate, experts, num_cu);
+                const float t = estimate(FACTS[k], M, N, K, gate, experts, num_cu, bytes);
                 if (best == KERNELS || t < time)
                     best = k, time = t;
             }

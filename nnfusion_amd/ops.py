@@ -286,8 +286,8 @@ def mxfp4_dequantize(codes, scales, out=None):
 
 
 MXFP4_VARIANTS = {name: i for i, name in enumerate((
-    "auto", "rows_16x16", "rows_16x32", "tile_8x32", "tile_16x32", "tile_16x64", "tile_16x64_deep", "tile_32x64", "tile_64x64", "tile_32x128",
-    "tile_64x64_deep", "tile_64x128", "tile_64x128_deep", "tile_128x128", "tile_128x128_deep", "tile_256x256"))}
+    "auto", "rows_16x16", "rows_16x32", "tile_8x32", "tile_16x32", "tile_16x32_2", "tile_16x32_4", "tile_16x64", "tile_32x64", "tile_32x128",
+    "tile_64x64", "tile_64x128", "tile_64x128_deep", "tile_128x128", "tile_128x128_deep", "tile_256x256"))}
 
 
 def mxfp4_variant_supported(variant, act=0):

@@ -164,7 +164,7 @@ int main()
                         {
                             const int c = choose(m, n, k, gate != 0, experts, 256);
                             EXPECT(c >= 0 && c < KERNELS && fits(FACTS[c], m, n, gate != 0, experts));
-                            const float t = estimate(FACTS[c], m, n, k, gate != 0, experts, 256);
+                            const float t = estimate(FACTS[c], m, n, k, gate != 0, experts, 256, bytes_of(m, n, k, gate != 0, experts));
                             EXPECT(t > 0 && t < 1e9f);
                             seen.insert(c);
                         }
