@@ -59,11 +59,11 @@ namespace nnf
         // form with SiLU-gate, and the constants of its time in us,
         //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps * (1 + off), wait * rounds * steps * (1 + off), bytes / rate)
         // with the rounds of workgroups that a CU runs, `off` where rows of codes do not start on lines of memory (K no multiple of
-        // 256), and the bytes of weights, activations and results at TB/s.  Fitted to 12700 timings on one MI355X (weights read from
-        // HBM: 19 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, nine mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and
-        // uneven, each with and without SiLU-gate), those of the kernels near the fastest with more weight: 17 .. 23 % (rms) from each; what
+        // 256), and the bytes of weights, activations and results at TB/s.  Fitted to 16900 timings on one MI355X (weights read from
+        // HBM: 19 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 17 mixtures of 4 .. 128 experts with 4 .. 16384 rows, even and
+        // uneven, each with and without SiLU-gate), those of the kernels near the fastest with more weight: 19 .. 26 % (rms) from each; what
         // they choose takes 1.02 times as long as the best of the kernels on average (matrices and mixtures that the fit has not
-        // seen: 1.03), at most 1.34 times (64 rows in 60 groups by 2050 x 1376).
+        // seen: 1.03 and 1.04), at most 1.36 times (128 rows in 8 uneven groups by 4096 x 14336).
         struct KernelFacts
         {
             int rows, cols, ranges, per_cu, step_values;
@@ -72,21 +72,21 @@ namespace nnf
         };
         constexpr KernelFacts FACTS[KERNELS] = {
             // (behind each: a product at which it is the fastest, its time and that of the next)
-            {16, 16, 8, 3, 128, false, 2.76f, 0.15f, 0.452f, 0.437f, 0.00f, 4.71f},   // ROWS_16x16: 2 rows by 4096 x 11008 in 7.9 us, the next best 9.8
-            {16, 32, 4, 5, 128, true, 2.62f, 0.03f, 0.328f, 0.393f, 0.00f, 5.52f},    // ROWS_16x32: 24 rows by 2050 x 2080, SiLU-gate: 4.4 us, 6.5
-            {8, 32, 2, 3, 256, true, 3.88f, 1.36f, 0.200f, 0.307f, 0.19f, 9.41f},     // TILE_8x32: 1 row by 11008 x 4096: 7.5 us, 8.2
-            {16, 32, 1, 4, 256, true, 3.72f, 1.47f, 0.108f, 0.240f, 0.37f, 7.86f},    // TILE_16x32: 16 rows by 22016 x 4096, SiLU-gate: 11.4 us, 13.0
-            {16, 32, 2, 2, 256, true, 4.02f, 1.28f, 0.239f, 0.230f, 0.41f, 7.80f},    // TILE_16x32_2: 32 rows by 4096 x 11008, SiLU-gate: 10.7 us, 12.1
-            {16, 32, 4, 1, 256, true, 3.30f, 1.65f, 0.496f, 0.367f, 0.61f, 5.94f},    // TILE_16x32_4: 96 rows by 1024 x 8192, SiLU-gate: 6.7 us, 7.4
-            {16, 64, 2, 2, 256, true, 4.03f, 1.31f, 0.372f, 0.343f, 0.44f, 7.41f},    // TILE_16x64: 16 rows by 28672 x 8192, SiLU-gate: 25.2 us, 27.9
-            {32, 64, 4, 1, 256, true, 3.33f, 1.67f, 0.917f, 0.852f, 0.48f, 5.55f},    // TILE_32x64: 384 rows by 1024 x 8192: 8.8 us, 11.1
-            {32, 128, 1, 2, 256, true, 3.19f, 1.76f, 0.412f, 0.495f, 0.13f, 8.96f},   // TILE_32x128: 256 rows, 8 experts of 2048 x 4096: 10.2 us, 11.6
-            {64, 64, 1, 2, 256, true, 4.02f, 1.42f, 0.293f, 0.260f, 0.29f, 6.49f},    // TILE_64x64: 1024 rows by 1000 x 5504, SiLU-gate: 11.5 us, 13.3
-            {64, 128, 1, 2, 256, true, 3.46f, 3.59f, 0.482f, 0.760f, 0.07f, 6.14f},   // TILE_64x128: 4096 rows, 60 uneven experts of 2050 x 1376: 52.7 us, 61.6
-            {64, 128, 1, 1, 256, true, 4.18f, 2.85f, 0.208f, 0.481f, 0.22f, 6.35f},   // TILE_64x128_DEEP: 128 rows by 12288 x 4096: 13.3 us, 15.0
-            {128, 128, 1, 2, 256, true, 4.61f, 4.64f, 0.620f, 0.860f, 0.17f, 6.82f},  // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376, SiLU-gate: 40.1 us, 50.4
-            {128, 128, 1, 1, 256, true, 5.21f, 4.34f, 0.564f, 0.652f, 0.24f, 6.84f},  // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 35.5 us, 47.1
-            {256, 256, 1, 1, 256, true, 6.44f, 10.18f, 1.554f, 1.554f, 0.29f, 5.25f}, // TILE_256x256: 4096 rows by 12288 x 4096: 106 us, 145
+            {16, 16, 8, 3, 128, false, 2.88f, 0.11f, 0.417f, 0.392f, 0.00f, 4.98f},  // ROWS_16x16: 2 rows by 4096 x 11008 in 7.9 us, the next best 9.8
+            {16, 32, 4, 5, 128, true, 2.62f, 0.02f, 0.311f, 0.412f, 0.00f, 6.25f},   // ROWS_16x32: 24 rows by 2050 x 2080, SiLU-gate: 4.4 us, 6.5
+            {8, 32, 2, 3, 256, true, 3.85f, 1.50f, 0.211f, 0.306f, 0.33f, 10.90f},   // TILE_8x32: 1 row by 11008 x 4096: 7.5 us, 8.2
+            {16, 32, 1, 4, 256, true, 3.63f, 1.56f, 0.112f, 0.235f, 0.48f, 8.02f},   // TILE_16x32: 16 rows by 22016 x 4096, SiLU-gate: 11.4 us, 13.0
+            {16, 32, 2, 2, 256, true, 4.00f, 1.27f, 0.250f, 0.233f, 0.38f, 8.19f},   // TILE_16x32_2: 32 rows by 4096 x 11008, SiLU-gate: 10.7 us, 12.1
+            {16, 32, 4, 1, 256, true, 3.32f, 1.61f, 0.515f, 0.515f, 0.59f, 6.34f},   // TILE_16x32_4: 96 rows by 1024 x 8192, SiLU-gate: 6.7 us, 7.4
+            {16, 64, 2, 2, 256, true, 3.88f, 1.64f, 0.373f, 0.310f, 0.56f, 7.61f},   // TILE_16x64: 16 rows by 28672 x 8192, SiLU-gate: 25.2 us, 27.9
+            {32, 64, 4, 1, 256, true, 3.32f, 1.74f, 0.920f, 0.920f, 0.46f, 5.67f},   // TILE_32x64: 384 rows by 1024 x 8192: 8.8 us, 11.1
+            {32, 128, 1, 2, 256, true, 3.07f, 1.87f, 0.436f, 0.505f, 0.33f, 9.41f},  // TILE_32x128: 256 rows, 8 experts of 2048 x 4096: 10.2 us, 11.6
+            {64, 64, 1, 2, 256, true, 4.05f, 1.56f, 0.293f, 0.276f, 0.27f, 6.53f},   // TILE_64x64: 1024 rows by 1000 x 5504, SiLU-gate: 11.5 us, 13.3
+            {64, 128, 1, 2, 256, true, 3.46f, 2.83f, 0.533f, 0.688f, 0.27f, 5.26f},  // TILE_64x128: 4096 rows, 60 uneven experts of 2050 x 1376: 52.7 us, 61.6
+            {64, 128, 1, 1, 256, true, 4.17f, 3.21f, 0.474f, 0.474f, 0.32f, 6.24f},  // TILE_64x128_DEEP: 128 rows by 12288 x 4096: 13.3 us, 15.0
+            {128, 128, 1, 2, 256, true, 4.41f, 4.14f, 0.636f, 0.871f, 0.23f, 6.12f}, // TILE_128x128: 4096 rows, 60 experts of 2050 x 1376, SiLU-gate: 40.1 us, 50.4
+            {128, 128, 1, 1, 256, true, 5.12f, 4.25f, 0.662f, 0.662f, 0.23f, 6.64f}, // TILE_128x128_DEEP: 1024 rows by 4096 x 11008: 35.5 us, 47.1
+            {256, 256, 1, 1, 256, true, 6.26f, 9.54f, 1.575f, 1.575f, 0.22f, 5.15f}, // TILE_256x256: 4096 rows by 12288 x 4096: 106 us, 145
         };
 
         // bytes of weights (every group's), activations and results
