@@ -7,8 +7,8 @@
 // its own (the memory pipeline's time goes by the lines that a load touches: the words of four steps are one load).  The weights are the
 // A operand: a lane then has four consecutive columns of one row of Y.
 //
-// Bound by the latency of a batch of loads where few workgroups have few batches (one row by 4096 x 4096, 8.9 MB: 4.3 us), then by the half
-// lines that its loads take (16 rows by 11008 x 4096, 24 MB: 10.7 us; the tile kernel, which loads whole lines into LDS, 8.3).  It is the
+// Bound by the latency of a batch of loads where few workgroups have few batches (one row by 4096 x 4096, 8.9 MB: 4.2 us), then by the half
+// lines that its loads take (16 rows by 12288 x 4096, 27 MB: 10.6 us; the tile kernel, which loads whole lines into LDS, 8.1).  It is the
 // fastest where a row of K is a few steps or does not start on a line: 333 rows in 60 groups by 2050 x 1376, 57 MB, in 14 us, 19.7
 // where the weights come from HBM (tiles through LDS: 22 and more).  92 registers instead of 104, for a fifth wavefront on a SIMD, changed
 // nothing.
