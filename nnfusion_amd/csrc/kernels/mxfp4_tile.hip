@@ -10,8 +10,8 @@
 //                     of 16 x 64 took 12.5); 64 rows in 32 groups by 4096 x 4096 with SiLU-gate, 233 MB, in 41 us (5.6 TB/s).
 //   64 .. 512 rows    a step's latencies one after the other -- a barrier, LDS, the loads into it at 64 bytes a cycle and CU --: 256 rows by
 //                     4096 x 11008 on 64 x 64 in 16 .. 20 us.  More steps under way (6, 8) or twice the wavefronts on half of K each: no change.
-//   128 x 128         four reads of 32 rows for four MFMAs and what the loads write keep LDS as busy as the matrix cores would be.  1024 rows
-//                     in 8 groups by 22016 x 4096 with SiLU-gate, 408 MB, in 117 us.
+//   128 x 128         the same latencies, two workgroups a CU taking turns; HBM where groups have few rows.  1024 rows in 8 groups by 22016 x 4096
+//                     with SiLU-gate, 408 MB, in 117 us (matrix cores busy 20 % of the cycles, reads of LDS 18 %).
 //   256 x 256         power: 4096 rows by 8192 x 8192 in 130 us (4.2 PFLOP/s, matrix cores busy 55 % of the cycles at 1.9 GHz), 92 us with
 //                     zero codes, the same cycles at 2.4 GHz; MFMAs alone reach 6.6 PFLOP/s on drawn data, 9.5 on constant data.  Short K:
 //                     every CU loads, multiplies and stores at the same time (16000 rows in 64 groups by 4096 x 2048 in 129 us).
