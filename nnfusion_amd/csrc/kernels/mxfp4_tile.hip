@@ -73,6 +73,22 @@ namespace nnf
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
         }
 
+        // What lanes have written to LDS is there for the lanes that read it, and what they have read may be written over.  WK: the ranges of
+        // K that meet.  One: only lanes of the same wavefront do, whose accesses LDS takes in the order of the code -- no instruction, but
+        // the compiler has to keep that order
+        template <int WK>
+        __device__ __forceinline__ void lanes_meet()
+        {
+            if constexpr (WK > 1)
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else
+            {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            }
+        }
+
         template <class T, bool GATE>
         __global__ __launch_bounds__(T::WAVES* WAVE, 1) void mxfp4_tile_kernel(Operands o, int col_tiles)
         {
@@ -427,16 +443,15 @@ namespace nnf
 #pragma unroll
             for (int fm = 0; fm < T::FM; ++fm)
             {
-                if (T::WK > 1 && fm > 0)
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (fm > 0)
+                    lanes_meet<T::WK>();
 #pragma unroll
                 for (int fn = 0; fn < T::FN; ++fn)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         *reinterpret_cast<floatx4*>(block + group * PART + r * T::PITCH + fn * 128 + q * 32 + g * 16) =
                             floatx4{sum[fn][fm][q * 4], sum[fn][fm][q * 4 + 1], sum[fn][fm][q * 4 + 2], sum[fn][fm][q * 4 + 3]};
-                if constexpr (T::WK > 1)
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                lanes_meet<T::WK>();
                 floatx4 y[MINE][2];
 #pragma unroll
                 for (int i = 0; i < MINE; ++i)
