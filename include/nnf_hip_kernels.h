@@ -467,7 +467,8 @@ NNF_API int nnf_mxfp4_gemm_variant(nnf_stream_t stream, const void* A, const voi
 /* The product of a mixture's experts: rows of A [M, K] and Y [M, N] sorted by expert, one weight matrix each (W u8 [experts, N, K/2],
  * 2N rows with NNF_ACT_SILU_GATE).  Group e is the rows offsets[e] .. offsets[e + 1] - 1; offsets i32 [experts + 1] on the device,
  * not decreasing, within 0 .. M: a group may be empty, and rows before offsets[0] or from offsets[experts] on are left as they
- * are in Y.  (Offsets that break this give undefined rows of Y, never an access outside the operands.) */
+ * are in Y.  (Offsets that break this give undefined rows of Y, never an access outside the operands.)  Sizes as above; experts above
+ * 2^30 are NNF_ERR_UNSUPPORTED_SHAPE. */
 NNF_API size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, int act);
 NNF_API int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
                            const void* offsets, void* Y, int experts, int M, int N, int K, int act,

@@ -883,7 +883,8 @@ namespace
             !aligned16(o.residual) || !aligned16(o.offsets))
             return NNF_ERR_INVALID_ARGUMENT;
         const bool gate = act == NNF_ACT_SILU_GATE;
-        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::product_supported(o.M, o.N, o.K, gate) || (gate && (o.bias || o.residual)))
+        const int experts = o.offsets ? o.experts : 0;
+        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::product_supported(o.M, o.N, o.K, gate, experts) || (gate && (o.bias || o.residual)))
             return NNF_ERR_UNSUPPORTED_SHAPE;
         const size_t y_bytes = (size_t)o.M * o.N * 2, w_rows = (size_t)o.experts * o.N * (gate ? 2 : 1);
         const size_t row = (size_t)o.K / 2, scale_row = nnf::mx::scale_bytes(o.K);
@@ -897,7 +898,6 @@ namespace
         const int st = current_device_info(dev);
         if (st != NNF_OK)
             return st;
-        const int experts = o.offsets ? o.experts : 0;
         const int kernel = variant != NNF_MXFP4_AUTO ? variant - 1 : nnf::mx::choose(o.M, o.N, o.K, gate, experts, dev.num_cu);
         if (kernel == nnf::mx::KERNELS || !nnf::mx::fits(nnf::mx::FACTS[kernel], o.M, o.N, gate, experts))
             return NNF_ERR_UNSUPPORTED_SHAPE;

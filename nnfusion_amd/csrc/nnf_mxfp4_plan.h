@@ -12,10 +12,11 @@ namespace nnf
         constexpr int scale_bytes(int K) { return ((K >> 5) + 15) & ~15; }
         constexpr bool supported(int K) { return K > 0 && K % 32 == 0 && K <= MAX_K; }
 
-        // sizes that a product may have.  With SiLU-gate the bytes from a gate row to its up row are counted in 32 bits
-        constexpr bool product_supported(int M, int N, int K, bool gate)
+        // sizes that a product may have (experts == 0: one weight matrix).  With SiLU-gate the bytes from a gate row to its up row are counted
+        // in 32 bits; groups are looked through 64 at a time, and the first number behind them is an int too
+        constexpr bool product_supported(int M, int N, int K, bool gate, int experts)
         {
-            return supported(K) && M <= 1 << 30 && N <= 1 << 29 && (!gate || (long long)N * K < 1LL << 32);
+            return supported(K) && M <= 1 << 30 && N <= 1 << 29 && (!gate || (long long)N * K < 1LL << 32) && experts <= 1 << 30;
         }
 
         // blocks of `rows` rows that there are at most, of M rows in `experts` groups (0: one product): every group may end in a block of its
