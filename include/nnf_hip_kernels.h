@@ -438,8 +438,8 @@ NNF_API int nnf_mxfp4_gemm(nnf_stream_t stream, const void* A, const void* a_sca
                    void* workspace, size_t workspace_bytes);
 
 /* The kernels behind the two products as selectable variants (see nnf_w4a16_variant): activation rows x weight rows of a
- * workgroup's tile.  Every one serves every shape; the one without a form with SiLU-gate is NNF_ERR_UNSUPPORTED_SHAPE there
- * (nnf_mxfp4_variant_supported).  NNF_MXFP4_AUTO: the one with the lowest estimated time for the shape. */
+ * workgroup's tile.  Each serves every shape whose tiles fit into a grid of its own; the one without a form with SiLU-gate is
+ * NNF_ERR_UNSUPPORTED_SHAPE there (nnf_mxfp4_variant_supported).  NNF_MXFP4_AUTO: the one with the lowest estimated time for the shape. */
 enum nnf_mxfp4_variant
 {
     NNF_MXFP4_AUTO = 0,

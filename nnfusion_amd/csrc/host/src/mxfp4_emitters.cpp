@@ -99,7 +99,7 @@ namespace nnfusion
                     const bool gate = cfg["act"].get<std::string>() == "silu_gate";
                     const Shape& y = m_context->outputs[0]->get_shape();
                     // what the launcher declines
-                    if ((gate && (bias || residual)) || !mx::product_supported((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate, 0))
+                    if ((gate && (bias || residual)) || !mx::servable((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate, 0))
                         return nullptr;
                     std::ostringstream ss;
                     ss << "input0, input1, input2, input3, output0, " << y[0] << ", " << y[1] << ", " << 2 * input(0)[1] << ", "
@@ -123,7 +123,7 @@ namespace nnfusion
                         return nullptr;
                     const bool gate = gop->localOpConfig.getRoot()["act"].get<std::string>() == "silu_gate";
                     const Shape& y = m_context->outputs[0]->get_shape();
-                    if (!mx::product_supported((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate, (int)input(2)[0]))
+                    if (!mx::servable((int)y[0], (int)y[1], 2 * (int)input(0)[1], gate, (int)input(2)[0]))
                         return nullptr;
                     std::ostringstream ss;
                     ss << "input0, input1, input2, input3, input4, output0, " << input(2)[0] << ", " << y[0] << ", " << y[1] << ", " << 2 * input(0)[1]

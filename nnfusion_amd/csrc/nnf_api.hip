@@ -884,7 +884,7 @@ namespace
             return NNF_ERR_INVALID_ARGUMENT;
         const bool gate = act == NNF_ACT_SILU_GATE;
         const int experts = o.offsets ? o.experts : 0;
-        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::product_supported(o.M, o.N, o.K, gate, experts) || (gate && (o.bias || o.residual)))
+        if (!nnf_mxfp4_variant_supported(variant, act) || !nnf::mx::servable(o.M, o.N, o.K, gate, experts) || (gate && (o.bias || o.residual)))
             return NNF_ERR_UNSUPPORTED_SHAPE;
         const size_t y_bytes = (size_t)o.M * o.N * 2, w_rows = (size_t)o.experts * o.N * (gate ? 2 : 1);
         const size_t row = (size_t)o.K / 2, scale_row = nnf::mx::scale_bytes(o.K);
@@ -899,8 +899,8 @@ namespace
         if (st != NNF_OK)
             return st;
         const int kernel = variant != NNF_MXFP4_AUTO ? variant - 1 : nnf::mx::choose(o.M, o.N, o.K, gate, experts, dev.num_cu);
-        if (kernel == nnf::mx::KERNELS || !nnf::mx::fits(nnf::mx::FACTS[kernel], o.M, o.N, gate, experts))
-            return NNF_ERR_UNSUPPORTED_SHAPE;
+        if (!nnf::mx::fits(nnf::mx::FACTS[kernel], o.M, o.N, gate, experts))
+            return NNF_ERR_UNSUPPORTED_SHAPE; // (of a variant that the caller names)
         return (int)(kernel <= nnf::mx::ROWS_16x32 ? nnf::launch_mxfp4_rows((hipStream_t)stream, o, kernel, gate)
                                                    : nnf::launch_mxfp4_tiles((hipStream_t)stream, o, kernel, gate));
     }

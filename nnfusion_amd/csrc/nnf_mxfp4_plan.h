@@ -129,6 +129,18 @@ namespace nnf
             return (!gate || k.gate) && most_row_blocks(M, experts, k.rows) * column_tiles(N, k.cols, gate) <= MAX_WORKGROUPS;
         }
 
+        // whether the library has a kernel for a product (experts == 0: one weight matrix): it takes these sizes, and some kernel's grid holds
+        // their tiles
+        constexpr bool servable(int M, int N, int K, bool gate, int experts)
+        {
+            if (!product_supported(M, N, K, gate, experts))
+                return false;
+            for (int k = 0; k < KERNELS; ++k)
+                if (fits(FACTS[k], M, N, gate, experts))
+                    return true;
+            return false;
+        }
+
         // the kernel with the lowest estimate of those that fit; KERNELS: none does
         inline Kernel choose(int M, int N, int K, bool gate, int experts, int num_cu)
         {

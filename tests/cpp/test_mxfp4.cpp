@@ -186,5 +186,26 @@ int main()
                     EXPECT(most >= (m + rows - 1) / rows && most >= even && most >= ones + (m - ones + rows - 1) / rows && most <= m);
                 }
     });
+
+    // a node gets a kernel where the call has one: not where every tile would need a larger grid than there is
+    run_case("nodes_beyond_every_grid", [] {
+        using namespace nnf::mx;
+        graph::Graph g;
+        const auto dot = [&](size_t m, size_t n) {
+            return emitted(add(g, "MxDot", {param(g, element::u8, Shape{m, 16}), param(g, element::u8, Shape{m, 16}), param(g, element::u8, Shape{n, 16}),
+                                            param(g, element::u8, Shape{n, 16})}));
+        };
+        const auto grouped = [&](size_t experts, size_t m, size_t rows, const char* act) {
+            return emitted(add(g, "MxGroupedDot", {param(g, element::u8, Shape{m, 16}), param(g, element::u8, Shape{m, 16}), param(g, element::u8, Shape{experts, rows, 16}),
+                                                   param(g, element::u8, Shape{experts, rows, 16}), param(g, element::i32, Shape{experts + 1})}, act));
+        };
+        EXPECT(choose(1 << 24, 4096, 32, false, 0, 256) != KERNELS && !dot(1 << 24, 4096).empty());
+        EXPECT(choose(1 << 28, 4096, 32, false, 0, 256) == KERNELS && dot(1 << 28, 4096).empty());
+        // experts of few rows each need a block of rows each
+        const char* const gate = "{\"act\": \"silu_gate\"}";
+        EXPECT(choose(1 << 14, 1 << 16, 32, true, 1 << 13, 256) != KERNELS && !grouped(1 << 13, 1 << 14, 1 << 17, gate).empty());
+        EXPECT(choose(1 << 23, 1 << 16, 32, true, 1 << 23, 256) == KERNELS && grouped(1 << 23, 1 << 23, 1 << 17, gate).empty());
+        EXPECT(choose(1 << 20, 4096, 32, false, 1 << 20, 256) == KERNELS && grouped(1 << 20, 1 << 20, 4096, "{}").empty());
+    });
     return failures ? 1 : 0;
 }
