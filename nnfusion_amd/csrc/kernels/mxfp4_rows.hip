@@ -23,6 +23,7 @@ namespace nnf
         using namespace mx;
 
         constexpr int ROWS = 16; // activation rows of a workgroup
+        typedef uintx4 words4 __attribute__((aligned(4))); // a load of 16 bytes that begins at any word
 
         // T tiles of 16 weight rows, W wavefronts
         template <int T, int W, bool GATE>
@@ -69,8 +70,8 @@ namespace nnf
                 const int scale_from = min(step * 4, scale_stride - 16), skip = step - scale_from / 4;
 #pragma unroll
                 for (int t = 0; t < TW; ++t)
-                    wsv[t] = *reinterpret_cast<const uintx4*>(ws_base + scale_from + ws[t]);
-                asv = *reinterpret_cast<const uintx4*>(as_base + scale_from + as);
+                    wsv[t] = *reinterpret_cast<const words4*>(ws_base + scale_from + ws[t]);
+                asv = *reinterpret_cast<const words4*>(as_base + scale_from + as);
 #pragma unroll
                 for (int s = 0; s < C; ++s)
                 {
