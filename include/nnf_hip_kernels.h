@@ -468,7 +468,9 @@ NNF_API int nnf_mxfp4_gemm_variant(nnf_stream_t stream, const void* A, const voi
  * 2N rows with NNF_ACT_SILU_GATE).  Group e is the rows offsets[e] .. offsets[e + 1] - 1; offsets i32 [experts + 1] on the device,
  * not decreasing, within 0 .. M: a group may be empty, and rows before offsets[0] or from offsets[experts] on are left as they
  * are in Y.  (Offsets that break this give undefined rows of Y, never an access outside the operands.)  Sizes as above; experts above
- * 2^30 are NNF_ERR_UNSUPPORTED_SHAPE. */
+ * 2^30 are NNF_ERR_UNSUPPORTED_SHAPE.  The kernel is chosen for M rows, as if the groups filled the buffer: where they fill little of a
+ * large one, a variant for the rows there are is faster (64 rows in 32 groups by 4096 x 4096 with SiLU-gate: 48 us in a buffer of 64
+ * rows, 74 in one of 8192, 49 there with NNF_MXFP4_TILE_32x128). */
 NNF_API size_t nnf_mxfp4_grouped_gemm_workspace_bytes(int experts, int M, int N, int K, int act);
 NNF_API int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
                            const void* offsets, void* Y, int experts, int M, int N, int K, int act,

@@ -5,8 +5,11 @@
 // maximum.  A unit is 1 KiB, 256 bytes and 16 bytes in memory order; the row of scale bytes is padded to 16, so units never share one.
 // The hardware's conversion does the division by the power of two, the rounding and the saturation of a pair of values at once.
 //
-// Bound by HBM from some thousand units on (22016 x 4096 quantised in 41 us and read back in 44: 5.5 and 5.2 TB/s, a copy of 1 GiB runs at
-// 5.2; 4000 x 5504 in 12.2 and 13.1), by the launch below (16 x 4096: 2.1 us; one row: 1.2 and 1.4 us of kernel).
+// Bound by HBM from some thousand units on: 22016 x 4096 quantised in 41 us and read back in 43 where each runs over buffers beyond the
+// cache, one launch after the other (5.6 and 5.3 TB/s; a copy of 1 GiB runs at 5.2); 4000 x 5504 in 12.0 and 13.1.  In turn, the results
+// of one read by the other, the two take 89 us together; a trace then shows 54 and 34, as what the 256 MB cache holds of a
+// kernel's results goes out under the next one.  Below, by the launch: 256 x 11008 in 3.0 us, 16 x 4096 in 2.1 (launches in a graph; 1.2
+// and 1.4 us of kernel for one row).
 #include "mxfp4.h"
 #include "nnf_launch.h"
 

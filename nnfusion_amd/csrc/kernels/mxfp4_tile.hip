@@ -7,16 +7,20 @@
 //
 // What bounds the tiles (MI355X; weights read from HBM):
 //   8 .. 64 rows      HBM: 16 rows by 22016 x 4096, 49 MB, in 11.0 us (one wavefront a workgroup of 16 x 32: 688 workgroups spread evenly, 344
-//                     of 16 x 64 took 12.5); 64 rows in 32 groups by 4096 x 4096 with SiLU-gate, 233 MB, in 41 us (5.6 TB/s).
+//                     of 16 x 64 took 12.5); 64 rows in 32 groups by 4096 x 4096 with SiLU-gate, 233 MB, in 41 .. 45 us (5.2 .. 5.7 TB/s).
 //   64 .. 512 rows    a step's latencies one after the other -- a barrier, LDS, the loads into it at 64 bytes a cycle and CU --: 256 rows by
-//                     4096 x 11008 on 64 x 64 in 16 .. 20 us.  More steps under way (6, 8) or twice the wavefronts on half of K each: no change.
+//                     4096 x 11008 on 64 x 64 in 15.4 us with the weights in the cache, 20.0 from HBM.  More steps under way (6, 8) or twice
+//                     the wavefronts on half of K each: no change.
 //   128 x 128         the same latencies, two workgroups a CU taking turns; HBM where groups have few rows.  1024 rows in 8 groups by 22016 x 4096
-//                     with SiLU-gate, 408 MB, in 117 us (matrix cores busy 20 % of the cycles, reads of LDS 18 %).
-//   256 x 256         power: 4096 rows by 8192 x 8192 in 130 us (4.2 PFLOP/s, matrix cores busy 55 % of the cycles at 1.9 GHz), 92 us with
-//                     zero codes, the same cycles at 2.4 GHz; MFMAs alone reach 6.6 PFLOP/s on drawn data, 9.5 on constant data.  Short K:
-//                     every CU loads, multiplies and stores at the same time (16000 rows in 64 groups by 4096 x 2048 in 129 us).
+//                     with SiLU-gate, 408 MB, in 117 us (matrix cores busy 20 % of the cycles, LDS 18 %).
+//   256 x 256         the clock by power, the cycles by the kernel: 4096 rows by 8192 x 8192 in 130 us (4.2 PFLOP/s) at 1.9 GHz, on zero codes the
+//                     same cycles at 2.4 GHz, 92 us.  MFMAs alone would take 83 us on drawn data (6.6 PFLOP/s) and 58 on constant data (9.5):
+//                     the matrix cores are busy for 55 % of the cycles, whatever the data.  What fewer cycles would give at the power limit
+//                     has not been measured.  Short K: every CU loads, multiplies and stores at the same time (16000 rows in 64 groups
+//                     by 4096 x 2048 in 130 us).
 // Measured and not kept: lines touched ahead into L2; fragments read two MFMA steps ahead; 256 x 256 by four wavefronts of 128 x 128 (143 us,
-// 134 by eight); 256 x 128 and 128 x 256 (181 us, 130 by 256 x 256); MFMAs at a higher wave priority (no change).
+// 134 by eight); 256 x 128 and 128 x 256 (181 us, 130 by 256 x 256; not timed on groups of about 100 rows); MFMAs at a higher wave priority
+// (no change).
 #include "mxfp4.h"
 #include "mxfp4_launch.h"
 #include "nnf_launch.h"
@@ -125,7 +129,7 @@ namespace nnf
             uint32_t offset[T::LOADS];
             const auto load_base = [&](auto j) { return (wave * T::LOADS + (T::COLS % (T::LOADS * 8) == 0 ? 0 : (int)j)) * 8 >= T::COLS ? a_base : w_base; };
             // piece of a row (16 bytes) that lies at slot `lane % 8` of row `row` in LDS: XORed so that the reads of 16 rows' pieces
-            // spread over all banks
+            // spread over all banks (4 cycles a read of a fragment, none of them for conflicts)
             const auto piece = [&](int row) { return (lane & 7) ^ ((row >> 1) & 7); };
 #pragma unroll
             for (int j = 0; j < T::LOADS; ++j)
@@ -223,6 +227,9 @@ namespace nnf
                 w_at[s] = codes_at + wave_n * T::FN * 32 * STEP_BYTES + in_row(r);
                 a_at[s] = codes_at + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES + in_row(r % T::ROWS);
             }
+            // (words of neighbouring rows lie 16 bytes apart, as the loads put them there, and meet four to a bank: 8 cycles a read where 2 would
+            // do.  These are the conflicts that the counters show, a quarter of the cycles of LDS in the loop -- 12 of 48 a step of
+            // 64 x 64, whose LDS is busy for 16 % of the time, 35 % with 256 x 256)
             const auto scale_at = [&](int row) { return scales_at + row / T::SCALE_ROWS * 1024 + row % T::SCALE_ROWS * 16 + 4 * g; };
             const uint32_t ws_at = scale_at(wave_n * T::FN * 32 + r), as_at = scale_at(T::COLS + wave_m * T::FM * 32 + r % T::ROWS);
             constexpr int FRAGMENT_SCALES = 32 / T::SCALE_ROWS * 1024; // from one fragment's scale bytes to the next one's
@@ -432,7 +439,8 @@ namespace nnf
             }
 
             // ---- Y: lane l of a fragment has columns 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32.  A block of 32 rows at a time goes through
-            // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane
+            // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane (8 cycles a write and
+            // a read, 4 of the read's for conflicts: a lane reads 32 bytes in two halves)
             constexpr int MY_COLS = T::FN * (GATE ? 16 : 32); // columns of Y of a wavefront
             constexpr int LANES = MY_COLS / 8, PASSES = 32 * LANES / WAVE, MINE = (PASSES + T::WK - 1) / T::WK;
             static_assert(32 * LANES % WAVE == 0, "whole passes");

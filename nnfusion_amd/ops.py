@@ -314,5 +314,6 @@ def mxfp4_grouped_gemm_workspace_bytes(experts, m, n, k, act=0):
 def mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, workspace=None, variant="auto"):
     """The product of a mixture's experts: rows of a sorted by expert, w u8 [experts, N, K/2] (2N rows with act=1, SiLU-gate), w_scales
     u8 [experts, N, mxfp4_scale_bytes(K)]; group e is the rows offsets[e] .. offsets[e+1] (offsets i32 [experts+1], on the device, not
-    decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here)."""
+    decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here).  The library chooses a
+    kernel for all rows of a; where the groups fill little of them, name a variant for the rows there are."""
     return _native.mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, workspace, MXFP4_VARIANTS[variant])
