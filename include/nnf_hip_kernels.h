@@ -479,6 +479,56 @@ NNF_API int nnf_mxfp4_grouped_gemm_variant(nnf_stream_t stream, const void* A, c
                                    const void* offsets, void* Y, int experts, int M, int N, int K, int act, int variant,
                                    void* workspace, size_t workspace_bytes);
 
+/* ---------------------------------------------------------------------------------------------
+ * Around the products of a mixture's experts: which experts a token goes to, with what weights and in which order the products take the
+ * tokens; and the experts' rows back to their tokens.  The reference has neither (nearest: TopK and the gathers of its ONNX front).  Base
+ * pointers need the alignment of their element only; rows of combining that all start on 16 bytes are faster.
+ * ------------------------------------------------------------------------------------------- */
+enum nnf_type
+{
+    NNF_TYPE_F16 = 0,
+    NNF_TYPE_BF16 = 1,
+    NNF_TYPE_F32 = 2
+};
+enum nnf_moe_score
+{
+    NNF_MOE_SOFTMAX = 0, /* over all experts */
+    NNF_MOE_SIGMOID = 1
+};
+typedef struct nnf_moe_routing
+{
+    int k;           /* experts of a token, 1 .. 16 */
+    int score;       /* nnf_moe_score */
+    int groups;      /* of equal size, 1 .. 16: experts e with e / (E / groups) equal.  1: no groups */
+    int top_groups;  /* groups that a token may use: those whose `group_top` best experts have the largest sum of score + bias */
+    int group_top;   /* 1 or 2 */
+    int renormalize; /* weights are divided by their sum + 1e-20 */
+    float scale;     /* weights are multiplied by this, last */
+} nnf_moe_routing;
+
+/* logits [tokens, E] (nnf_type) -> the k experts with the largest score + bias (bias f32 [E] or NULL) of each token, best first, the lowest
+ * index first among equals:
+ *   experts   i32 [tokens, k]
+ *   weights   f32 [tokens, k]   their scores (without the bias), renormalised, scaled
+ *   offsets   i32 [E + 1]       (token, slot) pairs sorted by expert, then token: expert e's are offsets[e] .. offsets[e + 1] - 1
+ *   rows      i32 [tokens * k]  the token of each pair in that order: the index that quantising rows takes; -1 behind the last
+ *   positions i32 [tokens, k]   where in that order a pair lies
+ * Without a bias experts are compared by their logits, else (and group sums of two) score + bias as if computed in 64 bits.  A logit of
+ * -inf or NaN, or a sum that is -inf or NaN, masks its expert: it comes behind all others of the groups in use, with weight 0.  +inf counts as the
+ * largest fp32 number.  live (i32, on the device; NULL: all): tokens from *live on (a padded batch) have experts -1, weights 0, positions -1.
+ * E up to 1024 and a multiple of groups, k up to top_groups * E / groups, tokens * k up to 2^23 (NNF_ERR_UNSUPPORTED_SHAPE).  No
+ * result may overlap an input, another result or the workspace.  Calls that may run at the same time need a workspace each. */
+NNF_API size_t nnf_moe_route_workspace_bytes(int tokens, int E, int k);
+NNF_API int nnf_moe_route(nnf_stream_t stream, const void* logits, int type, const void* bias, const void* live, const nnf_moe_routing* routing,
+                  void* weights, void* experts, void* rows, void* offsets, void* positions, int tokens, int E,
+                  void* workspace, size_t workspace_bytes);
+
+/* y[t, n] = residual[t, n] + sum_j weights[t, j] * x[positions[t, j], n]; x [rows, N], residual (or NULL) and y [tokens, N] fp16 or bf16 (`type`),
+ * fp32 sums, rounded once.  A position outside 0 .. rows - 1 adds nothing, nor does a weight of 0, whatever lies in its row.  y may be the
+ * residual; it must not overlap the inputs otherwise.  k up to 16, tokens * ceil(N / 512) up to 2^25 (NNF_ERR_UNSUPPORTED_SHAPE). */
+NNF_API int nnf_moe_combine(nnf_stream_t stream, const void* x, const void* weights, const void* positions, const void* residual, void* y,
+                    int type, int tokens, int rows, int k, int N);
+
 #ifdef __cplusplus
 }
 #endif

@@ -76,6 +76,9 @@ KERNEL_ABI = {
     "nnf_mxfp4_grouped_gemm_workspace_bytes": (_c_sz, [_c_int] * 5),
     "nnf_mxfp4_grouped_gemm": (_c_int, [_c_vp] * 7 + [_c_int] * 5 + [_c_vp, _c_sz]),
     "nnf_mxfp4_grouped_gemm_variant": (_c_int, [_c_vp] * 7 + [_c_int] * 6 + [_c_vp, _c_sz]),
+    "nnf_moe_route_workspace_bytes": (_c_sz, [_c_int] * 3),
+    "nnf_moe_route": (_c_int, [_c_vp, _c_vp, _c_int] + [_c_vp] * 8 + [_c_int] * 2 + [_c_vp, _c_sz]),
+    "nnf_moe_combine": (_c_int, [_c_vp] * 6 + [_c_int] * 5),
 }
 
 

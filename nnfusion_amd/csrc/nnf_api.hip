@@ -1,6 +1,7 @@
 // C ABI of libnnf_hip_kernels.so: argument checks, dispatch by shape, error mapping.
 // Declarations and the contract of each entry point are in include/nnf_hip_kernels.h.
 #include "nnf_hip_kernels.h"
+#include "kernels/moe_launch.h"
 #include "kernels/mxfp4_launch.h"
 #include "kernels/nnf_launch.h"
 #include "nnf_mxfp4_plan.h"
@@ -998,6 +999,79 @@ int nnf_mxfp4_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_sca
                            int experts, int M, int N, int K, int act, void* workspace, size_t workspace_bytes)
 {
     return nnf_mxfp4_grouped_gemm_variant(stream, A, a_scales, W, w_scales, offsets, Y, experts, M, N, K, act, NNF_MXFP4_AUTO, workspace, workspace_bytes);
+}
+
+} // extern "C"
+
+// ---- routing and combining ------------------------------------------------------------------------------------------------------
+namespace
+{
+    bool aligned_to(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+} // namespace
+
+extern "C" {
+
+size_t nnf_moe_route_workspace_bytes(int tokens, int E, int k)
+{
+    return tokens > 0 && E > 0 && k > 0 ? nnf::moe::workspace_bytes(tokens, E) : 0;
+}
+
+int nnf_moe_route(nnf_stream_t stream, const void* logits, int type, const void* bias, const void* live, const nnf_moe_routing* routing, void* weights,
+                  void* experts, void* rows, void* offsets, void* positions, int tokens, int E, void* workspace, size_t workspace_bytes)
+{
+    if (!logits || !routing || !weights || !experts || !rows || !offsets || !positions || tokens <= 0 || E <= 0 || routing->k <= 0)
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (type < NNF_TYPE_F16 || type > NNF_TYPE_F32 || (routing->score != NNF_MOE_SOFTMAX && routing->score != NNF_MOE_SIGMOID))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(logits, type == NNF_TYPE_F32 ? 4 : 2))
+        return NNF_ERR_INVALID_ARGUMENT;
+    for (const void* p : {bias, live, (const void*)weights, (const void*)experts, (const void*)rows, (const void*)offsets, (const void*)positions, (const void*)workspace})
+        if (!aligned_to(p, 4))
+            return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::moe::routable(tokens, E, routing->k, routing->groups, routing->top_groups, routing->group_top))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t need = nnf::moe::workspace_bytes(tokens, E);
+    if (need && (!workspace || workspace_bytes < need))
+        return NNF_ERR_WORKSPACE_TOO_SMALL;
+    // what is read, then what is written
+    const size_t pairs = (size_t)tokens * routing->k;
+    const struct
+    {
+        const void* at;
+        size_t bytes;
+    } memory[] = {{logits, (size_t)tokens * E * (type == NNF_TYPE_F32 ? 4 : 2)}, {bias, (size_t)E * 4}, {live, 4}, {weights, pairs * 4}, {experts, pairs * 4},
+                  {rows, pairs * 4}, {offsets, ((size_t)E + 1) * 4}, {positions, pairs * 4}, {need ? workspace : nullptr, need}};
+    for (int i = 3; i < 9; ++i)
+        for (int j = 0; j < i; ++j)
+            if (memory[i].at && memory[j].at && overlap(memory[i].at, memory[i].bytes, memory[j].at, memory[j].bytes))
+                return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_moe_route((hipStream_t)stream, {logits, (const float*)bias, (const int*)live, (float*)weights, (int*)experts, (int*)rows, (int*)offsets,
+                                                            (int*)positions, (uint32_t*)workspace, tokens, E, routing->k, type, routing->score == NNF_MOE_SIGMOID,
+                                                            routing->groups, routing->top_groups, routing->group_top, routing->renormalize != 0, routing->scale});
+}
+
+int nnf_moe_combine(nnf_stream_t stream, const void* x, const void* weights, const void* positions, const void* residual, void* y, int type, int tokens, int rows,
+                    int k, int N)
+{
+    if (!x || !weights || !positions || !y || tokens <= 0 || rows <= 0 || k <= 0 || N <= 0 || (type != NNF_TYPE_F16 && type != NNF_TYPE_BF16))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(x, 2) || !aligned_to(weights, 4) || !aligned_to(positions, 4) || !aligned_to(residual, 2) || !aligned_to(y, 2))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::moe::combinable(tokens, k, N))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t y_bytes = (size_t)tokens * N * 2, pairs = (size_t)tokens * k * 4;
+    if (overlap(y, y_bytes, x, (size_t)rows * N * 2) || overlap(y, y_bytes, weights, pairs) || overlap(y, y_bytes, positions, pairs) ||
+        (residual && residual != y && overlap(y, y_bytes, residual, y_bytes)))
+        return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_moe_combine((hipStream_t)stream, x, (const float*)weights, (const int*)positions, residual, y, tokens, rows, k, N, type == NNF_TYPE_BF16);
 }
 
 } // extern "C"

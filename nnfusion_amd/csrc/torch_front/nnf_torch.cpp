@@ -499,6 +499,89 @@ namespace
         return y.release();
     }
 
+    // ---- routing and combining, on the device that holds their first tensor too
+    bool truth(PyObject* o)
+    {
+        const int v = PyObject_IsTrue(o);
+        if (v < 0)
+            throw Raised();
+        return v != 0;
+    }
+    int type_of(const Tensor& t, bool wide, const char* text)
+    {
+        if (t.scalar_type() == at::kHalf)
+            return NNF_TYPE_F16;
+        if (t.scalar_type() == at::kBFloat16)
+            return NNF_TYPE_BF16;
+        require(wide && t.scalar_type() == at::kFloat, text);
+        return NNF_TYPE_F32;
+    }
+
+    // (logits, k, score, bias, groups, top_groups, group_top, renormalize, scale, tokens, out, workspace) -> (weights, experts, rows, offsets, positions)
+    PyObject* moe_route(Args v)
+    {
+        const Tensor& logits = tensor(v[0]);
+        matrix(logits);
+        require(logits.is_contiguous(), "contiguous logits [tokens, experts]");
+        const int type = type_of(logits, true, "logits: fp16, bf16 or fp32"), tokens = size32(logits.size(0)), E = size32(logits.size(1));
+        const nnf_moe_routing routing = {integer(v[1]), integer(v[2]), integer(v[4]), integer(v[5]), integer(v[6]), truth(v[7]), real(v[8])};
+        const int64_t k = routing.k > 0 ? routing.k : 0, pairs = tokens * k;
+        if (v[3] != Py_None)
+            require(is(tensor(v[3]), at::kFloat, {E}), "bias: contiguous fp32 [experts]");
+        if (v[9] != Py_None)
+            require(tensor(v[9]).scalar_type() == at::kInt && tensor(v[9]).numel() == 1, "tokens: one int32");
+        PyObject* given[5] = {Py_None, Py_None, Py_None, Py_None, Py_None};
+        if (v[10] != Py_None)
+        {
+            require(PyTuple_Check(v[10]) && PyTuple_GET_SIZE(v[10]) == 5, "out: (weights, experts, rows, offsets, positions)");
+            for (int i = 0; i < 5; ++i)
+                given[i] = PyTuple_GET_ITEM(v[10], i);
+        }
+        if (given[0] != Py_None)
+            require(is(tensor(given[0]), at::kFloat, {tokens, k}), "weights: contiguous fp32 [tokens, k]");
+        if (given[1] != Py_None)
+            require(is(tensor(given[1]), at::kInt, {tokens, k}), "experts: contiguous int32 [tokens, k]");
+        if (given[2] != Py_None)
+            require(is(tensor(given[2]), at::kInt, {pairs}), "rows: contiguous int32 [tokens * k]");
+        if (given[3] != Py_None)
+            require(is(tensor(given[3]), at::kInt, {(int64_t)E + 1}), "offsets: contiguous int32 [experts + 1]");
+        if (given[4] != Py_None)
+            require(is(tensor(given[4]), at::kInt, {tokens, k}), "positions: contiguous int32 [tokens, k]");
+        workspace_checked(v[11]);
+        on_device(logits, {v[3], v[9], given[0], given[1], given[2], given[3], given[4], v[11]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+        const Owned weights(output(given[0], {tokens, k}, at::kFloat, logits, "weights")), experts(output(given[1], {tokens, k}, at::kInt, logits, "experts")),
+            rows(output(given[2], {pairs}, at::kInt, logits, "rows")), offsets(output(given[3], {(int64_t)E + 1}, at::kInt, logits, "offsets")),
+            positions(output(given[4], {tokens, k}, at::kInt, logits, "positions"));
+        const Workspace w(v[11], logits, [&] { return nnf_moe_route_workspace_bytes(tokens, E, routing.k); });
+        call("nnf_moe_route", nnf_moe_route, stream(), logits.data_ptr(), type, address(v[3]), address(v[9]), &routing, weights.data(), experts.data(), rows.data(),
+             offsets.data(), positions.data(), tokens, E, w.data, w.bytes);
+        PyObject* const all = PyTuple_Pack(5, weights.object, experts.object, rows.object, offsets.object, positions.object);
+        if (!all)
+            throw Raised();
+        return all;
+    }
+
+    // (x, weights, positions, residual, out)
+    PyObject* moe_combine(Args v)
+    {
+        const Tensor &x = tensor(v[0]), &weights = tensor(v[1]), &positions = tensor(v[2]);
+        matrix(x), matrix(weights);
+        const int type = type_of(x, false, "x: fp16 or bf16"), rows = size32(x.size(0)), n = size32(x.size(1)), tokens = size32(weights.size(0)), k = size32(weights.size(1));
+        require(x.is_contiguous(), "contiguous x [rows, N]");
+        require(is(weights, at::kFloat, {tokens, k}), "weights: contiguous fp32 [tokens, k]");
+        require(is(positions, at::kInt, {tokens, k}), "positions: contiguous int32 [tokens, k]");
+        if (v[3] != Py_None)
+            require(is(tensor(v[3]), x.scalar_type(), {tokens, n}), "residual: contiguous [tokens, N] of x's type");
+        if (v[4] != Py_None)
+            require(is(tensor(v[4]), x.scalar_type(), {tokens, n}), "out: contiguous [tokens, N] of x's type");
+        on_device(x, {v[1], v[2], v[3], v[4]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+        Owned y(output(v[4], {tokens, n}, x.scalar_type(), x, "out"));
+        call("nnf_moe_combine", nnf_moe_combine, stream(), x.data_ptr(), weights.data_ptr(), positions.data_ptr(), address(v[3]), y.data(), type, tokens, rows, k, n);
+        return y.release();
+    }
+
     template <PyObject* (*F)(Args), int N>
     PyObject* entry(PyObject*, Args v, Py_ssize_t n)
     {
@@ -533,7 +616,8 @@ namespace
     PyMethodDef methods[] = {NNF_ENTRY(w4a16_gemm, 7),       NNF_ENTRY(wna16_gemm, 11),      NNF_ENTRY(w4a16_gemm_fused, 14), NNF_ENTRY(fused_mlp_w4a16, 13),
                              NNF_ENTRY(wna16_gemm_fused, 14), NNF_ENTRY(fused_mlp_wna16, 14), NNF_ENTRY(w8a8_gemm, 7),         NNF_ENTRY(w8a8_gemm_acc, 5),
                              NNF_ENTRY(elementwise, 4),       NNF_ENTRY(rms_norm, 4),         NNF_ENTRY(dequantize, 7),        NNF_ENTRY(mxfp4_quantize, 4),
-                             NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 10),        NNF_ENTRY(mxfp4_grouped_gemm, 9), {"set_error", set_error, METH_O, nullptr},
+                             NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 10),        NNF_ENTRY(mxfp4_grouped_gemm, 9),
+                             NNF_ENTRY(moe_route, 12),        NNF_ENTRY(moe_combine, 5),       {"set_error", set_error, METH_O, nullptr},
                              {nullptr, nullptr, 0, nullptr}};
     PyModuleDef module = {PyModuleDef_HEAD_INIT, "nnf_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

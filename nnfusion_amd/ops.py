@@ -317,3 +317,31 @@ def mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, works
     decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here).  The library chooses a
     kernel for all rows of a; where the groups fill little of them, name a variant for the rows there are."""
     return _native.mxfp4_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, workspace, MXFP4_VARIANTS[variant])
+
+
+MOE_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route_workspace_bytes(tokens, experts, k):
+    """Bytes of workspace moe_route wants (0: none)."""
+    return int(_lib.kernels().nnf_moe_route_workspace_bytes(tokens, experts, k))
+
+
+def moe_route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_top=1, renormalize=True, scale=1.0, tokens=None, out=None,
+              workspace=None):
+    """Routing to experts: logits [tokens, experts] (fp16, bf16 or fp32) -> (weights f32 [tokens, k], experts i32 [tokens, k], rows
+    i32 [tokens * k], offsets i32 [experts + 1], positions i32 [tokens, k]).  The k experts with the largest score + bias (bias f32 [experts]),
+    best first, among the top_groups of `groups` groups whose group_top (1 or 2) best ones have the largest sum; ties go to the lowest index.
+    weights: their scores (without the bias), divided by their sum with renormalize, times scale.  rows: the tokens sorted by expert, the `rows`
+    of mxfp4_quantize and fp8_quantize; offsets: the groups of mxfp4_grouped_gemm and fp8_grouped_gemm; positions: where in that order
+    a token's experts have it, for moe_combine.  A logit of -inf or NaN masks its expert (last choice, weight 0).  tokens: one i32 on the
+    device, how many tokens are there (a padded batch): the others have experts and positions -1, weights 0, and their rows come last, as -1.
+    out: the five results' tensors (None for one that is to be allocated)."""
+    return _native.moe_route(logits, k, MOE_SCORES[score], bias, groups, top_groups, group_top, renormalize, scale, tokens, out, workspace)
+
+
+def moe_combine(x, weights, positions, residual=None, out=None):
+    """The experts' rows back to their tokens: out[t] = residual[t] + sum_j weights[t, j] * x[positions[t, j]]; x [rows, N] fp16 or bf16, weights and
+    positions [tokens, k] as moe_route gives them.  fp32 sums, one rounding.  Positions outside x and weights of 0 add nothing.  out may be
+    the residual."""
+    return _native.moe_combine(x, weights, positions, residual, out)
