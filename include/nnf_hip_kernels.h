@@ -529,6 +529,64 @@ NNF_API int nnf_moe_route(nnf_stream_t stream, const void* logits, int type, con
 NNF_API int nnf_moe_combine(nnf_stream_t stream, const void* x, const void* weights, const void* positions, const void* residual, void* y,
                     int type, int tokens, int rows, int k, int N);
 
+/* ---------------------------------------------------------------------------------------------
+ * Block-scaled 8-bit floating point: quantising activations and weights, the product, and the product grouped by expert.  The product
+ * stands where nnf_w8a8_gemm does, quantising where the reference's Dequantize has its inverse; the reference has neither.
+ *   codes   u8 [rows, K]    E4M3 of the OCP 8-bit formats: sign, four exponent bits, three mantissa bits; largest 448, 0x7F and 0xFF NaN
+ *   scales of activations   f32 [ceil(K / 128), rows]: a row's 128 values along K share one
+ *   scales of weights       f32 [ceil(N / 128), ceil(K / 128)]: a block of 128 x 128 shares one; with NNF_ACT_SILU_GATE those of the N gate
+ *                           rows, then those of the N up rows (f32 [2 ceil(N / 128), ceil(K / 128)]: for N no multiple of 128 the up rows'
+ *                           blocks start anew)
+ * K a multiple of 16 up to 2^22 (NNF_ERR_UNSUPPORTED_SHAPE otherwise); the last block of K or N may be short.  The products of a block's values
+ * and their sum are fp32 (in the order of the matrix cores), so are the products with the scales and the sum over blocks; the result is
+ * rounded once, behind bias, residual or SiLU-gate.  Scales of any value: where one is NaN, what it belongs to is.  Every size is at least
+ * 1.  Scales, index and offsets need the alignment of their element only.  No function here needs a workspace or keeps state, the same call
+ * gives the same bits, and what belongs to one row or column of a product does not touch another.
+ * ------------------------------------------------------------------------------------------- */
+/* x [source_rows, K] fp16 or bf16 (`type`) -> codes and scales of `rows` rows: row i is x's row index[i] (i32 [rows] on the device; zeros
+ * where x has no such row), or x's row i where index is NULL (then rows == source_rows).  scale = max(largest magnitude, 2^-64) / 448, code =
+ * the E4M3 nearest to x / scale, ties to even, both quotients rounded to fp32; a block with an infinity or NaN has scale NaN and zero
+ * codes.  The results must not overlap each other, x or index; rows * ceil(K / 512) up to 2^28 - 16 (NNF_ERR_UNSUPPORTED_SHAPE above). */
+NNF_API int nnf_fp8_quantize(nnf_stream_t stream, const void* x, int type, const void* index, void* codes, void* scales,
+                     int rows, int source_rows, int K);
+/* w [matrices, N, K] -> codes [matrices, N, K], scales [matrices, ceil(N / 128), ceil(K / 128)].  (Gate and up rows are two matrices: the
+ * result with matrices = 2 is the operand of a product with SiLU-gate.)  Fewer than 2^23 blocks in all. */
+NNF_API int nnf_fp8_quantize_weights(nnf_stream_t stream, const void* w, int type, void* codes, void* scales, int matrices, int N, int K);
+
+/* Y [M, N] = A . W^T + bias + residual, or with act == NNF_ACT_SILU_GATE (W has 2N rows: gate rows, then up rows; no bias, no residual)
+ * SiLU(gate) * up.  Y, bias [N] and residual [M, N] fp16 or bf16 (`type`); the latter may be NULL, the residual may be Y itself.  Y must
+ * not overlap the operands otherwise.  NNF_ERR_UNSUPPORTED_SHAPE: N above 2^29, M above 2^30, N * K of 2^31 or more with SiLU-gate, more tiles than
+ * a grid holds (2^23 of the kernel's; the automatic choice passes over kernels with too small tiles). */
+NNF_API int nnf_fp8_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type,
+                 int M, int N, int K, const void* bias, const void* residual, int act);
+
+/* The kernels behind the two products as selectable variants (see nnf_w4a16_variant): activation rows x weight rows of a workgroup's
+ * tile.  Each serves every shape whose tiles fit into a grid of its own.  NNF_FP8_AUTO: by the shape. */
+enum nnf_fp8_variant
+{
+    NNF_FP8_AUTO = 0,
+    NNF_FP8_TILE_16x32 = 1, /* a wavefront for each range of K: one, two, four */
+    NNF_FP8_TILE_16x32_2 = 2,
+    NNF_FP8_TILE_16x32_4 = 3,
+    NNF_FP8_TILE_32x64 = 4, /* four */
+    NNF_FP8_TILE_64x64 = 5, /* the wavefronts share the tile */
+    NNF_FP8_TILE_64x128 = 6,
+    NNF_FP8_TILE_128x128 = 7
+};
+NNF_API int nnf_fp8_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type,
+                         int M, int N, int K, const void* bias, const void* residual, int act, int variant);
+
+/* The product of a mixture's experts: rows of A [M, K] and Y [M, N] sorted by expert, one weight matrix each (W u8 [experts, N, K], 2N rows with
+ * NNF_ACT_SILU_GATE, and their scales behind each other).  Group e is the rows offsets[e] .. offsets[e + 1] - 1; offsets i32 [experts + 1] on
+ * the device, not decreasing, within 0 .. M: a group may be empty, and rows before offsets[0] or from offsets[experts] on are left as
+ * they are in Y.  (Offsets that break this give undefined rows of Y, never an access outside the operands.)  Sizes as above; experts above
+ * 2^30 are NNF_ERR_UNSUPPORTED_SHAPE.  The kernel is chosen for M rows, as if the groups filled the buffer: where they fill little of a
+ * large one, name a variant for the rows there are. */
+NNF_API int nnf_fp8_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets,
+                         void* Y, int type, int experts, int M, int N, int K, int act);
+NNF_API int nnf_fp8_grouped_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales,
+                                 const void* offsets, void* Y, int type, int experts, int M, int N, int K, int act, int variant);
+
 #ifdef __cplusplus
 }
 #endif

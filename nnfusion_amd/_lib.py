@@ -79,6 +79,12 @@ KERNEL_ABI = {
     "nnf_moe_route_workspace_bytes": (_c_sz, [_c_int] * 3),
     "nnf_moe_route": (_c_int, [_c_vp, _c_vp, _c_int] + [_c_vp] * 8 + [_c_int] * 2 + [_c_vp, _c_sz]),
     "nnf_moe_combine": (_c_int, [_c_vp] * 6 + [_c_int] * 5),
+    "nnf_fp8_quantize": (_c_int, [_c_vp, _c_vp, _c_int] + [_c_vp] * 3 + [_c_int] * 3),
+    "nnf_fp8_quantize_weights": (_c_int, [_c_vp, _c_vp, _c_int] + [_c_vp] * 2 + [_c_int] * 3),
+    "nnf_fp8_gemm": (_c_int, [_c_vp] * 6 + [_c_int] * 4 + [_c_vp, _c_vp, _c_int]),
+    "nnf_fp8_gemm_variant": (_c_int, [_c_vp] * 6 + [_c_int] * 4 + [_c_vp, _c_vp, _c_int, _c_int]),
+    "nnf_fp8_grouped_gemm": (_c_int, [_c_vp] * 7 + [_c_int] * 6),
+    "nnf_fp8_grouped_gemm_variant": (_c_int, [_c_vp] * 7 + [_c_int] * 7),
 }
 
 

@@ -1,0 +1,464 @@
+// Block-scaled E4M3 x E4M3 in tiles through LDS.
+//
+// v_mfma_f32_32x32x64: lane l holds 32 values of row l % 32.  K goes in steps of 128 values -- 128 bytes of a row, a whole line of memory,
+// and one block of scales --: two MFMAs give a fragment of 32 x 32 its products of the step, which are then added to the sums times the
+// activation row's and the weight block's scale, 16 fma and one product of the vector units beside 128 cycles of the matrix cores.  The
+// weights are the A operand: a lane's 16 results are columns of one row of Y, and their scale is one number a lane.  The fma of a
+// fragment go between the MFMAs of the next one (of the next step, for a step's last), so that neither waits for the other.
+//
+// Sums are fp32.  Of eight products of neighbouring k the matrix cores keep what lies within 2^-13 of the power of two of the largest (cut towards
+// zero, measured with single products), and add these in fp32: 2^-16 of the sums' root mean square for normal data, a thousandth of what E4M3's own
+// rounding costs.  The exact products would take MFMAs of bf16, at half the rate.
+#include "fp8_launch.h"
+#include "nnf_launch.h"
+
+namespace nnf
+{
+    namespace
+    {
+        using namespace fp8;
+
+        constexpr int STEP_BYTES = 128; // of a row: a block of K
+
+        // WK groups of WM x WN wavefronts; a group has the whole tile over its part of K, a wavefront FM x 32 activation rows and FN x 32
+        // weight rows of it (ROWS below 32: that many rows of a fragment are fetched, the others repeat them).  LDS, a group: S steps of
+        // codes, and scales of activations twice for G steps, 64 rows to a load
+        template <int WM_, int WN_, int WK_, int FM_, int FN_, int S_, int G_, int ROWS_ = WM_ * FM_ * 32>
+        struct Tile
+        {
+            static constexpr int WM = WM_, WN = WN_, WK = WK_, FM = FM_, FN = FN_, S = S_, G = G_;
+            static constexpr int GROUP = WM * WN, WAVES = GROUP * WK, ROWS = ROWS_, COLS = WN * FN * 32;
+            static constexpr int LOADS = (ROWS + COLS) / 8 / GROUP;                   // of codes, a step and wavefront
+            static constexpr int ALL_SCALE_LOADS = (G * ROWS + WAVE - 1) / WAVE;      // for G steps
+            static constexpr int SCALE_LOADS = (ALL_SCALE_LOADS + GROUP - 1) / GROUP; // of a wavefront
+            static constexpr int STAGE = (ROWS + COLS) * STEP_BYTES, SCALES = ALL_SCALE_LOADS * WAVE * 4;
+            static constexpr int GROUP_LDS = S * STAGE + 2 * SCALES;
+            static constexpr int PITCH = FN * 128 + 16; // fp32 results of a row of a wavefront
+            static constexpr int LDS = GROUP_LDS * WK > WAVES * 32 * PITCH ? GROUP_LDS * WK : WAVES * 32 * PITCH;
+            static_assert((ROWS == WM * FM * 32 || (ROWS < 32 && GROUP * FM == 1)) && (ROWS + COLS) / 8 % GROUP == 0, "whole loads");
+            static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && S >= 2 && (S - 1) * LOADS < 64, "room for them, and a count");
+        };
+
+        template <int OFFSET>
+        __device__ __forceinline__ void lds_read_b32_nowait(float& dst, uint32_t addr)
+        {
+            asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(dst) : "v"(addr), "n"(OFFSET) : "memory");
+        }
+        // 16 bytes a lane, 4 bytes a lane
+        __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds)
+        {
+            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(base + offset), (void __attribute__((address_space(3)))*)(uintptr_t)lds, 16, 0, 0);
+        }
+        __device__ __forceinline__ void number_to_lds(const float* from, uint32_t lds)
+        {
+            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)from, (void __attribute__((address_space(3)))*)(uintptr_t)lds, 4, 0, 0);
+        }
+        // until at most N of this wavefront's loads are under way
+        template <int N>
+        __device__ __forceinline__ void wait_loads()
+        {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+        }
+
+        // What lanes have written to LDS is there for the lanes that read it, and what they have read may be written over.  WK: the ranges of
+        // K that meet.  One: only lanes of the same wavefront do, whose accesses LDS takes in the order of the code -- no instruction, but
+        // the compiler has to keep that order
+        template <int WK>
+        __device__ __forceinline__ void lanes_meet()
+        {
+            if constexpr (WK > 1)
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else
+            {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            }
+        }
+
+        template <class T, bool GATE>
+        __global__ __launch_bounds__(T::WAVES* WAVE, 2) void fp8_tile_kernel(Operands o, int col_tiles)
+        {
+            extern __shared__ __align__(256) uint8_t lds[];
+            const int lane = threadIdx.x & (WAVE - 1), wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+            const int group = wave_id / T::GROUP, wave = wave_id % T::GROUP;
+            TileAt rows;
+            if (!find_tile(o, blockIdx.x, T::ROWS, col_tiles, rows))
+                return;
+            constexpr int OUT = GATE ? T::COLS / 2 : T::COLS; // columns of Y
+            const int n0 = rows.column * OUT;
+            const int row_bytes = o.K;
+            const int all_steps = blocks_of(o.K);
+            // this group's steps (none, where the groups before have them all)
+            const int part = (all_steps + T::WK - 1) / T::WK, first_step = group * part;
+            const int steps = max(min(part, all_steps - first_step), 0);
+            const size_t w_row = (size_t)rows.expert * (GATE ? 2 * (size_t)o.N : o.N) + n0;
+            const int there = rows.end - rows.first; // rows of the tile and behind it
+
+            // ---- what this wavefront fetches: rows of the tile in memory order, weights first, eight to a load
+            // row `i` of the tile's weight rows, counted from its first: with SiLU-gate a wavefront's columns are half gate rows, half their
+            // up rows
+            const auto weight_row = [&](int i) {
+                if constexpr (GATE)
+                {
+                    constexpr int HALF = T::FN * 16;
+                    const int in = i % (2 * HALF);
+                    return min(i / (2 * HALF) * HALF + in % HALF, o.N - 1 - n0) + (in >= HALF ? o.N : 0);
+                }
+                else
+                    return min(i, o.N - 1 - n0);
+            };
+            const uint8_t* const a_base = o.A + (size_t)rows.first * row_bytes;
+            const uint8_t* const w_base = o.W + w_row * row_bytes;
+            uint32_t offset[T::LOADS];
+            const auto load_base = [&](auto j) { return (wave * T::LOADS + (T::COLS % (T::LOADS * 8) == 0 ? 0 : (int)j)) * 8 >= T::COLS ? a_base : w_base; };
+            // piece of a row (16 bytes) that lies at slot `lane % 8` of row `row` in LDS: XORed so that the reads of 16 rows' pieces
+            // spread over all banks
+            const auto piece = [&](int row) { return (lane & 7) ^ ((row >> 1) & 7); };
+#pragma unroll
+            for (int j = 0; j < T::LOADS; ++j)
+            {
+                const int row = (wave * T::LOADS + j) * 8 + (lane >> 3);
+                const int at = row < T::COLS ? weight_row(row) : min(row - T::COLS, there - 1);
+                offset[j] = (uint32_t)at * row_bytes + piece(row) * 16;
+            }
+            const uint32_t codes_at = lds_address(lds) + group * T::GROUP_LDS, scales_at = codes_at + T::S * T::STAGE;
+            // scales of G steps, a number a lane, a step's rows behind each other (where there are fewer loads than wavefronts, some fetch the
+            // same again; behind the last step: that one's, not used)
+            const auto fetch_scales = [&](int step) {
+#pragma unroll
+                for (int p = 0; p < T::SCALE_LOADS; ++p)
+                {
+                    const int q = min(p * T::GROUP + wave, T::ALL_SCALE_LOADS - 1), i = q * WAVE + lane;
+                    const int at = min(first_step + step + i / T::ROWS, all_steps - 1);
+                    number_to_lds(o.As + ((size_t)at * o.M + rows.first + min(i % T::ROWS, there - 1)), scales_at + (step / T::G & 1) * T::SCALES + q * (WAVE * 4));
+                }
+            };
+            // codes of a step, load by load.  FULL: the step ends within the rows; else a row's last piece stands for those behind its end, and
+            // is not used
+            const auto fetch_load = [&](auto j, int step, uint32_t stage, auto full) {
+                uint32_t from = offset[j];
+                int k0 = (first_step + step) * STEP_BYTES;
+                if constexpr (!full)
+                {
+                    const int p = piece((wave * T::LOADS + j) * 8 + (lane >> 3)) * 16;
+                    from += min(p, row_bytes - 16 - k0) - p;
+                }
+                else
+                    asm("" : "+v"(from)); // (or the compiler keeps a 64-bit address for each load: base + offset stays an address of two parts)
+                load_to_lds(load_base(j) + k0, from, codes_at + stage + (wave * T::LOADS + j) * 1024);
+            };
+            const auto fetch = [&](int step, uint32_t stage) {
+                unroll_for<0, T::LOADS>([&](auto j) { fetch_load(j, step, stage, std::false_type{}); });
+            };
+            // a step that does not end within the rows, landed: what this wavefront has fetched of the weights from behind their end becomes
+            // zeros (the activations there repeat values of their row: NaN only in rows that are NaN anyway)
+            const auto cut = [&](int step, uint32_t stage) {
+                const int pieces = (row_bytes >> 4) - (first_step + step) * 8;
+                unroll_for<0, T::LOADS>([&](auto j) {
+                    const int row = (wave * T::LOADS + j) * 8;
+                    if (row < T::COLS && piece(row + (lane >> 3)) >= pieces)
+                        *reinterpret_cast<uintx4*>(lds + group * T::GROUP_LDS + stage + row * STEP_BYTES + lane * 16) = uintx4{0, 0, 0, 0};
+                });
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            };
+            const auto ends_outside = [&](int step) { return (first_step + step + 1) * STEP_BYTES > row_bytes; };
+            // until no more than `steps` steps' loads are under way (scales asked for since then make it wait for more, never for less)
+            const auto landed_but = [&](int steps) {
+                unroll_for<1, T::S>([&](auto n) {
+                    if (steps == n)
+                        wait_loads<n * T::LOADS>();
+                });
+                if (steps <= 0)
+                    wait_loads<0>();
+            };
+            // ahead of the reads of step `step`: it is there, for all wavefronts of the group
+            const auto arrive = [&](int step, uint32_t stage, auto full) {
+                if constexpr (full)
+                    wait_loads<(T::S - 2) * T::LOADS>();
+                else if (step < steps && ends_outside(step))
+                {
+                    wait_loads<0>();
+                    cut(step, stage);
+                }
+                else
+                    landed_but(min(T::S - 2, steps - 1 - step));
+                if constexpr (T::GROUP > 1)
+                    asm volatile("s_barrier" ::: "memory");
+            };
+
+            // ---- what it reads from LDS
+            const int r = lane & 31, g = lane >> 5;
+            const int wave_n = wave % T::WN, wave_m = wave / T::WN;
+            uint32_t w_at[4], a_at[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+            {
+                const auto in_row = [&](int row) { return row * STEP_BYTES + (((4 * g + s) ^ ((row >> 1) & 7)) << 4); };
+                w_at[s] = codes_at + wave_n * T::FN * 32 * STEP_BYTES + in_row(r);
+                a_at[s] = codes_at + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES + in_row(r % T::ROWS);
+            }
+            const uint32_t as_at = scales_at + (wave_m * T::FM * 32 + r % T::ROWS) * 4;
+
+            // scales of the weights: a wavefront's columns lie in one block of them (with SiLU-gate in one of the gate's and one of the up rows'); a lane
+            // has those of one of 64 steps
+            constexpr int NS = GATE ? 2 : 1;
+            const int n_blocks = blocks_of(o.N), n_block = min((n0 + wave_n * T::FN * (GATE ? 16 : 32)) / BLOCK, n_blocks - 1);
+            const float* const ws_base = o.Ws + ((size_t)rows.expert * (NS * n_blocks) + n_block) * all_steps;
+            float ws[NS];
+            const auto load_weight_scales = [&](int step) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                {
+                    ws[i] = ws_base[(size_t)i * n_blocks * all_steps + min(first_step + step + lane, all_steps - 1)];
+                    asm volatile("" : "+v"(ws[i])); // (waited for here, not inside the loop)
+                }
+            };
+
+            constexpr int B = T::FN * T::FM;
+            floatx16 sum[T::FN][T::FM] = {};
+            floatx16 product[2] = {};                      // of a fragment and of the one before
+            intx8 wf[2][T::FN][2], af[2][T::FM][2];        // operands of a step and of the next
+            uintx4 w_read[T::FN][4], a_read[T::FM][4];     // the halves of those, on their way
+            float as[T::FM], as_next[T::FM], scale[NS] = {}; // scale: of the products that wait
+
+            const auto read_scales = [&](int step) {
+                const uint32_t from = as_at + (step / T::G & 1) * T::SCALES + step % T::G * (T::ROWS * 4);
+                unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * 128>(as_next[f], from); });
+            };
+            constexpr int READS = (T::FN + T::FM) * 4;
+            const auto read_piece = [&](auto q, uint32_t stage) {
+                constexpr int f = q / 4, s = q % 4;
+                if constexpr (f < T::FN)
+                    lds_read_b128_nowait<f * 32 * STEP_BYTES>(w_read[f][s], w_at[s] + stage);
+                else
+                    lds_read_b128_nowait<(f - T::FN) * 32 * STEP_BYTES>(a_read[f - T::FN][s], a_at[s] + stage);
+            };
+            // nothing read without a wait stays in flight past the straight line of code that asked for it
+            const auto landed = [&](auto set) {
+                lds_wait<0>(w_read[0][0]);
+                unroll_for<0, 4>([&](auto s) {
+                    unroll_for<0, T::FN>([&](auto f) { lds_wait_also(w_read[f][s]); });
+                    unroll_for<0, T::FM>([&](auto f) { lds_wait_also(a_read[f][s]); });
+                });
+                unroll_for<0, 2>([&](auto h) {
+                    unroll_for<0, T::FN>([&](auto f) { wf[set][f][h] = operand(w_read[f][2 * h], w_read[f][2 * h + 1]); });
+                    unroll_for<0, T::FM>([&](auto f) { af[set][f][h] = operand(a_read[f][2 * h], a_read[f][2 * h + 1]); });
+                });
+                unroll_for<0, T::FM>([&](auto f) {
+                    lds_wait_also(as_next[f]);
+                    as[f] = as_next[f];
+                });
+            };
+            // half h of the products of fragment i that wait
+            const auto add = [&](auto i, auto which, auto h) {
+                constexpr int fn = i % T::FN, fm = i / T::FN;
+#pragma unroll
+                for (int e = h * 8; e < h * 8 + 8; ++e)
+                {
+                    // (SiLU-gate with one fragment of columns: its first 16 are gate rows, its results 0 .. 7; else a fragment is one or the other)
+                    constexpr int of_fragment = GATE && T::FN > 1 ? fn * 2 / T::FN : 0;
+                    sum[fn][fm][e] = __builtin_fmaf(product[which][e], scale[GATE && T::FN == 1 ? h : of_fragment], sum[fn][fm][e]);
+                }
+            };
+
+            // a step: what comes S steps later is asked for and the next step's fragments are read, between its MFMAs.  FULL: that step ends within
+            // the rows
+            uint32_t stage = 0;
+            const auto body = [&](int step, auto set, auto full) {
+                using Next = std::integral_constant<int, 1 - set>;
+                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                if ((step & (WAVE - 1)) == 0 && step > 0)
+                    load_weight_scales(step);
+                float of_step[NS];
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    of_step[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ws[i]), step & (WAVE - 1)));
+                arrive(step + 1, next_stage, full);
+                if (step % T::G == 0 && step + T::G < steps)
+                    fetch_scales(step + T::G);
+                if (!full && step + T::S < steps)
+                    fetch(step + T::S, stage);
+                read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
+                unroll_for<0, B>([&](auto b) {
+                    constexpr int fn = b % T::FN, fm = b / T::FN;
+                    constexpr int SLOTS = 2 * B, EACH = (READS + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
+                    constexpr int mine = (set * B + b) & 1;
+                    unroll_for<0, 2>([&](auto h) {
+                        constexpr int slot = 2 * b + h;
+                        unroll_for<0, EACH>([&](auto q) {
+                            if constexpr (slot * EACH + q < READS)
+                                read_piece(std::integral_constant<int, slot * EACH + q>{}, next_stage);
+                        });
+                        if constexpr (full)
+                            unroll_for<0, FETCHES>([&](auto q) {
+                                if constexpr (slot * FETCHES + q < T::LOADS)
+                                    fetch_load(std::integral_constant<int, slot * FETCHES + q>{}, step + T::S, stage, std::true_type{});
+                            });
+                        product[mine] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[set][fn][h], af[set][fm][h], h == 0 ? floatx16{} : product[mine], E4M3, E4M3, 0, 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        add(std::integral_constant<int, (b + B - 1) % B>{}, std::integral_constant<int, 1 - mine>{}, h);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+#pragma unroll
+                    for (int i = 0; i < NS; ++i)
+                        scale[i] = as[fm] * of_step[i];
+                });
+                landed(Next{});
+                stage = next_stage;
+            };
+
+            if (steps > 0)
+            {
+                fetch_scales(0);
+#pragma unroll
+                for (int i = 0; i < T::S; ++i)
+                    if (i < steps)
+                        fetch(i, i * T::STAGE);
+                load_weight_scales(0);
+                if (ends_outside(0))
+                {
+                    wait_loads<0>();
+                    cut(0, 0);
+                }
+                else
+                    landed_but(min(T::S, steps) - 1);
+                if constexpr (T::GROUP > 1)
+                    asm volatile("s_barrier" ::: "memory");
+                // wavefronts whose rows all lie behind the group's end (a block of few rows in a tall tile) fetch for the others, no more
+                const bool idle = T::WM > 1 && wave_m * T::FM * 32 >= there;
+                int step = 0;
+                if (idle)
+                {
+#pragma unroll 1
+                    for (; step < steps; ++step)
+                    {
+                        const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                        arrive(step + 1, next_stage, std::false_type{});
+                        if (step % T::G == 0 && step + T::G < steps)
+                            fetch_scales(step + T::G);
+                        if (step + T::S < steps)
+                            fetch(step + T::S, stage);
+                        stage = next_stage;
+                    }
+                }
+                else
+                {
+                    using Even = std::integral_constant<int, 0>;
+                    using Odd = std::integral_constant<int, 1>;
+                    read_scales(0);
+                    unroll_for<0, READS>([&](auto q) { read_piece(q, 0); });
+                    landed(Even{});
+                    const int whole = min(steps, max(row_bytes / STEP_BYTES - first_step, 0)); // steps that end within the rows
+#pragma unroll 1
+                    for (; step + 1 + T::S < whole; step += 2)
+                    {
+                        body(step, Even{}, std::true_type{});
+                        body(step + 1, Odd{}, std::true_type{});
+                    }
+#pragma unroll 1
+                    for (; step < steps; step += 2)
+                    {
+                        body(step, Even{}, std::false_type{});
+                        if (step + 1 < steps)
+                            body(step + 1, Odd{}, std::false_type{});
+                        else if constexpr (B % 2 != 0)
+                            product[1] = product[0]; // (the last products, where two steps leave them)
+                    }
+                    unroll_for<0, 2>([&](auto h) { add(std::integral_constant<int, B - 1>{}, std::integral_constant<int, 1>{}, h); });
+                }
+            }
+
+            // ---- Y: lane l of a fragment has columns 8 (i / 4) + 4 (l / 32) + i % 4 of row l % 32.  A block of 32 rows at a time goes through
+            // LDS in fp32; there the groups' parts are added up, in their order, and whole rows leave, 16 bytes a lane
+            constexpr int MY_COLS = T::FN * (GATE ? 16 : 32); // columns of Y of a wavefront
+            constexpr int LANES = MY_COLS / 8, PASSES = 32 * LANES / WAVE, MINE = (PASSES + T::WK - 1) / T::WK;
+            static_assert(32 * LANES % WAVE == 0, "whole passes");
+            const int n = n0 + wave_n * MY_COLS + lane % LANES * 8;
+            uint8_t* const block = lds + wave * (32 * T::PITCH); // the first group's; the others' behind it
+            constexpr int PART = T::GROUP * 32 * T::PITCH;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+            for (int fm = 0; fm < T::FM; ++fm)
+            {
+                if (fm > 0)
+                    lanes_meet<T::WK>();
+#pragma unroll
+                for (int fn = 0; fn < T::FN; ++fn)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<floatx4*>(block + group * PART + r * T::PITCH + fn * 128 + q * 32 + g * 16) =
+                            floatx4{sum[fn][fm][q * 4], sum[fn][fm][q * 4 + 1], sum[fn][fm][q * 4 + 2], sum[fn][fm][q * 4 + 3]};
+                lanes_meet<T::WK>();
+                floatx4 y[MINE][2];
+#pragma unroll
+                for (int i = 0; i < MINE; ++i)
+                {
+                    const uint8_t* const at = block + ((i * T::WK + group) % PASSES * (WAVE / LANES) + lane / LANES) * T::PITCH + lane % LANES * 32;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        y[i][h] = *reinterpret_cast<const floatx4*>(at + h * 16);
+#pragma unroll
+                        for (int k = 1; k < T::WK; ++k)
+                            y[i][h] += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16);
+                        if constexpr (GATE)
+                        {
+                            floatx4 up = *reinterpret_cast<const floatx4*>(at + h * 16 + MY_COLS * 4);
+#pragma unroll
+                            for (int k = 1; k < T::WK; ++k)
+                                up += *reinterpret_cast<const floatx4*>(at + k * PART + h * 16 + MY_COLS * 4);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[i][h][e] = silu_gate(y[i][h][e], up[e]);
+                        }
+                    }
+                }
+                const int first = rows.first + (wave_m * T::FM + fm) * 32 + lane / LANES;
+                const auto row = [&](int i) {
+                    const int pass = i * T::WK + group, m = first + pass * (WAVE / LANES);
+                    return pass < PASSES && m < rows.end && (T::ROWS >= 32 || m < rows.first + T::ROWS) ? m : -1;
+                };
+                if (n < o.N)
+                {
+                    if (o.bf16)
+                        write_rows<bf16_t, MINE>(o, y, n, row);
+                    else
+                        write_rows<half_t, MINE>(o, y, n, row);
+                }
+            }
+        }
+
+        template <class T, bool GATE>
+        hipError_t launch(hipStream_t s, const Operands& o)
+        {
+            static LdsGrant granted;
+            const hipError_t e = allow_dynamic_lds((const void*)fp8_tile_kernel<T, GATE>, granted, T::LDS);
+            if (e != hipSuccess)
+                return e;
+            const int col_tiles = column_tiles(o.N, T::COLS, GATE);
+            fp8_tile_kernel<T, GATE><<<(unsigned)(row_blocks(o, T::ROWS) * col_tiles), T::WAVES * WAVE, T::LDS, s>>>(o, col_tiles);
+            return hipGetLastError();
+        }
+        template <class T>
+        hipError_t launch_either(hipStream_t s, const Operands& o, bool gate)
+        {
+            return gate ? launch<T, true>(s, o) : launch<T, false>(s, o);
+        }
+    } // namespace
+
+    hipError_t launch_fp8_tiles(hipStream_t s, const fp8::Operands& o, int kernel, bool gate)
+    {
+        // wavefronts in rows x columns x ranges of K, fragments of rows x columns, steps under way, steps of a load of scales
+        switch (kernel)
+        {
+        case fp8::TILE_16x32: return launch_either<Tile<1, 1, 1, 1, 1, 4, 4, 16>>(s, o, gate);
+        case fp8::TILE_16x32_2: return launch_either<Tile<1, 1, 2, 1, 1, 4, 4, 16>>(s, o, gate);
+        case fp8::TILE_16x32_4: return launch_either<Tile<1, 1, 4, 1, 1, 4, 4, 16>>(s, o, gate);
+        case fp8::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2, 2>>(s, o, gate);
+        case fp8::TILE_64x64: return launch_either<Tile<2, 2, 1, 1, 1, 4, 4>>(s, o, gate);
+        case fp8::TILE_64x128: return launch_either<Tile<2, 2, 1, 1, 2, 3, 4>>(s, o, gate);
+        default: return launch_either<Tile<2, 2, 1, 2, 2, 2, 2>>(s, o, gate);
+        }
+    }
+} // namespace nnf

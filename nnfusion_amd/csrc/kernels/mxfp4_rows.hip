@@ -137,7 +137,7 @@ namespace nnf
                 }
                 const int m = rows.first + r;
                 if (m < rows.end)
-                    write_four(o, y, m, n0 + f * 16 + g * 4);
+                    write_four<half_t>(o, y, m, n0 + f * 16 + g * 4);
             }
         }
 

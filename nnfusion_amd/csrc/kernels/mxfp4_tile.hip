@@ -486,7 +486,7 @@ namespace nnf
                 }
                 const int first = rows.first + (wave_m * T::FM + fm) * 32 + lane / LANES;
                 if (n < o.N)
-                    write_rows<MINE>(o, y, n, [&](int i) {
+                    write_rows<half_t, MINE>(o, y, n, [&](int i) {
                         const int pass = i * T::WK + group, m = first + pass * (WAVE / LANES);
                         return pass < PASSES && m < rows.end && (T::ROWS >= 32 || m < rows.first + T::ROWS) ? m : -1;
                     });

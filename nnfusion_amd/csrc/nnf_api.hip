@@ -1,6 +1,7 @@
 // C ABI of libnnf_hip_kernels.so: argument checks, dispatch by shape, error mapping.
 // Declarations and the contract of each entry point are in include/nnf_hip_kernels.h.
 #include "nnf_hip_kernels.h"
+#include "kernels/fp8_launch.h"
 #include "kernels/moe_launch.h"
 #include "kernels/mxfp4_launch.h"
 #include "kernels/nnf_launch.h"
@@ -1072,6 +1073,116 @@ int nnf_moe_combine(nnf_stream_t stream, const void* x, const void* weights, con
     if (st != NNF_OK)
         return st;
     return (int)nnf::launch_moe_combine((hipStream_t)stream, x, (const float*)weights, (const int*)positions, residual, y, tokens, rows, k, N, type == NNF_TYPE_BF16);
+}
+
+} // extern "C"
+
+// ---- block-scaled 8-bit floating point --------------------------------------------------------------------------------------------
+namespace
+{
+    bool sixteen_bits(int type) { return type == NNF_TYPE_F16 || type == NNF_TYPE_BF16; }
+
+    // what the two products have in common; offsets == null: one weight matrix
+    int fp8_product(nnf_stream_t stream, const nnf::fp8::Operands& o, int type, int act, int variant)
+    {
+        using namespace nnf::fp8;
+        static_assert((int)NNF_FP8_TILE_128x128 == (int)KERNELS, "variants and kernels in one order, automatic choice first");
+        if (!o.A || !o.As || !o.W || !o.Ws || !o.Y || o.M <= 0 || o.N <= 0 || o.K <= 0 || o.experts <= 0 || !sixteen_bits(type))
+            return NNF_ERR_INVALID_ARGUMENT;
+        if ((act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE) || variant < 0 || variant > KERNELS)
+            return NNF_ERR_INVALID_ARGUMENT;
+        for (const void* p : {(const void*)o.A, (const void*)o.W, (const void*)o.Y, o.bias, o.residual})
+            if (!aligned16(p))
+                return NNF_ERR_INVALID_ARGUMENT;
+        if (!aligned_to(o.As, 4) || !aligned_to(o.Ws, 4) || !aligned_to(o.offsets, 4))
+            return NNF_ERR_INVALID_ARGUMENT;
+        const bool gate = act == NNF_ACT_SILU_GATE;
+        const int experts = o.offsets ? o.experts : 0;
+        if (!servable(o.M, o.N, o.K, gate, experts) || (gate && (o.bias || o.residual)))
+            return NNF_ERR_UNSUPPORTED_SHAPE;
+        const size_t y_bytes = (size_t)o.M * o.N * 2, matrices = (size_t)o.experts * (gate ? 2 : 1);
+        // (workgroups still read when others write)
+        if (overlap(o.Y, y_bytes, o.A, (size_t)o.M * o.K) || overlap(o.Y, y_bytes, o.As, (size_t)o.M * blocks_of(o.K) * 4) ||
+            overlap(o.Y, y_bytes, o.W, matrices * o.N * o.K) || overlap(o.Y, y_bytes, o.Ws, matrices * blocks_of(o.N) * blocks_of(o.K) * 4) ||
+            (o.bias && overlap(o.Y, y_bytes, o.bias, (size_t)o.N * 2)) || (o.offsets && overlap(o.Y, y_bytes, o.offsets, ((size_t)o.experts + 1) * 4)) ||
+            (o.residual && o.residual != o.Y && overlap(o.Y, y_bytes, o.residual, y_bytes)))
+            return NNF_ERR_INVALID_ARGUMENT;
+        DeviceInfo dev;
+        const int st = current_device_info(dev);
+        if (st != NNF_OK)
+            return st;
+        const int kernel = variant != NNF_FP8_AUTO ? variant - 1 : choose(o.M, o.N, o.K, gate, experts, dev.num_cu);
+        if (!fits(FACTS[kernel], o.M, o.N, gate, experts))
+            return NNF_ERR_UNSUPPORTED_SHAPE; // (of a variant that the caller names)
+        return (int)nnf::launch_fp8_tiles((hipStream_t)stream, o, kernel, gate);
+    }
+} // namespace
+
+extern "C" {
+
+int nnf_fp8_quantize(nnf_stream_t stream, const void* x, int type, const void* index, void* codes, void* scales, int rows, int source_rows, int K)
+{
+    if (!x || !codes || !scales || rows <= 0 || source_rows <= 0 || K <= 0 || (!index && rows != source_rows) || !sixteen_bits(type))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!aligned16(x) || !aligned_to(index, 4) || !aligned16(codes) || !aligned_to(scales, 4))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::fp8::convertible(rows, K))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t x_bytes = (size_t)source_rows * K * 2, code_bytes = (size_t)rows * K, scale_bytes = (size_t)rows * nnf::fp8::blocks_of(K) * 4;
+    if (overlap(codes, code_bytes, x, x_bytes) || overlap(scales, scale_bytes, x, x_bytes) || overlap(codes, code_bytes, scales, scale_bytes) ||
+        (index && (overlap(codes, code_bytes, index, (size_t)rows * 4) || overlap(scales, scale_bytes, index, (size_t)rows * 4))))
+        return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_fp8_quantize((hipStream_t)stream, x, type == NNF_TYPE_BF16, index, codes, (float*)scales, rows, source_rows, K);
+}
+
+int nnf_fp8_quantize_weights(nnf_stream_t stream, const void* w, int type, void* codes, void* scales, int matrices, int N, int K)
+{
+    if (!w || !codes || !scales || matrices <= 0 || N <= 0 || K <= 0 || !sixteen_bits(type) || !aligned16(w) || !aligned16(codes) || !aligned_to(scales, 4))
+        return NNF_ERR_INVALID_ARGUMENT;
+    if (!nnf::fp8::weights_convertible(matrices, N, K))
+        return NNF_ERR_UNSUPPORTED_SHAPE;
+    const size_t values = (size_t)matrices * N * K, scale_bytes = (size_t)matrices * nnf::fp8::blocks_of(N) * nnf::fp8::blocks_of(K) * 4;
+    if (overlap(codes, values, w, values * 2) || overlap(scales, scale_bytes, w, values * 2) || overlap(codes, values, scales, scale_bytes))
+        return NNF_ERR_INVALID_ARGUMENT;
+    DeviceInfo dev;
+    const int st = current_device_info(dev);
+    if (st != NNF_OK)
+        return st;
+    return (int)nnf::launch_fp8_quantize_weights((hipStream_t)stream, w, type == NNF_TYPE_BF16, codes, (float*)scales, matrices, N, K);
+}
+
+int nnf_fp8_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type, int M, int N, int K,
+                         const void* bias, const void* residual, int act, int variant)
+{
+    return fp8_product(stream, {(const uint8_t*)A, (const float*)a_scales, (const uint8_t*)W, (const float*)w_scales, Y, bias, residual, nullptr, M, N, K, 1,
+                                type == NNF_TYPE_BF16},
+                       type, act, variant);
+}
+
+int nnf_fp8_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type, int M, int N, int K,
+                 const void* bias, const void* residual, int act)
+{
+    return nnf_fp8_gemm_variant(stream, A, a_scales, W, w_scales, Y, type, M, N, K, bias, residual, act, NNF_FP8_AUTO);
+}
+
+int nnf_fp8_grouped_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets, void* Y,
+                                 int type, int experts, int M, int N, int K, int act, int variant)
+{
+    if (!offsets)
+        return NNF_ERR_INVALID_ARGUMENT;
+    return fp8_product(stream, {(const uint8_t*)A, (const float*)a_scales, (const uint8_t*)W, (const float*)w_scales, Y, nullptr, nullptr, (const int*)offsets, M, N, K,
+                                experts, type == NNF_TYPE_BF16},
+                       type, act, variant);
+}
+
+int nnf_fp8_grouped_gemm(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, const void* offsets, void* Y, int type,
+                         int experts, int M, int N, int K, int act)
+{
+    return nnf_fp8_grouped_gemm_variant(stream, A, a_scales, W, w_scales, offsets, Y, type, experts, M, N, K, act, NNF_FP8_AUTO);
 }
 
 } // extern "C"

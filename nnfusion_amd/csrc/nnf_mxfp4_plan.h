@@ -1,12 +1,17 @@
 // Which kernel serves an MXFP4 product: shared by the library and the emitters (host arithmetic only).
 #pragma once
 
+#include "nnf_tiles_plan.h"
+
 #include <stddef.h>
 
 namespace nnf
 {
     namespace mx
     {
+        using nnf::column_tiles;
+        using nnf::most_row_blocks;
+
         constexpr int MAX_K = 1 << 22; // byte offsets inside a tile of 256 rows stay below 2^31
         // bytes from one row of scale bytes to the next: K / 32 rounded up to 16, so that every row starts on 16 bytes
         constexpr int scale_bytes(int K) { return ((K >> 5) + 15) & ~15; }
@@ -18,16 +23,6 @@ namespace nnf
         {
             return supported(K) && M <= 1 << 30 && N <= 1 << 29 && (!gate || (long long)N * K < 1LL << 32) && experts <= 1 << 30;
         }
-
-        // blocks of `rows` rows that there are at most, of M rows in `experts` groups (0: one product): every group may end in a block of its
-        // own, which has a row at least
-        constexpr long long most_row_blocks(int M, int experts, int rows)
-        {
-            const long long groups = experts == 0 ? 1 : experts < M ? experts : M;
-            return (M + groups * (rows - 1)) / rows;
-        }
-        // tiles of columns of Y, `cols` weight rows each
-        constexpr int column_tiles(int N, int cols, bool gate) { return (int)(((long long)N + (gate ? cols / 2 : cols) - 1) / (gate ? cols / 2 : cols)); }
 
         // a grid has fewer than 2^32 threads.  Of the products' kernels none has more than 512 in a workgroup
         constexpr long long MAX_WORKGROUPS = (1 << 23) - 1;

@@ -4,6 +4,7 @@
 // taken from the tensors one Python attribute at a time, a foreign call of up to twenty converted arguments) took the host
 // 10 - 13 us apiece, so that a step of twelve calls was bound by the interpreter.  Here a call checks its tensors, allocates
 // what the caller did not bring and enters the library in about a microsecond.  No state is kept between calls.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
@@ -582,6 +583,144 @@ namespace
         return y.release();
     }
 
+    // ---- block-scaled 8-bit floating point, likewise
+    constexpr auto E4M3 = at::kFloat8_e4m3fn;
+    int64_t blocks128(int64_t size) { return (size + 127) / 128; }
+    PyObject* pair(const Owned& a, const Owned& b)
+    {
+        PyObject* const both = PyTuple_Pack(2, a.object, b.object);
+        if (!both)
+            throw Raised();
+        return both;
+    }
+
+    // (x, rows, codes, scales) -> (codes, scales)
+    PyObject* fp8_quantize(Args v)
+    {
+        const Tensor& x = tensor(v[0]);
+        matrix(x);
+        const int type = type_of(x, false, "x: fp16 or bf16");
+        require(x.is_contiguous(), "a contiguous matrix");
+        const int source = size32(x.size(0)), k = size32(x.size(1));
+        int rows = source;
+        if (v[1] != Py_None)
+        {
+            const Tensor& index = tensor(v[1]);
+            require(index.scalar_type() == at::kInt && index.dim() == 1 && index.is_contiguous(), "rows: a contiguous int32 vector");
+            rows = size32(index.size(0));
+        }
+        if (v[2] != Py_None)
+            require(is(tensor(v[2]), E4M3, {rows, k}), "codes: contiguous float8_e4m3fn [rows, K]");
+        if (v[3] != Py_None)
+            require(is(tensor(v[3]), at::kFloat, {blocks128(k), rows}), "scales: contiguous fp32 [ceil(K/128), rows]");
+        on_device(x, {v[1], v[2], v[3]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+        const Owned codes(output(v[2], {rows, k}, E4M3, x, "codes")), scales(output(v[3], {blocks128(k), rows}, at::kFloat, x, "scales"));
+        call("nnf_fp8_quantize", nnf_fp8_quantize, stream(), x.data_ptr(), type, address(v[1]), codes.data(), scales.data(), rows, source, k);
+        return pair(codes, scales);
+    }
+
+    // (w, codes, scales) -> (codes, scales)
+    PyObject* fp8_quantize_weights(Args v)
+    {
+        const Tensor& w = tensor(v[0]);
+        if (w.dim() != 2 && w.dim() != 3)
+            raise(PyExc_ValueError, "weights [N, K] or [matrices, N, K] are expected");
+        const int type = type_of(w, false, "w: fp16 or bf16");
+        require(w.is_contiguous(), "contiguous weights");
+        const bool many = w.dim() == 3;
+        const int matrices = many ? size32(w.size(0)) : 1, n = size32(w.size(-2)), k = size32(w.size(-1));
+        const int64_t nb = blocks128(n), kb = blocks128(k);
+        if (v[1] != Py_None)
+            require(tensor(v[1]).scalar_type() == E4M3 && tensor(v[1]).is_contiguous() && tensor(v[1]).sizes() == w.sizes(), "codes: contiguous float8_e4m3fn of w's shape");
+        if (v[2] != Py_None)
+            require(many ? is(tensor(v[2]), at::kFloat, {matrices, nb, kb}) : is(tensor(v[2]), at::kFloat, {nb, kb}), "scales: contiguous fp32 [.., ceil(N/128), ceil(K/128)]");
+        on_device(w, {v[1], v[2]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(w.device());
+        const Owned codes(many ? output(v[1], {matrices, n, k}, E4M3, w, "codes") : output(v[1], {n, k}, E4M3, w, "codes"));
+        const Owned scales(many ? output(v[2], {matrices, nb, kb}, at::kFloat, w, "scales") : output(v[2], {nb, kb}, at::kFloat, w, "scales"));
+        call("nnf_fp8_quantize_weights", nnf_fp8_quantize_weights, stream(), w.data_ptr(), type, codes.data(), scales.data(), matrices, n, k);
+        return pair(codes, scales);
+    }
+
+    // the type of a product's result: that of the first tensor given, or the one named, or fp16
+    at::ScalarType fp8_result(std::initializer_list<PyObject*> tensors, PyObject* dtype)
+    {
+        at::ScalarType type = at::kHalf;
+        bool known = dtype != Py_None;
+        if (known)
+        {
+            if (!THPDtype_Check(dtype))
+                raise(PyExc_TypeError, "dtype: a torch.dtype is expected");
+            type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+        }
+        for (PyObject* o : tensors)
+            if (o != Py_None)
+            {
+                require(!known || tensor(o).scalar_type() == type, "bias, residual, out and dtype: one type");
+                type = tensor(o).scalar_type();
+                known = true;
+            }
+        require(type == at::kHalf || type == at::kBFloat16, "results of fp16 or bf16");
+        return type;
+    }
+    void fp8_activations(const Tensor& a, const Tensor& as, int& m, int& k)
+    {
+        matrix(a);
+        m = size32(a.size(0)), k = size32(a.size(1));
+        require(is(a, E4M3, {m, k}), "activations: contiguous float8_e4m3fn [M, K]");
+        require(is(as, at::kFloat, {blocks128(k), m}), "scales of the activations: contiguous fp32 [ceil(K/128), M]");
+    }
+
+    // (a, a_scales, w, w_scales, bias, residual, act, out, dtype, variant)
+    PyObject* fp8_gemm(Args v)
+    {
+        const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]);
+        int m, k;
+        fp8_activations(a, as, m, k);
+        matrix(w);
+        const int act = integer(v[6]), n = mxfp4_columns(w.size(0), act);
+        require(is(w, E4M3, {w.size(0), k}), "weights: contiguous float8_e4m3fn [N, K]");
+        require(is(ws, at::kFloat, {blocks128(n) * (act ? 2 : 1), blocks128(k)}), "scales of the weights: contiguous fp32 [ceil(N/128), ceil(K/128)], with SiLU-gate twice");
+        const at::ScalarType type = fp8_result({v[7], v[5], v[4]}, v[8]);
+        if (v[4] != Py_None)
+            require(is(tensor(v[4]), type, {n}), "bias: contiguous [N]");
+        if (v[5] != Py_None)
+            require(is(tensor(v[5]), type, {m, n}), "residual: contiguous [M, N]");
+        if (v[7] != Py_None)
+            require(is(tensor(v[7]), type, {m, n}), "out: contiguous [M, N]");
+        on_device(a, {v[1], v[2], v[3], v[4], v[5], v[7]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+        Owned y(output(v[7], {m, n}, type, a, "out"));
+        call("nnf_fp8_gemm", nnf_fp8_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data(),
+             type == at::kHalf ? NNF_TYPE_F16 : NNF_TYPE_BF16, m, n, k, address(v[4]), address(v[5]), act, integer(v[9]));
+        return y.release();
+    }
+
+    // (a, a_scales, w, w_scales, offsets, act, out, dtype, variant)
+    PyObject* fp8_grouped_gemm(Args v)
+    {
+        const Tensor &a = tensor(v[0]), &as = tensor(v[1]), &w = tensor(v[2]), &ws = tensor(v[3]), &offsets = tensor(v[4]);
+        int m, k;
+        fp8_activations(a, as, m, k);
+        if (w.dim() != 3)
+            raise(PyExc_ValueError, "weights [experts, N, K] are expected");
+        const int experts = size32(w.size(0)), act = integer(v[5]), n = mxfp4_columns(w.size(1), act);
+        require(is(w, E4M3, {experts, w.size(1), k}), "weights: contiguous float8_e4m3fn [experts, N, K]");
+        require(is(ws, at::kFloat, {experts, blocks128(n) * (act ? 2 : 1), blocks128(k)}),
+                "scales of the weights: contiguous fp32 [experts, ceil(N/128), ceil(K/128)], with SiLU-gate twice the blocks of N");
+        require(is(offsets, at::kInt, {(int64_t)experts + 1}), "offsets: contiguous int32 [experts + 1]");
+        const at::ScalarType type = fp8_result({v[6]}, v[7]);
+        if (v[6] != Py_None)
+            require(is(tensor(v[6]), type, {m, n}), "out: contiguous [M, N]");
+        on_device(a, {v[1], v[2], v[3], v[4], v[6]});
+        const c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+        Owned y(output(v[6], {m, n}, type, a, "out"));
+        call("nnf_fp8_grouped_gemm", nnf_fp8_grouped_gemm_variant, stream(), a.data_ptr(), as.data_ptr(), w.data_ptr(), ws.data_ptr(), offsets.data_ptr(), y.data(),
+             type == at::kHalf ? NNF_TYPE_F16 : NNF_TYPE_BF16, experts, m, n, k, act, integer(v[8]));
+        return y.release();
+    }
+
     template <PyObject* (*F)(Args), int N>
     PyObject* entry(PyObject*, Args v, Py_ssize_t n)
     {
@@ -617,7 +756,8 @@ namespace
                              NNF_ENTRY(wna16_gemm_fused, 14), NNF_ENTRY(fused_mlp_wna16, 14), NNF_ENTRY(w8a8_gemm, 7),         NNF_ENTRY(w8a8_gemm_acc, 5),
                              NNF_ENTRY(elementwise, 4),       NNF_ENTRY(rms_norm, 4),         NNF_ENTRY(dequantize, 7),        NNF_ENTRY(mxfp4_quantize, 4),
                              NNF_ENTRY(mxfp4_dequantize, 3),  NNF_ENTRY(mxfp4_gemm, 10),        NNF_ENTRY(mxfp4_grouped_gemm, 9),
-                             NNF_ENTRY(moe_route, 12),        NNF_ENTRY(moe_combine, 5),       {"set_error", set_error, METH_O, nullptr},
+                             NNF_ENTRY(moe_route, 12),        NNF_ENTRY(moe_combine, 5),       NNF_ENTRY(fp8_quantize, 4),      NNF_ENTRY(fp8_quantize_weights, 3),
+                             NNF_ENTRY(fp8_gemm, 10),         NNF_ENTRY(fp8_grouped_gemm, 9),  {"set_error", set_error, METH_O, nullptr},
                              {nullptr, nullptr, 0, nullptr}};
     PyModuleDef module = {PyModuleDef_HEAD_INIT, "nnf_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace

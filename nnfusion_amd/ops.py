@@ -345,3 +345,35 @@ def moe_combine(x, weights, positions, residual=None, out=None):
     positions [tokens, k] as moe_route gives them.  fp32 sums, one rounding.  Positions outside x and weights of 0 add nothing.  out may be
     the residual."""
     return _native.moe_combine(x, weights, positions, residual, out)
+
+
+def fp8_quantize(x, rows=None, codes=None, scales=None):
+    """fp16 or bf16 [source_rows, K] -> (codes float8_e4m3fn [rows, K], scales f32 [ceil(K/128), rows]): 8-bit values with a scale for each 128 of
+    a row along K, max(largest magnitude, 2^-64) / 448.  rows: i32, the row of x that each quantised row is (tokens in the order of their
+    experts, as moe_route gives it; zeros where x has no such row), or None for every row in turn.  K a multiple of 16."""
+    return _native.fp8_quantize(x, rows, codes, scales)
+
+
+def fp8_quantize_weights(w, codes=None, scales=None):
+    """fp16 or bf16 [N, K] or [matrices, N, K] -> (codes float8_e4m3fn of w's shape, scales f32 [.., ceil(N/128), ceil(K/128)]): a scale for each block of
+    128 x 128.  Gate and up rows are two matrices of N rows each."""
+    return _native.fp8_quantize_weights(w, codes, scales)
+
+
+FP8_VARIANTS = {name: i for i, name in enumerate(("auto", "tile_16x32", "tile_16x32_2", "tile_16x32_4", "tile_32x64", "tile_64x64", "tile_64x128", "tile_128x128"))}
+
+
+def fp8_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, dtype=None, variant="auto"):
+    """Y [M,N] = A . W^T (+ bias + residual) of block-scaled 8-bit operands: a [M,K] and a_scales [ceil(K/128), M] as fp8_quantize gives them, w [N,K] and
+    w_scales [ceil(N/128), ceil(K/128)] as fp8_quantize_weights does; with act=1 SiLU(gate) * up, where w holds the gate rows, then the up
+    rows, and w_scales the gate's blocks, then the up matrix's.  Sums in fp32, one rounding to dtype: that of out, residual or bias where
+    given, else fp16 unless named.  out may be the residual.  variant: one kernel (a key of FP8_VARIANTS) instead of the library's choice."""
+    return _native.fp8_gemm(a, a_scales, w, w_scales, bias, residual, act, out, dtype, FP8_VARIANTS[variant])
+
+
+def fp8_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, dtype=None, variant="auto"):
+    """The product of a mixture's experts: rows of a sorted by expert, w [experts, N, K] (2N rows with act=1, SiLU-gate), w_scales f32 [experts,
+    ceil(N/128), ceil(K/128)] (twice the blocks with act=1); group e is the rows offsets[e] .. offsets[e+1] (offsets i32 [experts+1], on the device, not
+    decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here).  The library chooses a
+    kernel for all rows of a; where the groups fill little of them, name a variant for the rows there are."""
+    return _native.fp8_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, dtype, FP8_VARIANTS[variant])
