@@ -34,7 +34,14 @@ namespace nnf
             static constexpr int STAGE = (ROWS + COLS) * STEP_BYTES, SCALES = ALL_SCALE_LOADS * WAVE * 4;
             static constexpr int GROUP_LDS = S * STAGE + 2 * SCALES;
             static constexpr int PITCH = FN * 128 + 16; // fp32 results of a row of a wavefront
+            // a wavefront of one fragment of rows has the operands of a whole step and of the next in registers; a taller one those of the weights, and
+            // of the activations a fragment and the next.  PRODUCTS: fragments of products under way: of eight fragments of sums there is room for one,
+            // and the other wavefront of the SIMD has the matrix cores meanwhile
+            static constexpr bool WHOLE = FM == 1;
+            static constexpr int PRODUCTS = FM * FN > 6 ? 1 : 2;
             static constexpr int LDS = GROUP_LDS * WK > WAVES * 32 * PITCH ? GROUP_LDS * WK : WAVES * 32 * PITCH;
+            static_assert(FM == 1 || FM % 2 == 0, "two fragments of rows in turn");
+            static_assert(ROWS % 16 == 0, "rows 16 apart have their pieces in one order");
             static_assert((ROWS == WM * FM * 32 || (ROWS < 32 && GROUP * FM == 1)) && (ROWS + COLS) / 8 % GROUP == 0, "whole loads");
             static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && S >= 2 && (S - 1) * LOADS < 64, "room for them, and a count");
         };
@@ -190,14 +197,13 @@ namespace nnf
             // ---- what it reads from LDS
             const int r = lane & 31, g = lane >> 5;
             const int wave_n = wave % T::WN, wave_m = wave / T::WN;
-            uint32_t w_at[4], a_at[4];
+            // a lane's piece s of a row that is a multiple of 32 (or of ROWS) from the first; the rows of the wavefront's weights and activations
+            uint32_t piece_at[4];
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-            {
-                const auto in_row = [&](int row) { return row * STEP_BYTES + (((4 * g + s) ^ ((row >> 1) & 7)) << 4); };
-                w_at[s] = codes_at + wave_n * T::FN * 32 * STEP_BYTES + in_row(r);
-                a_at[s] = codes_at + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES + in_row(r % T::ROWS);
-            }
+                piece_at[s] = r % T::ROWS * STEP_BYTES + (((4 * g + s) ^ ((r % T::ROWS >> 1) & 7)) << 4);
+            const uint32_t w_row_at = r / T::ROWS * (T::ROWS * STEP_BYTES); // (of the weights, rows behind ROWS are there)
+            const uint32_t w_at = codes_at + wave_n * T::FN * 32 * STEP_BYTES, a_at = codes_at + (T::COLS + wave_m * T::FM * 32) * STEP_BYTES;
             const uint32_t as_at = scales_at + (wave_m * T::FM * 32 + r % T::ROWS) * 4;
 
             // scales of the weights: a wavefront's columns lie in one block of them (with SiLU-gate in one of the gate's and one of the up rows'); a lane
@@ -217,38 +223,34 @@ namespace nnf
 
             constexpr int B = T::FN * T::FM;
             floatx16 sum[T::FN][T::FM] = {};
-            floatx16 product[2] = {};                      // of a fragment and of the one before
-            intx8 wf[2][T::FN][2], af[2][T::FM][2];        // operands of a step and of the next
-            uintx4 w_read[T::FN][4], a_read[T::FM][4];     // the halves of those, on their way
-            float as[T::FM], as_next[T::FM], scale[NS] = {}; // scale: of the products that wait
+            constexpr int WSETS = T::WHOLE ? 2 : 1;
+            floatx16 product[2] = {};                  // of a fragment and of the one before
+            intx8 wf[WSETS][T::FN][2], af[2][2];       // operands: of a step (and of the next); of a fragment of rows and of the next one
+            uintx4 w_read[T::FN][4], a_read[4];        // the halves of those, on their way
+            float as[T::FM], as_last, scale[NS] = {}; // of the rows of a step, the next step's last, the products that wait
 
-            const auto read_scales = [&](int step) {
+            const auto read_scales = [&](int step) { // (where this step's are used up, but for the last)
                 const uint32_t from = as_at + (step / T::G & 1) * T::SCALES + step % T::G * (T::ROWS * 4);
-                unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * 128>(as_next[f], from); });
+                unroll_for<0, T::FM - 1>([&](auto f) { lds_read_b32_nowait<f * 128>(as[f], from); });
+                lds_read_b32_nowait<(T::FM - 1) * 128>(as_last, from);
             };
-            constexpr int READS = (T::FN + T::FM) * 4;
-            const auto read_piece = [&](auto q, uint32_t stage) {
-                constexpr int f = q / 4, s = q % 4;
-                if constexpr (f < T::FN)
-                    lds_read_b128_nowait<f * 32 * STEP_BYTES>(w_read[f][s], w_at[s] + stage);
-                else
-                    lds_read_b128_nowait<(f - T::FN) * 32 * STEP_BYTES>(a_read[f - T::FN][s], a_at[s] + stage);
-            };
+            // piece s of fragment f
+            const auto read_weights = [&](auto f, auto s, uint32_t stage) { lds_read_b128_nowait<f * 32 * STEP_BYTES>(w_read[f][s], piece_at[s] + w_row_at + (w_at + stage)); };
+            const auto read_rows = [&](auto f, auto s, uint32_t stage) { lds_read_b128_nowait<f * 32 * STEP_BYTES>(a_read[s], piece_at[s] + (a_at + stage)); };
             // nothing read without a wait stays in flight past the straight line of code that asked for it
-            const auto landed = [&](auto set) {
-                lds_wait<0>(w_read[0][0]);
-                unroll_for<0, 4>([&](auto s) {
-                    unroll_for<0, T::FN>([&](auto f) { lds_wait_also(w_read[f][s]); });
-                    unroll_for<0, T::FM>([&](auto f) { lds_wait_also(a_read[f][s]); });
-                });
-                unroll_for<0, 2>([&](auto h) {
-                    unroll_for<0, T::FN>([&](auto f) { wf[set][f][h] = operand(w_read[f][2 * h], w_read[f][2 * h + 1]); });
-                    unroll_for<0, T::FM>([&](auto f) { af[set][f][h] = operand(a_read[f][2 * h], a_read[f][2 * h + 1]); });
-                });
-                unroll_for<0, T::FM>([&](auto f) {
-                    lds_wait_also(as_next[f]);
-                    as[f] = as_next[f];
-                });
+            const auto rows_landed = [&](auto set, auto since) { // since: reads asked for behind these
+                lds_wait<since>(a_read[0]);
+                unroll_for<1, 4>([&](auto s) { lds_wait_also(a_read[s]); });
+                unroll_for<0, 2>([&](auto h) { af[set][h] = operand(a_read[2 * h], a_read[2 * h + 1]); });
+            };
+            const auto weights_landed = [&](auto set, auto f) { // (behind a wait)
+                unroll_for<0, 4>([&](auto s) { lds_wait_also(w_read[f][s]); });
+                unroll_for<0, 2>([&](auto h) { wf[set][f][h] = operand(w_read[f][2 * h], w_read[f][2 * h + 1]); });
+            };
+            const auto scales_landed = [&] {
+                unroll_for<0, T::FM - 1>([&](auto f) { lds_wait_also(as[f]); });
+                lds_wait_also(as_last);
+                as[T::FM - 1] = as_last;
             };
             // half h of the products of fragment i that wait
             const auto add = [&](auto i, auto which, auto h) {
@@ -260,20 +262,32 @@ namespace nnf
                     constexpr int of_fragment = GATE && T::FN > 1 ? fn * 2 / T::FN : 0;
                     sum[fn][fm][e] = __builtin_fmaf(product[which][e], scale[GATE && T::FN == 1 ? h : of_fragment], sum[fn][fm][e]);
                 }
+                asm volatile("" : "+v"(sum[fn][fm])); // (here, and not where the compiler finds room: products kept until then are registers lost)
             };
 
-            // a step: what comes S steps later is asked for and the next step's fragments are read, between its MFMAs.  FULL: that step ends within
-            // the rows
-            uint32_t stage = 0;
-            const auto body = [&](int step, auto set, auto full) {
-                using Next = std::integral_constant<int, 1 - set>;
-                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+            const auto whole_landed = [&](auto set) {
+                rows_landed(set, std::integral_constant<int, 0>{});
+                unroll_for<0, T::FN>([&](auto f) { weights_landed(std::integral_constant<int, T::WHOLE ? (int)set : 0>{}, f); });
+                scales_landed();
+            };
+
+            const auto scales_of_step = [&](int step, float (&of_step)[NS]) {
                 if ((step & (WAVE - 1)) == 0 && step > 0)
                     load_weight_scales(step);
-                float of_step[NS];
 #pragma unroll
                 for (int i = 0; i < NS; ++i)
                     of_step[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ws[i]), step & (WAVE - 1)));
+            };
+            const auto multiply = [&](intx8 w, intx8 a, floatx16 c) { return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, E4M3, E4M3, 0, 0, 0, 0); };
+
+            // a step of a wavefront with one fragment of rows: what comes S steps later is asked for and the next step's operands are read, between its
+            // MFMAs.  FULL: that later step ends within the rows
+            uint32_t stage = 0;
+            const auto whole_body = [&](int step, auto set, auto full) __attribute__((always_inline)) {
+                using Next = std::integral_constant<int, 1 - set>;
+                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                float of_step[NS];
+                scales_of_step(step, of_step);
                 arrive(step + 1, next_stage, full);
                 if (step % T::G == 0 && step + T::G < steps)
                     fetch_scales(step + T::G);
@@ -281,30 +295,98 @@ namespace nnf
                     fetch(step + T::S, stage);
                 read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
                 unroll_for<0, B>([&](auto b) {
-                    constexpr int fn = b % T::FN, fm = b / T::FN;
-                    constexpr int SLOTS = 2 * B, EACH = (READS + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
+                    constexpr int SLOTS = 2 * B, READS = (T::FN + 1) * 4, EACH = (READS + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
                     constexpr int mine = (set * B + b) & 1;
                     unroll_for<0, 2>([&](auto h) {
                         constexpr int slot = 2 * b + h;
                         unroll_for<0, EACH>([&](auto q) {
-                            if constexpr (slot * EACH + q < READS)
-                                read_piece(std::integral_constant<int, slot * EACH + q>{}, next_stage);
+                            constexpr int i = slot * EACH + q;
+                            if constexpr (i < 4)
+                                read_rows(std::integral_constant<int, 0>{}, std::integral_constant<int, i>{}, next_stage);
+                            else if constexpr (i < READS)
+                                read_weights(std::integral_constant<int, i / 4 - 1>{}, std::integral_constant<int, i % 4>{}, next_stage);
                         });
                         if constexpr (full)
                             unroll_for<0, FETCHES>([&](auto q) {
                                 if constexpr (slot * FETCHES + q < T::LOADS)
                                     fetch_load(std::integral_constant<int, slot * FETCHES + q>{}, step + T::S, stage, std::true_type{});
                             });
-                        product[mine] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[set][fn][h], af[set][fm][h], h == 0 ? floatx16{} : product[mine], E4M3, E4M3, 0, 0, 0, 0);
+                        product[mine] = multiply(wf[T::WHOLE ? set : 0][b][h], af[set][h], h == 0 ? floatx16{} : product[mine]);
                         __builtin_amdgcn_sched_barrier(0);
                         add(std::integral_constant<int, (b + B - 1) % B>{}, std::integral_constant<int, 1 - mine>{}, h);
                         __builtin_amdgcn_sched_barrier(0);
                     });
 #pragma unroll
                     for (int i = 0; i < NS; ++i)
-                        scale[i] = as[fm] * of_step[i];
+                        scale[i] = as[0] * of_step[i];
                 });
-                landed(Next{});
+                whole_landed(Next{});
+                stage = next_stage;
+            };
+            // a step of a taller one: the fragments of rows one after the other, each against all of the weights'; each fragment of weights is read anew
+            // behind its last use, the rows' next one a fragment ahead.  Ahead of the last rows everything of this step has been read: there the
+            // wavefronts meet, and its place in LDS is free
+            const auto body = [&](int step, auto full) __attribute__((always_inline)) {
+                const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                float of_step[NS];
+                scales_of_step(step, of_step);
+                unroll_for<0, T::FM>([&](auto fm) __attribute__((always_inline)) {
+                    constexpr bool LAST = fm == T::FM - 1;
+                    constexpr int SLOTS = 2 * T::FN, EACH = (4 + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
+                    // (the fragments of weights behind the first are still on their way then)
+                    rows_landed(std::integral_constant<int, fm & 1>{}, std::integral_constant<int, fm == 0 ? (T::FN - 1) * 4 : 0>{});
+                    if constexpr (fm == 0)
+                    {
+                        weights_landed(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+                        scales_landed();
+                    }
+                    if constexpr (LAST)
+                    {
+                        arrive(step + 1, next_stage, full);
+                        if (step % T::G == 0 && step + T::G < steps)
+                            fetch_scales(step + T::G);
+                        if (!full && step + T::S < steps)
+                            fetch(step + T::S, stage);
+                        read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
+                    }
+                    unroll_for<0, T::FN>([&](auto fn) __attribute__((always_inline)) {
+                        constexpr int b = fm * T::FN + fn, mine = T::PRODUCTS == 1 ? 0 : b & 1;
+                        if constexpr (fm == 0 && fn > 0)
+                        {
+                            constexpr int SINCE = (2 * EACH * fn < 4 ? 2 * EACH * fn : 4) + (T::FN - 1 - fn) * 4;
+                            lds_wait<SINCE>(w_read[fn][0]);
+                            weights_landed(std::integral_constant<int, 0>{}, fn);
+                        }
+                        unroll_for<0, 2>([&](auto h) {
+                            constexpr int slot = 2 * fn + h;
+                            unroll_for<0, EACH>([&](auto q) {
+                                constexpr int i = slot * EACH + q;
+                                if constexpr (i < 4)
+                                    read_rows(std::integral_constant<int, LAST ? 0 : fm + 1>{}, std::integral_constant<int, i>{}, LAST ? next_stage : stage);
+                            });
+                            if constexpr (LAST && full)
+                                unroll_for<0, FETCHES>([&](auto q) {
+                                    if constexpr (slot * FETCHES + q < T::LOADS)
+                                        fetch_load(std::integral_constant<int, slot * FETCHES + q>{}, step + T::S, stage, std::true_type{});
+                                });
+                            product[mine] = multiply(wf[0][fn][h], af[fm & 1][h], h == 0 ? floatx16{} : product[mine]);
+                            __builtin_amdgcn_sched_barrier(0);
+                            if constexpr (T::PRODUCTS == 2)
+                            {
+                                add(std::integral_constant<int, (b + B - 1) % B>{}, std::integral_constant<int, 1 - mine>{}, h);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        });
+                        if constexpr (LAST)
+                            unroll_for<0, 4>([&](auto s) { read_weights(fn, s, next_stage); });
+#pragma unroll
+                        for (int i = 0; i < NS; ++i)
+                            scale[i] = as[fm] * of_step[i];
+                        if constexpr (T::PRODUCTS == 1)
+                            unroll_for<0, 2>([&](auto h) { add(std::integral_constant<int, b>{}, std::integral_constant<int, 0>{}, h); });
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                });
                 stage = next_stage;
             };
 
@@ -347,25 +429,42 @@ namespace nnf
                     using Even = std::integral_constant<int, 0>;
                     using Odd = std::integral_constant<int, 1>;
                     read_scales(0);
-                    unroll_for<0, READS>([&](auto q) { read_piece(q, 0); });
-                    landed(Even{});
+                    unroll_for<0, 4>([&](auto s) { read_rows(Even{}, s, 0); });
+                    unroll_for<0, T::FN>([&](auto f) { unroll_for<0, 4>([&](auto s) { read_weights(f, s, 0); }); });
+                    if constexpr (T::WHOLE)
+                        whole_landed(Even{});
                     const int whole = min(steps, max(row_bytes / STEP_BYTES - first_step, 0)); // steps that end within the rows
-#pragma unroll 1
-                    for (; step + 1 + T::S < whole; step += 2)
+                    if constexpr (T::WHOLE)
                     {
-                        body(step, Even{}, std::true_type{});
-                        body(step + 1, Odd{}, std::true_type{});
-                    }
 #pragma unroll 1
-                    for (; step < steps; step += 2)
-                    {
-                        body(step, Even{}, std::false_type{});
-                        if (step + 1 < steps)
-                            body(step + 1, Odd{}, std::false_type{});
-                        else if constexpr (B % 2 != 0)
-                            product[1] = product[0]; // (the last products, where two steps leave them)
+                        for (; step + 1 + T::S < whole; step += 2)
+                        {
+                            whole_body(step, Even{}, std::true_type{});
+                            whole_body(step + 1, Odd{}, std::true_type{});
+                        }
+#pragma unroll 1
+                        for (; step < steps; step += 2)
+                        {
+                            whole_body(step, Even{}, std::false_type{});
+                            if (step + 1 < steps)
+                                whole_body(step + 1, Odd{}, std::false_type{});
+                        }
                     }
-                    unroll_for<0, 2>([&](auto h) { add(std::integral_constant<int, B - 1>{}, std::integral_constant<int, 1>{}, h); });
+                    else
+                    {
+#pragma unroll 1
+                        for (; step + T::S < whole; ++step)
+                            body(step, std::true_type{});
+#pragma unroll 1
+                        for (; step < steps; ++step)
+                            body(step, std::false_type{});
+                    }
+                    // the products that wait still
+                    if constexpr (B % 2 != 0)
+                        if (steps & 1)
+                            product[1] = product[0];
+                    if constexpr (T::PRODUCTS == 2)
+                        unroll_for<0, 2>([&](auto h) { add(std::integral_constant<int, B - 1>{}, std::integral_constant<int, 1>{}, h); });
                 }
             }
 
@@ -458,7 +557,8 @@ namespace nnf
         case fp8::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2, 2>>(s, o, gate);
         case fp8::TILE_64x64: return launch_either<Tile<2, 2, 1, 1, 1, 4, 4>>(s, o, gate);
         case fp8::TILE_64x128: return launch_either<Tile<2, 2, 1, 1, 2, 3, 4>>(s, o, gate);
-        default: return launch_either<Tile<2, 2, 1, 2, 2, 2, 2>>(s, o, gate);
+        case fp8::TILE_128x128: return launch_either<Tile<2, 2, 1, 2, 2, 2, 2>>(s, o, gate);
+        default: return launch_either<Tile<2, 4, 1, 4, 2, 2, 2>>(s, o, gate);
         }
     }
 } // namespace nnf

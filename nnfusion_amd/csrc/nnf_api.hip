@@ -1086,7 +1086,7 @@ namespace
     int fp8_product(nnf_stream_t stream, const nnf::fp8::Operands& o, int type, int act, int variant)
     {
         using namespace nnf::fp8;
-        static_assert((int)NNF_FP8_TILE_128x128 == (int)KERNELS, "variants and kernels in one order, automatic choice first");
+        static_assert((int)NNF_FP8_TILE_256x256 == (int)KERNELS, "variants and kernels in one order, automatic choice first");
         if (!o.A || !o.As || !o.W || !o.Ws || !o.Y || o.M <= 0 || o.N <= 0 || o.K <= 0 || o.experts <= 0 || !sixteen_bits(type))
             return NNF_ERR_INVALID_ARGUMENT;
         if ((act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE) || variant < 0 || variant > KERNELS)

@@ -41,13 +41,14 @@ namespace nnf
             TILE_64x64, // the wavefronts share the tile and all of K
             TILE_64x128,
             TILE_128x128,
+            TILE_256x256,
             KERNELS
         };
         struct KernelFacts
         {
             int rows, cols, ranges;
         };
-        constexpr KernelFacts FACTS[KERNELS] = {{16, 32, 1}, {16, 32, 2}, {16, 32, 4}, {32, 64, 4}, {64, 64, 1}, {64, 128, 1}, {128, 128, 1}};
+        constexpr KernelFacts FACTS[KERNELS] = {{16, 32, 1}, {16, 32, 2}, {16, 32, 4}, {32, 64, 4}, {64, 64, 1}, {64, 128, 1}, {128, 128, 1}, {256, 256, 1}};
 
         constexpr bool fits(const KernelFacts& k, int M, int N, bool gate, int experts)
         {
@@ -67,7 +68,7 @@ namespace nnf
         inline Kernel choose(int M, int N, int K, bool gate, int experts, int num_cu)
         {
             const int rows = experts > 0 ? M / (experts < M ? experts : M) : M;
-            int k = rows <= 32 ? TILE_16x32_2 : rows <= 128 ? TILE_64x64 : TILE_128x128;
+            int k = rows <= 32 ? TILE_16x32_2 : rows <= 128 ? TILE_64x64 : rows < 1024 ? TILE_128x128 : TILE_256x256;
             while (k < KERNELS - 1 && !fits(FACTS[k], M, N, gate, experts))
                 ++k;
             return (Kernel)k;
