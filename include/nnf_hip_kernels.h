@@ -546,7 +546,7 @@ NNF_API int nnf_moe_combine(nnf_stream_t stream, const void* x, const void* weig
 /* x [source_rows, K] fp16 or bf16 (`type`) -> codes and scales of `rows` rows: row i is x's row index[i] (i32 [rows] on the device; zeros
  * where x has no such row), or x's row i where index is NULL (then rows == source_rows).  scale = max(largest magnitude, 2^-64) / 448, code =
  * the E4M3 nearest to x / scale, ties to even, both quotients rounded to fp32; a block with an infinity or NaN has scale NaN and zero
- * codes.  The results must not overlap each other, x or index; rows * ceil(K / 512) up to 2^28 - 16 (NNF_ERR_UNSUPPORTED_SHAPE above). */
+ * codes.  The results must not overlap each other, x or index; rows * ceil(K / 512) up to 2^24 (NNF_ERR_UNSUPPORTED_SHAPE above). */
 NNF_API int nnf_fp8_quantize(nnf_stream_t stream, const void* x, int type, const void* index, void* codes, void* scales,
                      int rows, int source_rows, int K);
 /* w [matrices, N, K] -> codes [matrices, N, K], scales [matrices, ceil(N / 128), ceil(K / 128)].  (Gate and up rows are two matrices: the

@@ -1,10 +1,12 @@
 // fp16 or bf16 -> block-scaled E4M3 (fp8.h): rows, picked by an index or not, with a scale for each 128 values, and weight matrices with
 // a scale for each block of 128 x 128.
 //
-// scale = max(largest magnitude, 2^-64) / 448, code = E4M3(x / scale): both quotients rounded to fp32 as IEEE has it, so that a code next to a tie
-// is the one that any fp32 implementation gets.  x / scale is the product with the scale's rounded inverse, put right twice by its remainder
-// (each step an fma: the first leaves less than half a step and a bit, the second rounds correctly); the bound of 2^-64 keeps all of that
-// away from subnormals.  A block with an infinity or NaN: scale NaN, codes 0.
+// scale = max(largest magnitude, 2^-64) / 448, code = E4M3(x / scale): both quotients as IEEE rounds them to fp32, so that a code next to a tie is
+// the one that any fp32 implementation gets.  Neither is divided for.  The scale is a product with the rounded 1 / 448 and one step of its
+// remainder, exact for every significand of 11 bits.  x / scale is x (inverse + rest) rounded once, rest being what the rounded inverse of the scale lacks:
+// off by 2^-41 before the rounding, where a quotient that is a tie of E4M3 but for the scale's rounding is never nearer than 2^-35 to a midpoint of
+// fp32 and any other one is 2^-17 away from a tie.  Powers of two are kept out of it until the conversion, which takes them for nothing, so that no
+// number leaves fp32's range.  A block with an infinity or NaN: scale NaN, codes 0.
 //
 // One pass over memory, two bytes read and one written a value.
 #include "fp8_launch.h"
@@ -18,6 +20,7 @@ namespace nnf
 
         constexpr int CONVERT_THREADS = 256;
         constexpr int WAVES = CONVERT_THREADS / WAVE;
+        constexpr int ROWS_OF_GRID = 1 << 15; // in y; the others in z
 
         __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b)
         {
@@ -42,81 +45,72 @@ namespace nnf
         {
             return BF16 ? __builtin_bit_cast(float, bits << 16) : (float)__builtin_bit_cast(half_t, (uint16_t)bits);
         }
-        template <bool BF16>
-        __device__ __forceinline__ float scale_of(uint32_t top)
+        // What a block's values are quantised with: x / scale = x (inverse + rest) / power, rest >= 0 (so that -0 stays what it is)
+        struct Quotient
         {
-            return top < (BF16 ? 0x7F80u : 0x7C00u) ? fmaxf(number<BF16>(top), 0x1p-64f) / 448.0f : __builtin_nanf("");
+            float scale, power, inverse, rest;
+        };
+        template <bool BF16>
+        __device__ __forceinline__ Quotient quotient_of(uint32_t top)
+        {
+            constexpr float C = 1.0f / 448.0f;
+            const float a = fmaxf(number<BF16>(top), 0x1p-64f), q = a * C;
+            Quotient v;
+            v.scale = __builtin_fmaf(__builtin_fmaf(-q, 448.0f, a), C, q);
+            const uint32_t bits = __builtin_bit_cast(uint32_t, v.scale);
+            const float m = __builtin_bit_cast(float, (bits & 0x007FFFFFu) | 0x3F800000u);
+            v.power = __builtin_bit_cast(float, bits & 0x7F800000u);
+            // (the hardware's inverse is good to a step: two steps lower it is below 1 / m)
+            v.inverse = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, __builtin_amdgcn_rcpf(m)) - 2);
+            v.rest = __builtin_fmaf(-m, v.inverse, 1.0f) * v.inverse;
+            if (top >= (BF16 ? 0x7F80u : 0x7C00u))
+                v.scale = __builtin_nanf("");
+            return v;
         }
         // eight values' codes
         template <bool BF16>
-        __device__ __forceinline__ uintx2 codes_of(uintx4 v, float scale)
+        __device__ __forceinline__ uintx2 codes_of(uintx4 v, const Quotient& by)
         {
-            const float inverse = 1.0f / scale;
-            const bool fine = scale == scale;
+            typedef short shortx2 __attribute__((ext_vector_type(2)));
             float q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
             {
-                const float x = number<BF16>(v[i / 2] >> (i % 2 * 16) & 0xFFFFu);
-                float y = x * inverse;
-                y = __builtin_fmaf(__builtin_fmaf(-y, scale, x), inverse, y);
-                q[i] = __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-y, scale, x), inverse, y), x); // (of -0 the sums above are 0)
+                const float x = BF16 ? __builtin_bit_cast(float, i & 1 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16) : (float)as_half2(v[i / 2])[i & 1];
+                q[i] = __builtin_fmaf(x, by.inverse, x * by.rest);
             }
             uintx2 c;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], 0, false);
-                w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h + 2], q[4 * h + 3], w, true);
-                c[h] = fine ? (uint32_t)w : 0u;
+                shortx2 w = {};
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, q[4 * h], q[4 * h + 1], by.power, false);
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, q[4 * h + 2], q[4 * h + 3], by.power, true);
+                c[h] = by.scale == by.scale ? __builtin_bit_cast(uint32_t, w) : 0u;
             }
             return c;
         }
 
-        // A wavefront takes UNITS units of 512 values of one row, eight to a lane, all their loads ahead of the first use
-        template <int UNITS, bool BF16>
+        // A wavefront takes 512 values of a row, eight to a lane; a workgroup up to four such units of the same row
+        template <bool BF16>
         __global__ __launch_bounds__(CONVERT_THREADS) void fp8_quantize_kernel(const uint16_t* __restrict__ x, const int* __restrict__ index, uint8_t* __restrict__ codes,
-                                                                               float* __restrict__ scales, int units, int row_units, int rows, int source_rows, int K)
+                                                                               float* __restrict__ scales, int rows, int source_rows, int K)
         {
-            const int lane = threadIdx.x & (WAVE - 1);
-            const int first = ((int)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) * UNITS;
-            int row[UNITS], unit[UNITS];
-            row[0] = first / row_units;
-            unit[0] = first - row[0] * row_units;
-#pragma unroll
-            for (int i = 1; i < UNITS; ++i)
+            const int lane = threadIdx.x & (WAVE - 1), row = (int)(blockIdx.z * ROWS_OF_GRID + blockIdx.y);
+            const int unit = (int)(blockIdx.x * (blockDim.x / WAVE)) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), k = unit * 512 + lane * 8;
+            if (row >= rows)
+                return;
+            const int from = index ? index[row] : row;
+            uintx4 v = {0, 0, 0, 0}; // (a row that is not there is a row of zeros)
+            if (k < K && from >= 0 && from < source_rows)
+                v = *reinterpret_cast<const uintx4*>(x + (size_t)from * K + k);
+            const Quotient by = quotient_of<BF16>(top_of_16_lanes(top_of(v)));
+            const uintx2 c = codes_of<BF16>(v, by);
+            if (k < K)
             {
-                const bool next = unit[i - 1] + 1 == row_units;
-                row[i] = row[i - 1] + (next ? 1 : 0);
-                unit[i] = next ? 0 : unit[i - 1] + 1;
-            }
-            uintx4 v[UNITS];
-#pragma unroll
-            for (int i = 0; i < UNITS; ++i)
-            {
-                const int k = unit[i] * 512 + lane * 8;
-                v[i] = uintx4{0, 0, 0, 0};
-                if (first + i < units && k < K)
-                {
-                    const long long from = index ? index[row[i]] : (long long)row[i];
-                    if (from >= 0 && from < source_rows)
-                        v[i] = *reinterpret_cast<const uintx4*>(x + from * K + k);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < UNITS; ++i)
-            {
-                if (first + i >= units)
-                    return;
-                const float scale = scale_of<BF16>(top_of_16_lanes(top_of(v[i])));
-                const uintx2 c = codes_of<BF16>(v[i], scale);
-                const int k = unit[i] * 512 + lane * 8;
-                if (k < K)
-                {
-                    *reinterpret_cast<uintx2*>(codes + (size_t)row[i] * K + k) = c;
-                    if ((lane & 15) == 0)
-                        scales[(size_t)(k >> 7) * rows + row[i]] = scale;
-                }
+                *reinterpret_cast<uintx2*>(codes + (size_t)row * K + k) = c;
+                if ((lane & 15) == 0)
+                    scales[(size_t)(k >> 7) * rows + row] = by.scale;
             }
         }
 
@@ -153,27 +147,21 @@ namespace nnf
 #pragma unroll
             for (int i = 0; i < WAVES; ++i)
                 top = max(top, tops[i]);
-            const float scale = scale_of<BF16>(top);
+            const Quotient by = quotient_of<BF16>(top);
             if (threadIdx.x == 0)
-                scales[blockIdx.x] = scale;
+                scales[blockIdx.x] = by.scale;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 if (n0 + i * 4 < N && k < K)
-                    *reinterpret_cast<uintx2*>(codes + (base + n0 + i * 4) * K + k) = codes_of<BF16>(v[i], scale);
+                    *reinterpret_cast<uintx2*>(codes + (base + n0 + i * 4) * K + k) = codes_of<BF16>(v[i], by);
         }
 
         template <bool BF16>
         hipError_t launch_rows(hipStream_t s, const void* x, const void* index, void* codes, float* scales, int rows, int source_rows, int K)
         {
-            // four units a wavefront once these fill the CUs; one below, where the time is one load's latency
-            constexpr int MANY = 4;
-            const int each = row_units(K), units = rows * each;
-            if (units < 256 * WAVES * MANY * 2)
-                fp8_quantize_kernel<1, BF16><<<(units + WAVES - 1) / WAVES, CONVERT_THREADS, 0, s>>>((const uint16_t*)x, (const int*)index, (uint8_t*)codes, scales, units,
-                                                                                                      each, rows, source_rows, K);
-            else
-                fp8_quantize_kernel<MANY, BF16><<<(units + WAVES * MANY - 1) / (WAVES * MANY), CONVERT_THREADS, 0, s>>>(
-                    (const uint16_t*)x, (const int*)index, (uint8_t*)codes, scales, units, each, rows, source_rows, K);
+            const int units = row_units(K), waves = units < WAVES ? units : WAVES;
+            const dim3 grid((units + waves - 1) / waves, rows < ROWS_OF_GRID ? rows : ROWS_OF_GRID, (rows + ROWS_OF_GRID - 1) / ROWS_OF_GRID);
+            fp8_quantize_kernel<BF16><<<grid, waves * WAVE, 0, s>>>((const uint16_t*)x, (const int*)index, (uint8_t*)codes, scales, rows, source_rows, K);
             return hipGetLastError();
         }
         template <bool BF16>
