@@ -1,14 +1,15 @@
 // Routing to experts: from logits to each token's experts and weights, and to the order in which the experts' products take the tokens.
 //
 // A score is softmax(l) or 1 / (1 + exp(-l)); experts are chosen by score + bias among the groups whose best one or two such sums are largest; the
-// lowest index wins a tie.  Several tokens share a wavefront, LANES lanes each, V experts to a lane (expert j LANES + lane): the largest of
-// a token is a few comparisons in registers and a reduction over its lanes, k times.  Without a bias the order of the scores is that of the
-// logits, which is exact.  Else sums are computed in fp32 first; where two that are compared lie closer than fp32 can tell (2^-20, a bound on
-// both errors), the wavefront chooses again in 64 bits: a choice does not depend on how exp rounds.
+// lowest index wins a tie.  LANES lanes of a wavefront have a token, V experts to a lane (expert j LANES + lane): the largest is a few
+// comparisons in registers and a reduction over the lanes, k times.  Four tokens to a wavefront share the instructions of that; a token of
+// its own is the shorter way where there are few.  Without a bias the order of the scores is that of the logits, which is exact.  Else
+// sums are computed in fp32 first; where two that are compared lie closer than fp32 can tell (2^-20, a bound on both errors), the whole
+// wavefront chooses again for that token in 64 bits: a choice does not depend on how exp rounds.
 //
-// The order is a counting sort: how many of each expert come from the workgroups and wavefronts ahead (counts in LDS, 16 bits each in the
-// workspace between two launches), then each wavefront goes through its pairs 64 at a time, equal experts found by a ballot for each bit of
-// their number.  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
+// The order is a counting sort.  A pair's place among those of its expert comes from a ballot for each bit of the expert's number inside a
+// wavefront, then from the counts of the wavefronts ahead in LDS, then, in a launch of its own, from those of the workgroups ahead (16 bits
+// each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 #include "moe_launch.h"
 #include "nnf_device.h"
 
@@ -55,29 +56,69 @@ namespace nnf
         {
             return __builtin_bit_cast(double, moved<CTRL>(__builtin_bit_cast(uint64_t, v)));
         }
-        // f(what another lane has) until every lane of the token has met all of them
-        template <int LANES, class T, class F>
-        __device__ __forceinline__ T over_lanes(T v, F f)
+        // f of what a lane and the one a quarter, or half, a wavefront away have
+        template <int AWAY, class F>
+        __device__ __forceinline__ uint32_t across(uint32_t v, F f)
+        {
+            const auto both = AWAY == 32 ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+            return f((uint32_t)both[0], (uint32_t)both[1]);
+        }
+        template <int AWAY, class F>
+        __device__ __forceinline__ float across(float v, F f)
+        {
+            return __builtin_bit_cast(float, across<AWAY>(__builtin_bit_cast(uint32_t, v), [&](uint32_t a, uint32_t b) {
+                                          return __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+                                      }));
+        }
+        template <int AWAY, class F>
+        __device__ __forceinline__ uint64_t across(uint64_t v, F f)
+        {
+            const auto pairs = [](uint32_t h) {
+                return AWAY == 32 ? __builtin_amdgcn_permlane32_swap(h, h, false, false) : __builtin_amdgcn_permlane16_swap(h, h, false, false);
+            };
+            const auto low = pairs((uint32_t)v), high = pairs((uint32_t)(v >> 32));
+            return f((uint64_t)high[0] << 32 | low[0], (uint64_t)high[1] << 32 | low[1]);
+        }
+        template <int AWAY, class F>
+        __device__ __forceinline__ double across(double v, F f)
+        {
+            return __builtin_bit_cast(double, across<AWAY>(__builtin_bit_cast(uint64_t, v), [&](uint64_t a, uint64_t b) {
+                                          return __builtin_bit_cast(uint64_t, f(__builtin_bit_cast(double, a), __builtin_bit_cast(double, b)));
+                                      }));
+        }
+        // f(what another lane has) until every lane of 16 has met the others, and of 64
+        template <class T, class F>
+        __device__ __forceinline__ T over_16_lanes(T v, F f)
         {
             v = f(v, moved<0x128>(v)); // row_ror:8
             v = f(v, moved<0x124>(v)); // row_ror:4
             v = f(v, moved<0x122>(v)); // row_ror:2
             v = f(v, moved<0x121>(v)); // row_ror:1
-            if constexpr (LANES == 64)
-            {
-                v = f(v, __shfl_xor(v, 16));
-                v = f(v, __shfl_xor(v, 32));
-            }
             return v;
         }
-        // the largest key of a token's lanes and the lowest index that has it
-        template <int LANES, class Key>
-        __device__ __forceinline__ void best_of_lanes(Key& key, int& index)
+        template <int LANES, class T, class F>
+        __device__ __forceinline__ T over_lanes(T v, F f)
         {
-            const Key top = over_lanes<LANES>(key, [](Key a, Key b) { return a > b ? a : b; });
-            const uint32_t mine = key == top ? (uint32_t)index : ~0u;
-            index = (int)over_lanes<LANES>(mine, [](uint32_t a, uint32_t b) { return min(a, b); });
-            key = top;
+            v = over_16_lanes(v, f);
+            if constexpr (LANES == 64)
+                v = across<32>(across<16>(v, f), f);
+            return v;
+        }
+        __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+        __device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
+        // the largest of a token's keys; with a token to the wavefront in scalar registers
+        template <int LANES, class Key>
+        __device__ __forceinline__ Key largest(Key key)
+        {
+            const Key most = over_lanes<LANES>(key, [](Key a, Key b) { return a > b ? a : b; });
+            if constexpr (LANES == 64)
+                return uniform(most);
+            else
+                return most;
+        }
+        __device__ __forceinline__ uint32_t least_of_16_lanes(uint32_t v)
+        {
+            return over_16_lanes(v, [](uint32_t a, uint32_t b) { return min(a, b); });
         }
 
         __device__ __forceinline__ void lanes_meet()
@@ -87,32 +128,66 @@ namespace nnf
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
 
-        __device__ __forceinline__ float logit(const Routing& r, size_t at)
+        __device__ __forceinline__ float as_logit(float v) { return v != v ? LOWEST : fminf(v, LARGEST); }
+        // logit `at`, counted from the first of token `row / E`
+        __device__ __forceinline__ float logit(const Routing& r, size_t row, uint32_t at)
         {
-            float v;
             if (r.type == 0)
-                v = (float)((const half_t*)r.logits)[at];
-            else if (r.type == 1)
-                v = __builtin_bit_cast(float, (uint32_t)((const uint16_t*)r.logits)[at] << 16);
-            else
-                v = ((const float*)r.logits)[at];
-            return v != v ? LOWEST : fminf(v, LARGEST);
+                return as_logit((float)((const half_t*)r.logits + row)[at]);
+            if (r.type == 1)
+                return as_logit(__builtin_bit_cast(float, (uint32_t)((const uint16_t*)r.logits + row)[at] << 16));
+            return as_logit(((const float*)r.logits + row)[at]);
         }
-        __device__ __forceinline__ float exp_of(float v) { return expf(v); }
-        __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+        // the logits of the token whose first one is `from` behind `row`; behind the last one the lowest number
+        template <int LANES, int V>
+        __device__ __forceinline__ void logits_of(const Routing& r, size_t row, uint32_t from, float (&v)[V])
+        {
+            const int lane = threadIdx.x & (LANES - 1);
+            int E = r.E;
+            if (r.type == 2)
+            {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    v[j] = ((const float*)r.logits + row)[from + min(j * LANES + lane, E - 1)];
+            }
+            else
+            {
+                uint16_t bits[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    bits[j] = ((const uint16_t*)r.logits + row)[from + min(j * LANES + lane, E - 1)];
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    v[j] = r.type == 0 ? (float)__builtin_bit_cast(half_t, bits[j]) : __builtin_bit_cast(float, (uint32_t)bits[j] << 16);
+            }
+            asm volatile("" : "+s"(E)); // (compared again: V comparisons kept are as many pairs of scalar registers)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                v[j] = j * LANES + lane < E ? as_logit(v[j]) : LOWEST;
+        }
 
-        // The experts of a token, its logits in v: lane p < k gets the p-th, and its score (0 of one that is masked).  room: E + groups values
-        // in LDS.  false: numbers that decide lie closer than Real can tell
+        __device__ __forceinline__ float exp_of(float v) { return __expf(v); }
+        __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+        __device__ __forceinline__ float inverse_of(float v) { return __builtin_amdgcn_rcpf(v); }
+        __device__ __forceinline__ double inverse_of(double v) { return 1 / v; }
+
+        // The experts of the token whose logits begin `from` behind `row`: its lane p < k gets the p-th, and its score (0 of one that is masked).  room: a place
+        // in LDS for E + groups values.  false: numbers that decide lie closer than Real can tell
         template <int LANES, int V, class Real, class Key>
-        __device__ __forceinline__ bool choose(const Routing& r, const float (&v)[V], size_t row, int lane, Real* room, int& expert, Real& score)
+        __device__ __forceinline__ bool choose(const Routing& r, size_t row, uint32_t from, Real* room, int& expert, Real& score)
         {
             constexpr bool APPROXIMATE = sizeof(Real) == 4;
             constexpr Real UNIT = (Real)(1.0 / (1 << 20));
-            // whether a comes ahead of b whatever their errors are (of sums: 2 of them each)
+            const int lane = threadIdx.x & (LANES - 1);
+            float v[V];
+            logits_of<LANES>(r, row, from, v);
+            // whether a comes ahead of b whatever their errors are (of sums: 2 of them each).  fp32: exp and the inverse are off by 2^-23 of themselves, exp's
+            // argument l by 2^-23 |l|, which moves a score by 2^-24 at most (its slope falls faster than |l| grows), the softmax's sum by as much as its
+            // terms: 2^-21 of a score of at most 1, and half a step of the sum with the bias
             const auto sure = [&](Real a, Real b, Real errors) { return a - b > errors * UNIT * (1 + __builtin_fabs(a) + __builtin_fabs(b)); };
             bool certain = true;
 
-            Real top = 0, sum = 0;
+            Real top = 0, over = 0;
             if (!r.sigmoid)
             {
                 float most = v[0];
@@ -125,64 +200,74 @@ namespace nnf
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     all += (double)exp_of((Real)v[j] - top);
-                sum = (Real)over_lanes<LANES>(all, [](double a, double b) { return a + b; });
+                all = over_lanes<LANES>(all, [](double a, double b) { return a + b; });
+                over = all > 0 ? inverse_of((Real)all) : 0;
             }
-            const auto score_of = [&](float x) -> Real {
-                if (r.sigmoid)
-                    return 1 / (1 + exp_of(-(Real)x));
-                return sum > 0 ? exp_of((Real)x - top) / sum : 0;
-            };
+            const auto score_of = [&](float x) -> Real { return r.sigmoid ? inverse_of(1 + exp_of(-(Real)x)) : exp_of((Real)x - top) * over; };
 
             const bool restricted = r.top_groups < r.groups, by_logit = !r.bias, exact = by_logit && (!restricted || r.group_top == 1);
             const int size = r.E / r.groups;
             const uint32_t inverse = ((1u << 22) + size - 1) / size; // i / size = i inverse >> 22 for i below 1024: the excess stays below 1 / size
+            int E = r.E;
+            asm volatile("" : "+s"(E));
             Key key[V];
 #pragma unroll
             for (int j = 0; j < V; ++j)
             {
                 const int i = j * LANES + lane;
                 Real c = v[j];
-                if (!exact && v[j] != LOWEST)
+                if (!exact)
                 {
-                    c = score_of(v[j]);
-                    if (r.bias && i < r.E)
-                        c += (Real)r.bias[i];
-                    c = c != c ? (Real)LOWEST : c > (Real)LARGEST ? (Real)LARGEST : c;
+                    c = score_of(v[j]) + (r.bias ? (Real)r.bias[min(i, E - 1)] : 0);
+                    c = c != c || v[j] == LOWEST ? (Real)LOWEST : c > (Real)LARGEST ? (Real)LARGEST : c;
                 }
-                key[j] = i < r.E ? key_of(by_logit ? (Real)v[j] : c) : 0;
-                if (restricted && i < r.E)
+                key[j] = i < E ? key_of(by_logit ? (Real)v[j] : c) : 0;
+                if (restricted && i < E)
                     room[i + (i * inverse >> 22)] = c; // (a group's values behind each other, a group a value further: other banks)
             }
             if (restricted)
             {
+                constexpr int PARTS = LANES / MAX_GROUPS; // lanes to a group
                 lanes_meet();
-                Key group_key = 0;
-                if (lane < r.groups)
-                {
-                    const Real* const at = room + lane * (size + 1);
-                    Real first = LOWEST, second = LOWEST;
-                    for (int i = 0; i < size; ++i)
+                const int group = lane / PARTS;
+                Real first = LOWEST, second = LOWEST;
+                if (group < r.groups)
+                    for (int i = lane % PARTS; i < size; i += PARTS)
                     {
-                        const Real c = at[i];
+                        const Real c = room[group * (size + 1) + i];
                         second = c > first ? first : c > second ? c : second;
                         first = c > first ? c : first;
                     }
-                    group_key = key_of(r.group_top == 1 ? first : first + second);
+                if constexpr (PARTS > 1)
+                {
+                    static_assert(PARTS == 4, "a group's lanes are four neighbours");
+                    const auto meet = [&](Real other_first, Real other_second) {
+                        const Real less = first < other_first ? first : other_first;
+                        first = first < other_first ? other_first : first;
+                        second = second < other_second ? other_second : second;
+                        second = second < less ? less : second;
+                    };
+                    meet(moved<0xB1>(first), moved<0xB1>(second)); // quad_perm 1,0,3,2
+                    meet(moved<0x4E>(first), moved<0x4E>(second)); // 2,3,0,1
                 }
                 lanes_meet();
+                Key group_key = group < r.groups ? key_of(r.group_top == 1 ? first : first + second) : 0;
                 uint32_t kept = 0;
                 Key last = 0;
                 for (int g = 0; g <= r.top_groups; ++g)
                 {
-                    Key best = group_key;
-                    int at = lane;
-                    best_of_lanes<LANES>(best, at);
+                    const Key best = largest<LANES>(group_key);
                     if (APPROXIMATE && !exact && g > 0)
                         certain = certain && sure(value_of(last), value_of(best), 2);
                     last = best;
+                    int at;
+                    if constexpr (LANES == 64)
+                        at = __builtin_ctzll(__ballot(group_key == best)) / PARTS;
+                    else
+                        at = (int)least_of_16_lanes(group_key == best ? (uint32_t)group : ~0u);
                     if (g < r.top_groups)
                         kept |= 1u << at;
-                    if (lane == at)
+                    if (group == at)
                         group_key = 0;
                 }
 #pragma unroll
@@ -196,44 +281,58 @@ namespace nnf
             expert = 0;
             for (int p = 0; p < turns; ++p)
             {
-                Key best = key[0];
-                int at = lane;
+                Key most = key[0];
 #pragma unroll
                 for (int j = 1; j < V; ++j)
-                    if (key[j] > best)
-                        best = key[j], at = j * LANES + lane;
-                best_of_lanes<LANES>(best, at);
+                    most = key[j] > most ? key[j] : most;
+                const Key best = largest<LANES>(most);
                 if (APPROXIMATE && !by_logit && p > 0 && best != 0)
                     certain = certain && sure(value_of(last), value_of(best), 1);
                 last = best;
+                // the lowest index that has it: of the registers the first, of the lanes the first
+                int at = 0;
+                if constexpr (LANES == 64)
+                {
+                    uint64_t has = 0;
+#pragma unroll
+                    for (int j = V - 1; j >= 0; --j)
+                    {
+                        const uint64_t m = __ballot(key[j] == best);
+                        has = m ? m : has;
+                        at = m ? j * WAVE : at;
+                    }
+                    at += __builtin_ctzll(has);
+                }
+                else
+                {
+                    uint32_t mine = ~0u;
+#pragma unroll
+                    for (int j = V - 1; j >= 0; --j)
+                        mine = key[j] == best ? (uint32_t)(j * LANES + lane) : mine;
+                    at = (int)least_of_16_lanes(mine);
+                }
                 if (lane == p)
                     expert = at, own = best;
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (at == j * LANES + lane)
+                    if (j * LANES + lane == at)
                         key[j] = 0;
             }
             score = 0;
             if (lane < r.k && own != key_of((Real)LOWEST))
-                score = score_of(logit(r, row + expert));
+                score = score_of(logit(r, row, from + expert));
             return certain;
         }
 
-        // A workgroup's counts, [WAVES][E], become where each wavefront's next pair of an expert goes; `total` and `ahead` [E] hold how many
-        // there are of each and how many of them the workgroups ahead have.  sums: a word for each wavefront
-        template <int WAVES>
-        __device__ __forceinline__ void find_places(const Routing& r, uint32_t* counts, const uint32_t* total, const uint32_t* ahead, uint32_t* sums, bool writes)
+        // `before` of thread t's run of EACH experts: how many pairs the experts ahead have (own: its own ones').  sums: a word for each wavefront
+        template <int WAVES, int EACH>
+        __device__ __forceinline__ uint32_t pairs_ahead(const uint32_t (&own)[EACH], uint32_t* sums)
         {
-            constexpr int THREADS = WAVES * WAVE, EACH = (MAX_EXPERTS + THREADS - 1) / THREADS;
             const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-            uint32_t own[EACH], all = 0;
+            uint32_t all = 0;
 #pragma unroll
             for (int i = 0; i < EACH; ++i)
-            {
-                const int e = (int)threadIdx.x * EACH + i;
-                own[i] = e < r.E ? total[e] : 0;
                 all += own[i];
-            }
             uint32_t before = all;
 #pragma unroll
             for (int step = 1; step < WAVE; step *= 2)
@@ -245,152 +344,169 @@ namespace nnf
                 sums[wave] = before;
             __syncthreads();
             before -= all;
-            for (int w = 0; w < wave; ++w)
-                before += sums[w];
+            uint32_t ahead[WAVES];
 #pragma unroll
-            for (int i = 0; i < EACH; ++i)
-            {
-                const int e = (int)threadIdx.x * EACH + i;
-                if (e < r.E)
-                {
-                    if (writes)
-                        r.offsets[e] = (int)before;
-                    uint32_t at = before + ahead[e];
-                    for (int w = 0; w < WAVES; ++w)
-                    {
-                        const uint32_t n = counts[w * r.E + e];
-                        counts[w * r.E + e] = at;
-                        at += n;
-                    }
-                    before += own[i];
-                    if (writes && e == r.E - 1)
-                        r.offsets[r.E] = (int)before;
-                }
-            }
-            __syncthreads();
-        }
-
-        // the pairs [first, end) of a wavefront to their places; next: where its next pair of each expert goes
-        template <class Expert>
-        __device__ __forceinline__ void place_pairs(const Routing& r, int first, int end, uint32_t* next, Expert expert_of)
-        {
-            const int lane = threadIdx.x & (WAVE - 1), bits = 32 - __builtin_clz(r.E);
-            for (int at = first; at < end; at += WAVE)
-            {
-                const int p = at + lane;
-                const int e = p < end ? expert_of(p) : -1;
-                uint64_t peers = __ballot(e >= 0);
-                for (int b = 0; b < bits; ++b)
-                {
-                    const uint64_t set = __ballot(e >> b & 1);
-                    peers &= e >> b & 1 ? set : ~set;
-                }
-                if (e >= 0)
-                {
-                    const uint32_t place = next[e] + (uint32_t)__builtin_popcountll(peers & ((1ull << lane) - 1));
-                    r.positions[p] = (int)place;
-                    r.rows[place] = p / r.k;
-                    lanes_meet();
-                    if (peers >> lane == 1) // the last of them
-                        next[e] = place + 1;
-                }
-                else if (p < end)
-                {
-                    // (tokens that are not there come behind all others, in their place as in the input)
-                    r.positions[p] = -1;
-                    r.rows[p] = -1;
-                }
-                lanes_meet();
-            }
+            for (int w = 0; w < WAVES; ++w)
+                ahead[w] = sums[w];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w)
+                before += w < wave ? ahead[w] : 0;
+            return before;
         }
 
         __device__ __forceinline__ int live_tokens(const Routing& r) { return r.live ? min(max(*r.live, 0), r.tokens) : r.tokens; }
 
-        // ONE: a workgroup does all, its wavefronts a run of tokens each; else it counts its own for the launch that sorts
+        // the values that LDS holds for a wavefront's tokens, in the first choice and in 64 bits
+        template <int LANES>
+        constexpr __host__ __device__ int room_bytes(int E)
+        {
+            return (E + MAX_GROUPS) * (WAVE / LANES * 4 > 8 ? WAVE / LANES * 4 : 8);
+        }
+
+        // ONE: a workgroup does all, in one turn; else it leaves its counts and its pairs' places among its own to the launch that sorts
         template <int LANES, int V, int WAVES, bool ONE>
         __global__ __launch_bounds__(WAVES* WAVE) void moe_route_kernel(Routing r)
         {
             extern __shared__ __align__(16) uint8_t lds[];
-            constexpr int TURN = WAVE / LANES; // tokens of a wavefront at a time
-            uint32_t* const counts = (uint32_t*)lds;                      // [ONE ? WAVES : 1][E]
-            uint32_t* const total = counts + (ONE ? WAVES : 1) * r.E;     // [E], zeros [E] (ONE)
-            uint32_t* const sums = total + (ONE ? 2 * r.E : 0);           // [WAVES]
-            uint16_t* const ids = (uint16_t*)(sums + WAVES);              // [ONE_LAUNCH * MAX_K] (ONE)
-            double* const rooms = (double*)(lds + (((uint8_t*)(ids + (ONE ? ONE_LAUNCH * MAX_K : 0)) - lds + 7) & ~7));
-            const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (LANES - 1), slot = threadIdx.x % WAVE / LANES;
-            for (int i = threadIdx.x; i < (ONE ? WAVES + 2 : 1) * r.E; i += WAVES * WAVE)
-                counts[i] = 0;
-            __syncthreads();
-
-            const int live = live_tokens(r);
-            const int each = ONE ? (r.tokens + WAVES - 1) / WAVES : tokens_of_workgroup(r.tokens);
-            // ONE: the wavefront's own run; else the workgroup's, its wavefronts in turn
-            const int first = (ONE ? wave : (int)blockIdx.x) * each, end = min(first + each, r.tokens);
-            for (int t0 = first + (ONE ? 0 : wave * TURN); t0 < end; t0 += ONE ? TURN : TURN * WAVES)
+            constexpr int TURN = WAVE / LANES, EACH = (MAX_EXPERTS + WAVES * WAVE - 1) / (WAVES * WAVE); // tokens of a wavefront; experts of a thread
+            uint32_t* const counts = (uint32_t*)lds;        // [WAVES][E]
+            uint32_t* const sums = counts + WAVES * r.E;    // [WAVES]
+            uint8_t* const rooms = (uint8_t*)(sums + WAVES);
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x & (LANES - 1), slot = threadIdx.x % WAVE / LANES;
+            const int live = live_tokens(r), bits = 32 - __builtin_clz(r.E);
+            const int each = ONE ? r.tokens : tokens_of_workgroup(r.tokens);
+            const int first = (int)blockIdx.x * each, end = min(first + each, r.tokens);
+            uint32_t so_far[EACH] = {}; // pairs of the thread's experts in the turns before
+            for (int turn = first; turn < end; turn += TURN * WAVES)
             {
-                const int t = min(t0 + slot, end - 1);
-                const bool mine = t0 + slot < end, there = t < live;
-                const size_t row = (size_t)t * r.E;
-                float v[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    v[j] = j * LANES + lane < r.E ? logit(r, row + j * LANES + lane) : LOWEST;
-                double* const room = rooms + (wave * TURN + slot) * (r.E + r.groups);
-                int expert;
-                float score;
-                if (__any(!choose<LANES, V, float, uint32_t>(r, v, row, lane, (float*)room, expert, score)))
+                for (int i = threadIdx.x; i < WAVES * r.E; i += WAVES * WAVE)
+                    counts[i] = 0;
+                __syncthreads();
+                const int t0 = turn + wave * TURN, t = t0 + slot;
+                const bool there = t < end && t < live;
+                int expert = 0;
+                float score = 0;
+                if (t0 < end && t0 < live)
                 {
-                    double s;
-                    choose<LANES, V, double, uint64_t>(r, v, row, lane, room, expert, s);
-                    score = (float)s;
+                    // (a slot without a token looks at the last one)
+                    const size_t row = (size_t)t0 * r.E;
+                    const int last = min(end, live) - 1 - t0;
+                    uint8_t* const room = rooms + wave * room_bytes<LANES>(r.E);
+                    const bool certain = choose<LANES, V, float, uint32_t>(r, row, min(slot, last) * r.E, (float*)room + slot * (r.E + MAX_GROUPS), expert, score);
+                    if (const uint64_t again = __ballot(!certain))
+                        for (int s = 0; s < TURN; ++s)
+                            if (again >> (s * LANES) & 1)
+                            {
+                                int e;
+                                double x;
+                                choose<64, V * LANES / 64, double, uint64_t>(r, row, min(s, last) * r.E, (double*)room, e, x);
+                                const int e_here = __shfl(e, lane);
+                                const float x_here = __shfl((float)x, lane);
+                                expert = slot == s ? e_here : expert;
+                                score = slot == s ? x_here : score;
+                            }
+                    if (r.renormalize)
+                        score /= over_16_lanes(score, [](float a, float b) { return a + b; }) + 1e-20f;
                 }
-                if (r.renormalize)
-                    score /= over_lanes<16>(score, [](float a, float b) { return a + b; }) + 1e-20f;
-                if (mine && lane < r.k)
+                const bool pair = there && lane < r.k;
+                if (t < end && lane < r.k)
                 {
                     r.weights[(size_t)t * r.k + lane] = there ? score * r.scale : 0.0f;
                     r.experts[(size_t)t * r.k + lane] = there ? expert : -1;
-                    if (there)
-                        atomicAdd(&counts[(ONE ? wave : 0) * r.E + expert], 1u);
+                }
+                // the wavefront's pairs of the same expert: how many are ahead, and the last one counts them
+                uint64_t peers = __ballot(pair);
+                for (int b = 0; b < bits; ++b)
+                {
+                    const uint64_t set = __ballot(expert >> b & 1);
+                    peers &= expert >> b & 1 ? set : ~set;
+                }
+                const int id = threadIdx.x & (WAVE - 1);
+                uint32_t place = (uint32_t)__builtin_popcountll(peers & ((1ull << id) - 1));
+                if (pair && peers >> id == 1)
+                    counts[wave * r.E + expert] = place + 1;
+                __syncthreads();
+                // counts become what is ahead of a wavefront: the turns before, the wavefronts before; ONE: the experts before
+                uint32_t n[EACH][WAVES], own[EACH] = {};
+#pragma unroll
+                for (int i = 0; i < EACH; ++i)
+                {
+                    const int e = (int)threadIdx.x * EACH + i;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w)
+                        n[i][w] = e < r.E ? counts[w * r.E + e] : 0;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w)
+                        own[i] += n[i][w];
+                }
+                uint32_t before = ONE ? pairs_ahead<WAVES>(own, sums) : 0;
+#pragma unroll
+                for (int i = 0; i < EACH; ++i)
+                {
+                    const int e = (int)threadIdx.x * EACH + i;
+                    uint32_t at = ONE ? before : so_far[i];
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w)
+                    {
+                        if (e < r.E)
+                            counts[w * r.E + e] = at;
+                        at += n[i][w];
+                    }
                     if constexpr (ONE)
                     {
-                        ids[t * r.k + lane] = (uint16_t)(there ? expert : 0xFFFF);
-                        if (there)
-                            atomicAdd(&total[expert], 1u);
+                        if (e < r.E)
+                            r.offsets[e] = (int)before;
+                        if (e == r.E - 1)
+                            r.offsets[r.E] = (int)at;
                     }
+                    before += own[i];
+                    so_far[i] += own[i];
                 }
+                __syncthreads();
+                if (pair)
+                {
+                    place += counts[wave * r.E + expert];
+                    r.positions[(size_t)t * r.k + lane] = (int)place;
+                    if constexpr (ONE)
+                        r.rows[place] = t;
+                }
+                else if (ONE && t < end && lane < r.k)
+                {
+                    // (tokens that are not there come behind all others, in their place as in the input)
+                    r.positions[t * r.k + lane] = -1;
+                    r.rows[t * r.k + lane] = -1;
+                }
+                if constexpr (!ONE)
+                    __syncthreads();
             }
-            __syncthreads();
-            if constexpr (ONE)
+            if constexpr (!ONE)
             {
-                find_places<WAVES>(r, counts, total, total + r.E, sums, true);
-                place_pairs(r, first * r.k, end * r.k, counts + wave * r.E, [&](int p) { return ids[p] == 0xFFFF ? -1 : (int)ids[p]; });
-            }
-            else
+#pragma unroll
+                for (int i = 0; i < EACH; ++i)
+                    if (const int e = (int)threadIdx.x * EACH + i; e < r.E)
+                        counts[e] = so_far[i];
+                __syncthreads();
                 for (int i = threadIdx.x; i < count_words(r.E); i += WAVES * WAVE)
                     r.counts[(size_t)blockIdx.x * count_words(r.E) + i] = counts[2 * i] | (2 * i + 1 < r.E ? counts[2 * i + 1] << 16 : 0);
+            }
         }
 
+        // pairs go from their place among their workgroup's to their place among all
         template <int WAVES>
         __global__ __launch_bounds__(WAVES* WAVE) void moe_sort_kernel(Routing r)
         {
             extern __shared__ __align__(16) uint8_t lds[];
-            constexpr int THREADS = WAVES * WAVE;
-            uint32_t* const counts = (uint32_t*)lds;           // [WAVES][E]
-            uint32_t* const total = counts + WAVES * r.E;      // [E]
-            uint32_t* const ahead = total + r.E;               // [E]
-            uint32_t* const sums = ahead + r.E;                // [WAVES]
-            const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-            for (int i = threadIdx.x; i < (WAVES + 2) * r.E; i += THREADS)
-                counts[i] = 0;
+            constexpr int THREADS = WAVES * WAVE, EACH = (MAX_EXPERTS + THREADS - 1) / THREADS;
+            uint32_t* const total = (uint32_t*)lds;    // [E]
+            uint32_t* const ahead = total + r.E;       // [E]: of the workgroups before; then with the experts before
+            uint32_t* const sums = ahead + r.E;        // [WAVES]
+            for (int i = threadIdx.x; i < 2 * r.E; i += THREADS)
+                total[i] = 0;
+            const int each = tokens_of_workgroup(r.tokens), begin = (int)blockIdx.x * each * r.k, end = min(((int)blockIdx.x + 1) * each, r.tokens) * r.k;
+            // (the first pair of a thread is asked for ahead of all else)
+            const int p0 = begin + (int)threadIdx.x;
+            int expert = p0 < end ? r.experts[p0] : -1, place = p0 < end ? r.positions[p0] : 0;
             __syncthreads();
-            // a wavefront's run of pairs, counted
-            const int each = tokens_of_workgroup(r.tokens), end = min(((int)blockIdx.x + 1) * each, r.tokens) * r.k;
-            const int run = (each * r.k + WAVES - 1) / WAVES;
-            const int begin = min((int)blockIdx.x * each * r.k + wave * run, end), last = min(begin + run, end);
-            for (int p = begin + lane; p < last; p += WAVE)
-                if (const int e = r.experts[p]; e >= 0)
-                    atomicAdd(&counts[wave * r.E + e], 1u);
             // everybody's counts: a thread has a word of some of the rows, a run of loads at a time
             const int words = count_words(r.E), groups = (int)gridDim.x;
             const int parts = max(THREADS / words, 1), part = threadIdx.x / words;
@@ -423,18 +539,44 @@ namespace nnf
                         }
                 }
             __syncthreads();
-            find_places<WAVES>(r, counts, total, ahead, sums, blockIdx.x == 0);
-            place_pairs(r, begin, last, counts + wave * r.E, [&](int p) { return r.experts[p]; });
+            uint32_t own[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+            {
+                const int e = (int)threadIdx.x * EACH + i;
+                own[i] = e < r.E ? total[e] : 0;
+            }
+            uint32_t before = pairs_ahead<WAVES>(own, sums);
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+            {
+                const int e = (int)threadIdx.x * EACH + i;
+                if (e < r.E)
+                {
+                    ahead[e] += before;
+                    if (blockIdx.x == 0)
+                        r.offsets[e] = (int)before;
+                }
+                before += own[i];
+                if (blockIdx.x == 0 && e == r.E - 1)
+                    r.offsets[r.E] = (int)before;
+            }
+            __syncthreads();
+            for (int p = p0; p < end; p += THREADS)
+            {
+                if (p != p0)
+                    expert = r.experts[p], place = r.positions[p];
+                // (tokens that are not there come behind all others, in their place as in the input)
+                const int at = expert < 0 ? p : place + (int)ahead[expert];
+                r.positions[p] = expert < 0 ? -1 : at;
+                r.rows[at] = expert < 0 ? -1 : p / r.k;
+            }
         }
-
-        constexpr int SORT_WAVES = 4;
 
         template <int LANES, int V, int WAVES, bool ONE>
         hipError_t launch(hipStream_t s, const Routing& r)
         {
-            const int words = (ONE ? WAVES + 2 : 1) * r.E + WAVES;
-            const int ids = ONE ? ONE_LAUNCH * MAX_K * 2 : 0, rooms = r.top_groups < r.groups ? WAVES * (WAVE / LANES) * (r.E + r.groups) * 8 : 0;
-            const int bytes = words * 4 + ids + 8 + rooms;
+            const int bytes = (WAVES * r.E + WAVES) * 4 + (r.top_groups < r.groups ? WAVES * room_bytes<LANES>(r.E) : 0);
             static LdsGrant granted;
             const hipError_t e = allow_dynamic_lds((const void*)moe_route_kernel<LANES, V, WAVES, ONE>, granted, bytes);
             if (e != hipSuccess)
@@ -442,29 +584,43 @@ namespace nnf
             moe_route_kernel<LANES, V, WAVES, ONE><<<ONE ? 1 : workgroups(r.tokens), WAVES * WAVE, bytes, s>>>(r);
             return hipGetLastError();
         }
-        template <int LANES, int V>
-        hipError_t launch_either(hipStream_t s, const Routing& r)
+        template <int LANES, int V, int WAVES>
+        hipError_t launch_both(hipStream_t s, const Routing& r)
         {
-            if (r.tokens <= ONE_LAUNCH)
-                return launch<LANES, V, 8, true>(s, r);
-            const hipError_t e = launch<LANES, V, 4, false>(s, r);
+            const hipError_t e = launch<LANES, V, WAVES, false>(s, r);
             if (e != hipSuccess)
                 return e;
-            moe_sort_kernel<SORT_WAVES><<<workgroups(r.tokens), SORT_WAVES * WAVE, ((SORT_WAVES + 2) * r.E + SORT_WAVES) * 4, s>>>(r);
+            // a wavefront for each 64 pairs of a workgroup, up to 16: these have all counts of 128 experts under way at once
+            const int pairs = tokens_of_workgroup(r.tokens) * r.k, bytes = (2 * r.E + 16) * 4;
+            if (pairs <= 4 * WAVE)
+                moe_sort_kernel<4><<<workgroups(r.tokens), 4 * WAVE, bytes, s>>>(r);
+            else
+                moe_sort_kernel<16><<<workgroups(r.tokens), 16 * WAVE, bytes, s>>>(r);
             return hipGetLastError();
+        }
+        // V: experts of a lane where four tokens share a wavefront
+        template <int V>
+        hipError_t launch_any(hipStream_t s, const Routing& r)
+        {
+            if (r.tokens <= 16)
+                return launch<64, V / 4, 16, true>(s, r);
+            if (r.tokens <= ONE_LAUNCH)
+                return launch<16, V, 16, true>(s, r);
+            return launch_both<16, V, 16>(s, r);
         }
     } // namespace
 
     hipError_t launch_moe_route(hipStream_t s, const moe::Routing& r)
     {
         if (r.E <= 64)
-            return launch_either<16, 4>(s, r);
+            return launch_any<4>(s, r);
         if (r.E <= 128)
-            return launch_either<16, 8>(s, r);
+            return launch_any<8>(s, r);
         if (r.E <= 256)
-            return launch_either<16, 16>(s, r);
+            return launch_any<16>(s, r);
+        // (registers for more experts of a lane, and LDS for their counts, there are of fewer wavefronts)
         if (r.E <= 512)
-            return launch_either<64, 8>(s, r);
-        return launch_either<64, 16>(s, r);
+            return r.tokens <= ONE_LAUNCH_WIDE ? launch<64, 8, 8, true>(s, r) : launch_both<64, 8, 8>(s, r);
+        return r.tokens <= ONE_LAUNCH_WIDE ? launch<64, 16, 8, true>(s, r) : launch_both<64, 16, 8>(s, r);
     }
 } // namespace nnf

@@ -22,17 +22,18 @@ namespace nnf
             return choosable(E, k, groups, top_groups, group_top) && tokens > 0 && (long long)tokens * k <= MAX_PAIRS;
         }
 
-        // Up to ONE_LAUNCH tokens one workgroup scores, counts and sorts; above, up to MANY workgroups score, and a second launch sorts
-        constexpr int ONE_LAUNCH = 64, MANY = 256, TOKENS_TURN = 16;
+        // up to so many tokens one workgroup scores and sorts; above, up to MANY workgroups score, and a second launch sorts
+        constexpr int ONE_LAUNCH = 64, ONE_LAUNCH_WIDE = 8, MANY = 256;
+        constexpr int one_launch(int E) { return E <= 256 ? ONE_LAUNCH : ONE_LAUNCH_WIDE; }
         constexpr int tokens_of_workgroup(int tokens)
         {
             const int each = (tokens + MANY - 1) / MANY;
-            return (each + TOKENS_TURN - 1) / TOKENS_TURN * TOKENS_TURN;
+            return (each + 3) / 4 * 4;
         }
         constexpr int workgroups(int tokens) { return (tokens + tokens_of_workgroup(tokens) - 1) / tokens_of_workgroup(tokens); }
         // a row of counts: 16 bits an expert, whole words
         constexpr int count_words(int E) { return (E + 1) / 2; }
-        constexpr size_t workspace_bytes(int tokens, int E) { return tokens <= ONE_LAUNCH ? 0 : (size_t)workgroups(tokens) * count_words(E) * 4; }
+        constexpr size_t workspace_bytes(int tokens, int E) { return tokens <= one_launch(E) ? 0 : (size_t)workgroups(tokens) * count_words(E) * 4; }
 
         // combining takes units of 512 columns of a token, four to a workgroup of 256 threads: fewer than 2^32 threads
         constexpr int combine_units(int N) { return (int)(((long long)N + 511) / 512); }
