@@ -4,7 +4,7 @@
 // lowest index wins a tie.  LANES lanes of a wavefront have a token, V experts to a lane (expert j LANES + lane): the largest is a few
 // comparisons in registers and a reduction over the lanes, k times.  Four tokens to a wavefront share the instructions of that; a token of
 // its own is the shorter way where there are few.  Without a bias the order of the scores is that of the logits, which is exact.  Else
-// sums are computed in fp32 first; where two that are compared lie closer than fp32 can tell (2^-20, a bound on both errors), the whole
+// sums are computed in fp32 first; where two that are compared lie closer than fp32 can tell (some 2^-21, a bound on both errors), the whole
 // wavefront chooses again for that token in 64 bits: a choice does not depend on how exp rounds.
 //
 // The order is a counting sort.  A pair's place among those of its expert comes from a ballot for each bit of the expert's number inside a
@@ -177,14 +177,15 @@ namespace nnf
         __device__ __forceinline__ bool choose(const Routing& r, size_t row, uint32_t from, Real* room, int& expert, Real& score)
         {
             constexpr bool APPROXIMATE = sizeof(Real) == 4;
-            constexpr Real UNIT = (Real)(1.0 / (1 << 20));
+            constexpr Real UNIT = (Real)(1.0 / (1 << 23));
             const int lane = threadIdx.x & (LANES - 1);
             float v[V];
             logits_of<LANES>(r, row, from, v);
-            // whether a comes ahead of b whatever their errors are (of sums: 2 of them each).  fp32: exp and the inverse are off by 2^-23 of themselves, exp's
-            // argument l by 2^-23 |l|, which moves a score by 2^-24 at most (its slope falls faster than |l| grows), the softmax's sum by as much as its
-            // terms: 2^-21 of a score of at most 1, and half a step of the sum with the bias
-            const auto sure = [&](Real a, Real b, Real errors) { return a - b > errors * UNIT * (1 + __builtin_fabs(a) + __builtin_fabs(b)); };
+            // whether a comes ahead of b whatever their errors are, of sums of `terms` scores each.  fp32: exp and the inverse are off by 2^-23 of themselves, exp's
+            // argument l by 2^-24 |l| 1.5, which a score feels s (1 - s) times (at most 1/4, with |l| 0.28): two sigmoids by 4 of 2^-23.  Two softmax
+            // scores, of at most 1 together, by 3 of these and by as much as their sum over 1024 experts can be, 3 more.  Sums round to 2^-24 of
+            // themselves, those of two scores and biases as if they were 2 larger (see below)
+            const auto sure = [&](Real a, Real b, Real terms) { return a - b > terms * (r.sigmoid ? 6 : 8) * UNIT + 2 * UNIT * (__builtin_fabs(a) + __builtin_fabs(b)); };
             bool certain = true;
 
             Real top = 0, over = 0;
@@ -199,7 +200,11 @@ namespace nnf
                 double all = 0; // (so that the sum adds nothing to the errors of the terms)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
+                {
                     all += (double)exp_of((Real)v[j] - top);
+                    if (j % 4 == 3)
+                        __builtin_amdgcn_sched_barrier(0); // (all of them at once would be registers that there are not)
+                }
                 all = over_lanes<LANES>(all, [](double a, double b) { return a + b; });
                 over = all > 0 ? inverse_of((Real)all) : 0;
             }
@@ -224,6 +229,8 @@ namespace nnf
                 key[j] = i < E ? key_of(by_logit ? (Real)v[j] : c) : 0;
                 if (restricted && i < E)
                     room[i + (i * inverse >> 22)] = c; // (a group's values behind each other, a group a value further: other banks)
+                if (j % 4 == 3)
+                    __builtin_amdgcn_sched_barrier(0);
             }
             if (restricted)
             {
@@ -251,6 +258,9 @@ namespace nnf
                     meet(moved<0x4E>(first), moved<0x4E>(second)); // 2,3,0,1
                 }
                 lanes_meet();
+                // (large biases that cancel in a group's sum: their rounding is not in the sum's size)
+                if (APPROXIMATE && r.group_top == 2)
+                    certain = !__any(__builtin_fabs(first) + __builtin_fabs(second) > 4 + 2 * __builtin_fabs(first + second));
                 Key group_key = group < r.groups ? key_of(r.group_top == 1 ? first : first + second) : 0;
                 uint32_t kept = 0;
                 Key last = 0;
@@ -320,7 +330,7 @@ namespace nnf
             }
             score = 0;
             if (lane < r.k && own != key_of((Real)LOWEST))
-                score = score_of(logit(r, row, from + expert));
+                score = score_of(by_logit ? (float)value_of(own) : logit(r, row, from + expert));
             return certain;
         }
 
@@ -602,11 +612,18 @@ namespace nnf
         template <int V>
         hipError_t launch_any(hipStream_t s, const Routing& r)
         {
-            if (r.tokens <= 16)
-                return launch<64, V / 4, 16, true>(s, r);
+            const int each = tokens_of_workgroup(r.tokens);
+            // (a workgroup starts when its last wavefront does: 1.4 us later with 16 of them than with four)
+            if (r.tokens <= 4)
+                return launch<64, V / 4, 4, true>(s, r);
             if (r.tokens <= ONE_LAUNCH)
-                return launch<16, V, 16, true>(s, r);
-            return launch_both<16, V, 16>(s, r);
+                return launch<64, V / 4, 16, true>(s, r);
+            // a token to a wavefront as long as one turn of the workgroup takes them all
+            if (each <= 4)
+                return launch_both<64, V / 4, 4>(s, r);
+            if (each <= 16)
+                return launch_both<64, V / 4, 16>(s, r);
+            return launch_both<16, V, V == 16 ? 8 : 16>(s, r);
         }
     } // namespace
 

@@ -23,7 +23,7 @@ namespace nnf
         }
 
         // up to so many tokens one workgroup scores and sorts; above, up to MANY workgroups score, and a second launch sorts
-        constexpr int ONE_LAUNCH = 64, ONE_LAUNCH_WIDE = 8, MANY = 256;
+        constexpr int ONE_LAUNCH = 16, ONE_LAUNCH_WIDE = 8, MANY = 256;
         constexpr int one_launch(int E) { return E <= 256 ? ONE_LAUNCH : ONE_LAUNCH_WIDE; }
         constexpr int tokens_of_workgroup(int tokens)
         {

@@ -74,6 +74,21 @@ def test_sums_closer_than_fp32_can_tell_are_compared_in_64_bits(gpu):
     _check_route(gpu, logits, 8, bias=1e6 * torch.ones(64))
 
 
+@pytest.mark.parametrize("tokens", [3, 200, 5000])
+def test_large_biases_that_cancel(gpu, tokens):
+    """A group's two best sums are 1000 and -1000 and something: what decides is far below their rounding."""
+    gen = _gen(tokens)
+    n = 32
+    logits = torch.randn((min(tokens, 200), n), generator=gen)
+    bias = torch.tensor([1000.0, -1000.0] * (n // 2)) + 2.0 ** -12 * torch.randn((n,), generator=gen)
+    for kw in (dict(groups=16, top_groups=5, group_top=2), dict(groups=16, top_groups=5, group_top=1), dict()):
+        for score in ("softmax", "sigmoid"):
+            want = ref.route(logits, 3, score=score, bias=bias, **kw)
+            x = logits[torch.arange(tokens) % len(logits)]
+            got = ops.moe_route(x.to(gpu), 3, score=score, bias=bias.to(gpu), **kw)
+            assert torch.equal(got[1].cpu(), want[1][torch.arange(tokens) % len(logits)])
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("tokens", [12, 77])
 def test_masked_experts(gpu, score, tokens):

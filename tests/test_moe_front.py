@@ -54,7 +54,7 @@ def test_routing_refuses_at_the_c_entry():
 
 def test_routing_wants_its_workspace():
     _no_device()
-    assert ops.moe_route_workspace_bytes(64, 256, 8) == 0 and ops.moe_route_workspace_bytes(0, 256, 8) == 0
+    assert ops.moe_route_workspace_bytes(1, 256, 8) == 0 and ops.moe_route_workspace_bytes(0, 256, 8) == 0
     need = ops.moe_route_workspace_bytes(1000, 256, 8)
     assert need > 0
     assert _route(tokens=1000, E=256, workspace_bytes=need) == NO_DEVICE
