@@ -325,14 +325,25 @@ namespace nnf
             };
             // a step of a taller one: the fragments of rows one after the other, each against all of the weights'; each fragment of weights is read anew
             // behind its last use, the rows' next one a fragment ahead.  Ahead of the last rows everything of this step has been read: there the
-            // wavefronts meet, and its place in LDS is free
+            // wavefronts meet, and its place in LDS is free.  Half of what comes S steps later is asked for then, the other half beside the next step's
+            // first rows, where there are enough of them: the loads come at an even rate (all at once: 187 us in place of 167 for 4096 x 8192 x 8192 of zeros, which no
+            // power limit slows)
+            constexpr int EARLY = T::FM > 2 ? (T::LOADS + 1) / 2 : T::LOADS;
+            bool late = false; // whether the other half is still to be asked for
             const auto body = [&](int step, auto full) __attribute__((always_inline)) {
                 const uint32_t next_stage = stage == (T::S - 1) * T::STAGE ? 0 : stage + T::STAGE;
+                const uint32_t last_stage = stage == 0 ? (T::S - 1) * T::STAGE : stage - T::STAGE;
                 float of_step[NS];
                 scales_of_step(step, of_step);
                 unroll_for<0, T::FM>([&](auto fm) __attribute__((always_inline)) {
                     constexpr bool LAST = fm == T::FM - 1;
-                    constexpr int SLOTS = 2 * T::FN, EACH = (4 + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
+                    constexpr int SLOTS = 2 * T::FN, EACH = (4 + SLOTS - 1) / SLOTS, FETCHES = (EARLY + SLOTS - 1) / SLOTS;
+                    if constexpr (fm == 0 && !full)
+                        if (late)
+                        {
+                            unroll_for<EARLY, T::LOADS>([&](auto j) { fetch_load(j, step - 1 + T::S, last_stage, std::true_type{}); });
+                            late = false;
+                        }
                     // (the fragments of weights behind the first are still on their way then)
                     rows_landed(std::integral_constant<int, fm & 1>{}, std::integral_constant<int, fm == 0 ? (T::FN - 1) * 4 : 0>{});
                     if constexpr (fm == 0)
@@ -366,8 +377,13 @@ namespace nnf
                             });
                             if constexpr (LAST && full)
                                 unroll_for<0, FETCHES>([&](auto q) {
-                                    if constexpr (slot * FETCHES + q < T::LOADS)
+                                    if constexpr (slot * FETCHES + q < EARLY)
                                         fetch_load(std::integral_constant<int, slot * FETCHES + q>{}, step + T::S, stage, std::true_type{});
+                                });
+                            if constexpr (fm == 0 && full)
+                                unroll_for<0, FETCHES>([&](auto q) {
+                                    if constexpr (EARLY + slot * FETCHES + q < T::LOADS)
+                                        fetch_load(std::integral_constant<int, EARLY + slot * FETCHES + q>{}, step - 1 + T::S, last_stage, std::true_type{});
                                 });
                             product[mine] = multiply(wf[0][fn][h], af[fm & 1][h], h == 0 ? floatx16{} : product[mine]);
                             __builtin_amdgcn_sched_barrier(0);
@@ -383,7 +399,13 @@ namespace nnf
                         for (int i = 0; i < NS; ++i)
                             scale[i] = as[fm] * of_step[i];
                         if constexpr (T::PRODUCTS == 1)
+                        {
+                            // (the other wavefront's MFMAs go first meanwhile)
+                            __builtin_amdgcn_s_setprio(0);
                             unroll_for<0, 2>([&](auto h) { add(std::integral_constant<int, b>{}, std::integral_constant<int, 0>{}, h); });
+                            __builtin_amdgcn_sched_barrier(0);
+                            __builtin_amdgcn_s_setprio(2);
+                        }
                         __builtin_amdgcn_sched_barrier(0);
                     });
                 });
@@ -454,7 +476,8 @@ namespace nnf
                     {
 #pragma unroll 1
                         for (; step + T::S < whole; ++step)
-                            body(step, std::true_type{});
+                            body(step, std::true_type{}); // (the first one asks again for half of the last step that is there, the same bytes)
+                        late = step > 0;
 #pragma unroll 1
                         for (; step < steps; ++step)
                             body(step, std::false_type{});
