@@ -571,7 +571,7 @@ enum nnf_fp8_variant
     NNF_FP8_TILE_32x64 = 4, /* four */
     NNF_FP8_TILE_64x64 = 5, /* the wavefronts share the tile */
     NNF_FP8_TILE_64x128 = 6,
-    NNF_FP8_TILE_128x128 = 7,
+    NNF_FP8_TILE_128x256 = 7,
     NNF_FP8_TILE_256x256 = 8
 };
 NNF_API int nnf_fp8_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type,

@@ -580,7 +580,7 @@ namespace nnf
         case fp8::TILE_32x64: return launch_either<Tile<1, 1, 4, 1, 2, 2, 2>>(s, o, gate);
         case fp8::TILE_64x64: return launch_either<Tile<2, 2, 1, 1, 1, 4, 4>>(s, o, gate);
         case fp8::TILE_64x128: return launch_either<Tile<2, 2, 1, 1, 2, 3, 4>>(s, o, gate);
-        case fp8::TILE_128x128: return launch_either<Tile<2, 2, 1, 2, 2, 2, 2>>(s, o, gate);
+        case fp8::TILE_128x256: return launch_either<Tile<2, 4, 1, 2, 2, 3, 4>>(s, o, gate);
         default: return launch_either<Tile<2, 4, 1, 4, 2, 2, 2>>(s, o, gate);
         }
     }

@@ -40,7 +40,7 @@ namespace nnf
             TILE_32x64, // four
             TILE_64x64, // the wavefronts share the tile and all of K
             TILE_64x128,
-            TILE_128x128,
+            TILE_128x256,
             TILE_256x256,
             KERNELS
         };
@@ -49,23 +49,24 @@ namespace nnf
         // with steps of 128 values, the rounds of workgroups that a CU runs and `off` where rows do not start on lines of memory (K no multiple of
         // 128).  They are chosen for the choice that comes of them, not for the times (which they give within 15 .. 20 %): fitted to 1194 products on one
         // MI355X, each on every kernel with its weights from HBM (15 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 13 mixtures of 4 .. 256
-        // experts with 4 .. 16000 rows, even and uneven, each with and without SiLU-gate), what they choose takes 1.010 times as long as the best kernel on
-        // average, more than 1.15 times at 11 of them and at most 1.24 times (a row by 2 x 8192 x 8192, SiLU-gate).  Without any one of the
-        // kernels the best of the others would take 1.003 .. 1.017 times as long on average, 1.13 .. 1.42 times at worst.
+        // experts with 4 .. 16000 rows, even and uneven, each with and without SiLU-gate), what they choose takes 1.007 times as long as the best kernel on
+        // average (1.014 of matrices and mixtures that a fit to the others has not seen), more than 1.15 times at 8 of them and at most 1.27 times
+        // (8192 rows in 60 even groups by 2 x 2050 x 1376, SiLU-gate: 189 us on TILE_128x256, 149 on TILE_256x256).  Without any one of the kernels the best
+        // of the others would take 1.003 .. 1.020 times as long on average, 1.13 .. 1.45 times at worst.
         struct KernelFacts
         {
             int rows, cols, ranges, per_cu;
             float start, turn, step, wait, off, rate;
         };
         constexpr KernelFacts FACTS[KERNELS] = {
-            {16, 32, 1, 6, 2.724f, 0.756f, 0.134f, 0.383f, 0.020f, 6.189f},
-            {16, 32, 2, 3, 3.514f, 1.619f, 0.191f, 0.265f, 0.091f, 7.135f},
-            {16, 32, 4, 1, 3.807f, 7.304f, 0.232f, 0.409f, 0.170f, 4.443f},
-            {32, 64, 4, 1, 3.402f, 0.815f, 0.595f, 0.705f, 0.218f, 5.349f},
-            {64, 64, 1, 2, 2.884f, 2.191f, 0.301f, 0.257f, 0.023f, 5.104f},
-            {64, 128, 1, 2, 3.708f, 1.140f, 0.398f, 0.412f, 0.149f, 6.293f},
-            {128, 128, 1, 2, 3.131f, 1.631f, 0.605f, 1.066f, 0.172f, 6.050f},
-            {256, 256, 1, 1, 0.822f, 4.596f, 0.000f, 1.946f, 0.122f, 4.086f},
+            {16, 32, 1, 6, 3.193f, 1.089f, 0.118f, 0.367f, 0.025f, 6.159f},
+            {16, 32, 2, 3, 3.665f, 1.442f, 0.188f, 0.229f, 0.099f, 6.615f},
+            {16, 32, 4, 1, 4.276f, 3.490f, 0.292f, 0.292f, 0.328f, 8.216f},
+            {32, 64, 4, 1, 3.356f, 5.162f, 0.768f, 0.768f, 0.186f, 3.829f},
+            {64, 64, 1, 2, 3.551f, 1.428f, 0.308f, 0.176f, 0.198f, 6.267f},
+            {64, 128, 1, 2, 3.505f, 0.765f, 0.459f, 0.015f, 0.122f, 5.912f},
+            {128, 256, 1, 1, 3.154f, 4.626f, 1.015f, 1.015f, 0.198f, 5.430f},
+            {256, 256, 1, 1, 3.727f, 6.209f, 1.674f, 1.674f, 0.187f, 4.144f},
         };
 
         // bytes of weights (every group's), activations and results
