@@ -15,6 +15,8 @@
 //                                                         into one 3N-row QuantDot + three Slices; three results)
 //   nnf_compile_example mx_experts <out_dir> M H I       (a mixture of four experts on MXFP4: rows picked by an index are quantised,
 //                                                         gate | up with SiLU-gate, quantised, down; x, index, offsets are inputs)
+//   nnf_compile_example fp8_experts <out_dir> M H I      (a mixture of eight experts in block-scaled 8-bit floating point: three of them
+//                                                         for each token by its logits and a bias, gate | up with SiLU-gate, down, weighted back onto x; x, logits, bias are inputs)
 // every form: [include_dir lib_dir [kernel_profiling_dir [prepare]]] at the end; a kernel_profiling_dir switches
 // profiling-based kernel selection on (every candidate kernel of a QuantDot node is timed on the GPU)
 //   nnf_compile_example onnx      <out_dir> <model.onnx> [include_dir lib_dir]
@@ -63,6 +65,20 @@ namespace
         return {g.add_node_and_edge(std::make_shared<op::Constant>(element::u8, Shape{experts, n, k / 2}, data.data()), graph::GNodeVector{}),
                 g.add_node_and_edge(std::make_shared<op::Constant>(element::u8, Shape{experts, n, stride}, bytes.data()), graph::GNodeVector{})};
     }
+    // codes (either sign, up to 0x6F: 240) and scales of `experts` weight matrices of parts * n rows
+    std::pair<std::shared_ptr<graph::GNode>, std::shared_ptr<graph::GNode>> constant_fp8(graph::Graph& g, uint64_t codes, uint64_t scales, size_t experts,
+                                                                                         size_t parts, size_t n, size_t k)
+    {
+        std::vector<int8_t> data(experts * parts * n * k);
+        nnf_gen_uniform_i8(0, codes, -111, 111, data.data(), data.size());
+        for (auto& v : data)
+            v = (int8_t)(v < 0 ? 0x80 | -v : v);
+        const size_t nb = parts * ((n + 127) / 128), kb = (k + 127) / 128;
+        std::vector<float> s(experts * nb * kb);
+        nnf_gen_uniform_f32(0, scales, 0.0005, 0.002, s.data(), s.size());
+        return {g.add_node_and_edge(std::make_shared<op::Constant>(element::u8, Shape{experts, parts * n, k}, data.data()), graph::GNodeVector{}),
+                g.add_node_and_edge(std::make_shared<op::Constant>(element::f32, Shape{experts, nb, kb}, s.data()), graph::GNodeVector{})};
+    }
 } // namespace
 
 int main(int argc, char** argv)
@@ -70,7 +86,7 @@ int main(int argc, char** argv)
     const bool from_onnx = argc >= 4 && std::string(argv[1]) == "onnx";
     if (argc < 6 && !(from_onnx && argc >= 4))
     {
-        fprintf(stderr, "usage: %s <quant_dot|w8a8|mlp|mlp_nodes|mlp_graph|qkv_graph|mx_experts> <out_dir> <d0> <d1> <d2> [include_dir lib_dir]\n"
+        fprintf(stderr, "usage: %s <quant_dot|w8a8|mlp|mlp_nodes|mlp_graph|qkv_graph|mx_experts|fp8_experts> <out_dir> <d0> <d1> <d2> [include_dir lib_dir]\n"
                         "       %s onnx <out_dir> <model.onnx> [include_dir lib_dir]\n", argv[0], argv[0]);
         return 2;
     }
@@ -184,6 +200,26 @@ int main(int argc, char** argv)
             auto y = g->add_node_and_edge(std::make_shared<op::GenericOp>("down", "MxGroupedDot", op::OpConfig::any()),
                                           Inputs{{b, 0}, {b, 1}, {down.first, 0}, {down.second, 0}, {offsets, 0}});
             g->add_node_and_edge(std::make_shared<op::Result>(), {y});
+        }
+        else if (kind == "fp8_experts")
+        {
+            const size_t M = d0, H = d1, I = d2, E = 8;
+            auto x = g->add_node_and_edge(std::make_shared<op::Parameter>(element::f16, Shape{M, H}), graph::GNodeVector{});
+            auto logits = g->add_node_and_edge(std::make_shared<op::Parameter>(element::f32, Shape{M, E}), graph::GNodeVector{});
+            auto bias = g->add_node_and_edge(std::make_shared<op::Parameter>(element::f32, Shape{E}), graph::GNodeVector{});
+            auto up = constant_fp8(*g, S_WQ, S_MXS, E, 2, I, H), down = constant_fp8(*g, S_WQ2, S_MXS2, E, 1, H, I);
+            using Inputs = std::vector<std::pair<std::shared_ptr<graph::GNode>, int>>;
+            const auto node = [&](const char* name, const char* type, const char* config, const Inputs& in) {
+                return g->add_node_and_edge(std::make_shared<op::GenericOp>(name, type, op::OpConfig::any::parse(config)), in);
+            };
+            auto to = node("route", "MoeRoute", "{\"has_bias\": true, \"k\": 3, \"score\": \"sigmoid\", \"groups\": 4, \"top_groups\": 2, \"group_top\": 2, \"scale\": 2.5}",
+                           Inputs{{logits, 0}, {bias, 0}});
+            auto a = node("quantize", "Fp8Quantize", "{\"has_index\": true}", Inputs{{x, 0}, {to, 2}});
+            auto h = node("gate_up", "Fp8GroupedDot", "{\"act\": \"silu_gate\"}", Inputs{{a, 0}, {a, 1}, {up.first, 0}, {up.second, 0}, {to, 3}});
+            auto b = node("quantize_h", "Fp8Quantize", "{}", Inputs{{h, 0}});
+            auto y = node("down", "Fp8GroupedDot", "{}", Inputs{{b, 0}, {b, 1}, {down.first, 0}, {down.second, 0}, {to, 3}});
+            auto out = node("combine", "MoeCombine", "{\"has_residual\": true}", Inputs{{y, 0}, {to, 0}, {to, 4}, {x, 0}});
+            g->add_node_and_edge(std::make_shared<op::Result>(), {out});
         }
         else if (kind == "qkv_graph")
         {
