@@ -116,7 +116,7 @@ namespace
         void* data = nullptr;
         size_t bytes = 0;
         template <typename F>
-        Workspace(PyObject* given, const Tensor& like, F need)
+        Workspace(PyObject* given, const Tensor& like, F need, size_t least = 16)
         {
             if (given != Py_None)
             {
@@ -126,7 +126,9 @@ namespace
                 return;
             }
             const size_t n = need();
-            bytes = n > 16 ? n : 16;
+            bytes = n > least ? n : least;
+            if (!bytes)
+                return;
             own = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
             data = own.data_ptr();
         }
@@ -554,7 +556,7 @@ namespace
         const Owned weights(output(given[0], {tokens, k}, at::kFloat, logits, "weights")), experts(output(given[1], {tokens, k}, at::kInt, logits, "experts")),
             rows(output(given[2], {pairs}, at::kInt, logits, "rows")), offsets(output(given[3], {(int64_t)E + 1}, at::kInt, logits, "offsets")),
             positions(output(given[4], {tokens, k}, at::kInt, logits, "positions"));
-        const Workspace w(v[11], logits, [&] { return nnf_moe_route_workspace_bytes(tokens, E, routing.k); });
+        const Workspace w(v[11], logits, [&] { return nnf_moe_route_workspace_bytes(tokens, E, routing.k); }, 0);
         call("nnf_moe_route", nnf_moe_route, stream(), logits.data_ptr(), type, address(v[3]), address(v[9]), &routing, weights.data(), experts.data(), rows.data(),
              offsets.data(), positions.data(), tokens, E, w.data, w.bytes);
         PyObject* const all = PyTuple_Pack(5, weights.object, experts.object, rows.object, offsets.object, positions.object);
