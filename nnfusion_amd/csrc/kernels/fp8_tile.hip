@@ -41,6 +41,7 @@ namespace nnf
             static constexpr int PRODUCTS = FM * FN > 6 ? 1 : 2;
             static constexpr int LDS = GROUP_LDS * WK > WAVES * 32 * PITCH ? GROUP_LDS * WK : WAVES * 32 * PITCH;
             static_assert(FM == 1 || FM % 2 == 0, "two fragments of rows in turn");
+            static_assert(WK == 1 || GROUP == 1, "wavefronts that meet inside the loop have steps alike");
             static_assert(ROWS % 16 == 0, "rows 16 apart have their pieces in one order");
             static_assert((ROWS == WM * FM * 32 || (ROWS < 32 && GROUP * FM == 1)) && (ROWS + COLS) / 8 % GROUP == 0, "whole loads");
             static_assert(LDS <= (int)MAX_LDS_BYTES && G >= S && S >= 2 && (S - 1) * LOADS < 64, "room for them, and a count");

@@ -577,7 +577,8 @@ namespace nnf
                 if (p != p0)
                     expert = r.experts[p], place = r.positions[p];
                 // (tokens that are not there come behind all others, in their place as in the input)
-                const int at = expert < 0 ? p : place + (int)ahead[expert];
+                // -- inside the buffer also where another call has written to the same workspace meanwhile
+                const int at = expert < 0 ? p : (int)min((uint32_t)place + ahead[min(expert, r.E - 1)], (uint32_t)(r.tokens * r.k - 1));
                 r.positions[p] = expert < 0 ? -1 : at;
                 r.rows[at] = expert < 0 ? -1 : p / r.k;
             }

@@ -528,7 +528,8 @@ namespace
         require(logits.is_contiguous(), "contiguous logits [tokens, experts]");
         const int type = type_of(logits, true, "logits: fp16, bf16 or fp32"), tokens = size32(logits.size(0)), E = size32(logits.size(1));
         const nnf_moe_routing routing = {integer(v[1]), integer(v[2]), integer(v[4]), integer(v[5]), integer(v[6]), truth(v[7]), real(v[8])};
-        const int64_t k = routing.k > 0 ? routing.k : 0, pairs = tokens * k;
+        require(routing.k > 0 && routing.k <= E, "k: at least 1, at most the experts there are"); // (ahead of results of that size)
+        const int64_t k = routing.k, pairs = tokens * k;
         if (v[3] != Py_None)
             require(is(tensor(v[3]), at::kFloat, {E}), "bias: contiguous fp32 [experts]");
         if (v[9] != Py_None)

@@ -389,3 +389,13 @@ def test_route_with_the_mxfp4_products(gpu):
         row = sum(weights[t, j] * ops.mxfp4_gemm(*ops.mxfp4_quantize(x[t:t + 1].contiguous()), wq.view(8, 96, -1)[ids[t, j]], ws.view(8, 96, -1)[ids[t, j]]).float() for j in range(2))
         # two roundings of the experts' rows in fp16 either way (other kernels, another order of sums: a step), one of the result
         assert bool(((y[t].float() - row[0]).abs() <= 2.0 ** -9 * row[0].abs() + 2.0 ** -9 * 2 * 64).all())
+
+
+def test_nothing_to_do_is_refused(gpu):
+    x, w, no = torch.zeros((0, 256), dtype=torch.float16, device=gpu), torch.zeros((8, 256), dtype=torch.float16, device=gpu), torch.zeros(0, dtype=torch.int32, device=gpu)
+    wq, ws = ops.fp8_quantize_weights(w)
+    a, a_s = ops.fp8_quantize(w)
+    for call in (lambda: ops.fp8_quantize(x), lambda: ops.fp8_quantize(w, rows=no), lambda: ops.fp8_quantize_weights(x), lambda: ops.fp8_gemm(a[:0], a_s[:, :0], wq, ws),
+                 lambda: ops.fp8_gemm(a, a_s, wq[:0], ws[:0]), lambda: ops.fp8_grouped_gemm(a, a_s, wq[None][:0], ws[None][:0], torch.zeros(1, dtype=torch.int32, device=gpu))):
+        with pytest.raises(RuntimeError):
+            call()

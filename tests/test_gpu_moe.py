@@ -194,6 +194,71 @@ def test_on_another_stream(gpu):
     assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
+def test_two_graphs_and_another_stream_at_once(gpu):
+    """Each call with results and a workspace of its own, as torch's allocator gives it"""
+    gens = [torch.randn((tokens, n), generator=_gen(20 + n)).to(gpu) for tokens, n in ((700, 64), (300, 128), (2000, 60))]
+    want = [ops.moe_route(x, 6) for x in gens]
+    graphs = []
+    for x in gens[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.moe_route(x, 6)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (graph, out), stream in zip(graphs, streams):
+            for t in out:
+                t.fill_(-5)
+            stream.wait_stream(torch.cuda.current_stream())
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = ops.moe_route(gens[2], 6)
+        torch.cuda.synchronize()
+        for got, w in zip([g[1] for g in graphs] + [eager], want):
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+def test_a_workspace_that_two_calls_share_at_once_leads_nowhere_else(gpu):
+    """What such calls give is not defined, but they write only where their results are."""
+    tokens, n, k, guard = 3000, 200, 8, 4096
+    sizes = [(tokens, k), (tokens, k), (tokens * k,), (n + 1,), (tokens, k)]
+    workspace = torch.zeros(ops.moe_route_workspace_bytes(tokens, n, k), dtype=torch.uint8, device=gpu)
+    calls = []
+    for seed in (1, 2):
+        buffers, out = [], []
+        for i, size in enumerate(sizes):
+            count = torch.Size(size).numel()
+            b = torch.full((count + 2 * guard,), -77, dtype=torch.float32 if i == 0 else torch.int32, device=gpu)
+            buffers.append(b)
+            out.append(b[guard : guard + count].view(size))
+        # (all pairs on a few experts here, on other ones there)
+        logits = 4 * torch.randn((tokens, n), generator=_gen(seed)) + torch.where(torch.arange(n) // 16 == seed, 20.0, 0.0)
+        calls.append((logits.to(gpu), tuple(out), buffers, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for logits, out, _, stream in calls:
+            with torch.cuda.stream(stream):
+                ops.moe_route(logits, k, out=out, workspace=workspace)
+    torch.cuda.synchronize()
+    for logits, out, buffers, _ in calls:
+        for b in buffers:
+            assert bool((b[:guard] == -77).all()) and bool((b[-guard:] == -77).all())
+        for got, want in zip(ops.moe_route(logits, k, out=out, workspace=workspace), ops.moe_route(logits, k)):  # (one at a time they are right)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens", [0, 5])
+def test_nothing_to_do_is_refused(gpu, tokens):
+    logits = torch.zeros((tokens, 8 if tokens == 0 else 0), device=gpu)
+    with pytest.raises((RuntimeError, AssertionError)):
+        ops.moe_route(logits, 2)
+    with pytest.raises(RuntimeError):
+        ops.moe_combine(torch.zeros((0, 64), dtype=torch.float16, device=gpu), torch.zeros((tokens, 2), device=gpu), torch.zeros((tokens, 2), dtype=torch.int32, device=gpu))
+
+
 def _check_combine(gpu, x, weights, positions, residual=None, out=None):
     got = ops.moe_combine(x.to(gpu), weights.to(gpu), positions.to(gpu), None if residual is None else residual.to(gpu), out)
     want, size = ref.combine(x, weights, positions, residual)

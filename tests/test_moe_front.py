@@ -101,6 +101,7 @@ def test_routing_refuses_tensors_it_would_misread():
         "rows of a matrix": {"out": (None, None, torch.zeros((4, 2), dtype=torch.int32), None, None)},
         "offsets without the end": {"out": (None, None, None, torch.zeros(8, dtype=torch.int32), None)},
         "float positions": {"out": (None, None, None, None, torch.zeros((4, 2)))}, "workspace of words": {"workspace": torch.zeros(64, dtype=torch.int32)},
+        "no expert": {"k": 0}, "fewer than none": {"k": -1}, "more than there are": {"k": 9}, "results of terabytes": {"k": 2**31 - 1},
         "host tensors": {},
     }.items():
         with pytest.raises(AssertionError):
