@@ -149,8 +149,9 @@ namespace nnf
             }
     }
 
-    // Y[row(i), n .. n + 7] for each i with a row (row(i) < 0: none), n a multiple of 8 below N
-    template <class T, int COUNT, class Operands, class Row>
+    // Y[row(i), n .. n + 7] for each i with a row (row(i) < 0: none), n a multiple of 8 below N.  PASSING: groups' results, where
+    // that is 16 bytes a lane, past the caches
+    template <class T, int COUNT, bool PASSING = false, class Operands, class Row>
     __device__ __forceinline__ void write_rows(const Operands& o, floatx4 (&y)[COUNT][2], int n, Row row)
     {
         typedef T Eight __attribute__((ext_vector_type(8)));
@@ -189,8 +190,14 @@ namespace nnf
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
             if (row(i) >= 0)
-                *reinterpret_cast<Eight*>((T*)o.Y + (size_t)row(i) * o.N + n) = Eight{(T)y[i][0].x, (T)y[i][0].y, (T)y[i][0].z, (T)y[i][0].w,
-                                                                                     (T)y[i][1].x, (T)y[i][1].y, (T)y[i][1].z, (T)y[i][1].w};
+            {
+                const Eight v = {(T)y[i][0].x, (T)y[i][0].y, (T)y[i][0].z, (T)y[i][0].w, (T)y[i][1].x, (T)y[i][1].y, (T)y[i][1].z, (T)y[i][1].w};
+                uintx4* const to = reinterpret_cast<uintx4*>((T*)o.Y + (size_t)row(i) * o.N + n);
+                if (PASSING && o.offsets) // (of a builtin and a plain store the compiler makes one, plain; the no-op: what has been stored may be overwritten next)
+                    asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 0" ::"v"(to), "v"(__builtin_bit_cast(uintx4, v)) : "memory");
+                else
+                    *to = __builtin_bit_cast(uintx4, v);
+            }
     }
 
     // SiLU(g) * u in fp32
