@@ -228,12 +228,11 @@ namespace nnf
             floatx16 product[2] = {};                  // of a fragment and of the one before
             intx8 wf[WSETS][T::FN][2], af[2][2];       // operands: of a step (and of the next); of a fragment of rows and of the next one
             uintx4 w_read[T::FN][4], a_read[4];        // the halves of those, on their way
-            float as[T::FM], as_last, scale[NS] = {}; // of the rows of a step, the next step's last, the products that wait
+            float as[T::FM], scale[NS] = {};           // of the rows of a step, the products that wait
 
-            const auto read_scales = [&](int step) { // (where this step's are used up, but for the last)
+            const auto read_scales = [&](int step) { // (where this step's are used up)
                 const uint32_t from = as_at + (step / T::G & 1) * T::SCALES + step % T::G * (T::ROWS * 4);
-                unroll_for<0, T::FM - 1>([&](auto f) { lds_read_b32_nowait<f * 128>(as[f], from); });
-                lds_read_b32_nowait<(T::FM - 1) * 128>(as_last, from);
+                unroll_for<0, T::FM>([&](auto f) { lds_read_b32_nowait<f * 128>(as[f], from); });
             };
             // piece s of fragment f
             const auto read_weights = [&](auto f, auto s, uint32_t stage) { lds_read_b128_nowait<f * 32 * STEP_BYTES>(w_read[f][s], piece_at[s] + w_row_at + (w_at + stage)); };
@@ -248,10 +247,9 @@ namespace nnf
                 unroll_for<0, 4>([&](auto s) { lds_wait_also(w_read[f][s]); });
                 unroll_for<0, 2>([&](auto h) { wf[set][f][h] = operand(w_read[f][2 * h], w_read[f][2 * h + 1]); });
             };
-            const auto scales_landed = [&] {
-                unroll_for<0, T::FM - 1>([&](auto f) { lds_wait_also(as[f]); });
-                lds_wait_also(as_last);
-                as[T::FM - 1] = as_last;
+            const auto scales_landed = [&](auto since) {
+                lds_wait<since>(as[0]);
+                unroll_for<1, T::FM>([&](auto f) { lds_wait_also(as[f]); });
             };
             // half h of the products of fragment i that wait
             const auto add = [&](auto i, auto which, auto h) {
@@ -269,7 +267,7 @@ namespace nnf
             const auto whole_landed = [&](auto set) {
                 rows_landed(set, std::integral_constant<int, 0>{});
                 unroll_for<0, T::FN>([&](auto f) { weights_landed(std::integral_constant<int, T::WHOLE ? (int)set : 0>{}, f); });
-                scales_landed();
+                scales_landed(std::integral_constant<int, 0>{});
             };
 
             const auto scales_of_step = [&](int step, float (&of_step)[NS]) {
@@ -278,6 +276,14 @@ namespace nnf
 #pragma unroll
                 for (int i = 0; i < NS; ++i)
                     of_step[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ws[i]), step & (WAVE - 1)));
+            };
+            const auto scales_of_fragment = [&](int fm, const float (&of_step)[NS], float (&of_fragment)[NS]) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                {
+                    of_fragment[i] = as[fm] * of_step[i];
+                    asm volatile("" : "+v"(of_fragment[i])); // (here: the number it comes of is read anew next)
+                }
             };
             const auto multiply = [&](intx8 w, intx8 a, floatx16 c) { return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, E4M3, E4M3, 0, 0, 0, 0); };
 
@@ -294,6 +300,8 @@ namespace nnf
                     fetch_scales(step + T::G);
                 if (!full && step + T::S < steps)
                     fetch(step + T::S, stage);
+                float mine_scale[NS];
+                scales_of_fragment(0, of_step, mine_scale);
                 read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
                 unroll_for<0, B>([&](auto b) {
                     constexpr int SLOTS = 2 * B, READS = (T::FN + 1) * 4, EACH = (READS + SLOTS - 1) / SLOTS, FETCHES = (T::LOADS + SLOTS - 1) / SLOTS;
@@ -319,7 +327,7 @@ namespace nnf
                     });
 #pragma unroll
                     for (int i = 0; i < NS; ++i)
-                        scale[i] = as[0] * of_step[i];
+                        scale[i] = mine_scale[i];
                 });
                 whole_landed(Next{});
                 stage = next_stage;
@@ -348,10 +356,7 @@ namespace nnf
                     // (the fragments of weights behind the first are still on their way then)
                     rows_landed(std::integral_constant<int, fm & 1>{}, std::integral_constant<int, fm == 0 ? (T::FN - 1) * 4 : 0>{});
                     if constexpr (fm == 0)
-                    {
                         weights_landed(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
-                        scales_landed();
-                    }
                     if constexpr (LAST)
                     {
                         arrive(step + 1, next_stage, full);
@@ -359,8 +364,11 @@ namespace nnf
                             fetch_scales(step + T::G);
                         if (!full && step + T::S < steps)
                             fetch(step + T::S, stage);
-                        read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
                     }
+                    float mine_scale[NS];
+                    scales_of_fragment(fm, of_step, mine_scale);
+                    if constexpr (LAST)
+                        read_scales(step + 1); // (behind the last step: what lies in LDS, not used)
                     unroll_for<0, T::FN>([&](auto fn) __attribute__((always_inline)) {
                         constexpr int b = fm * T::FN + fn, mine = T::PRODUCTS == 1 ? 0 : b & 1;
                         if constexpr (fm == 0 && fn > 0)
@@ -398,7 +406,7 @@ namespace nnf
                             unroll_for<0, 4>([&](auto s) { read_weights(fn, s, next_stage); });
 #pragma unroll
                         for (int i = 0; i < NS; ++i)
-                            scale[i] = as[fm] * of_step[i];
+                            scale[i] = mine_scale[i];
                         if constexpr (T::PRODUCTS == 1)
                         {
                             // (the other wavefront's MFMAs go first meanwhile)
@@ -410,6 +418,8 @@ namespace nnf
                         __builtin_amdgcn_sched_barrier(0);
                     });
                 });
+                // (the next step's: what is on its way from one turn of the loop to the next must stay in its registers, and one number changes them)
+                scales_landed(std::integral_constant<int, 4 + T::FN * 4>{});
                 stage = next_stage;
             };
 
@@ -456,6 +466,8 @@ namespace nnf
                     unroll_for<0, T::FN>([&](auto f) { unroll_for<0, 4>([&](auto s) { read_weights(f, s, 0); }); });
                     if constexpr (T::WHOLE)
                         whole_landed(Even{});
+                    else
+                        scales_landed(std::integral_constant<int, 4 + T::FN * 4>{});
                     const int whole = min(steps, max(row_bytes / STEP_BYTES - first_step, 0)); // steps that end within the rows
                     if constexpr (T::WHOLE)
                     {
@@ -482,6 +494,7 @@ namespace nnf
 #pragma unroll 1
                         for (; step < steps; ++step)
                             body(step, std::false_type{});
+                        whole_landed(Even{}); // (what the last step has read ahead: its registers are others' from here on)
                     }
                     // the products that wait still
                     if constexpr (B % 2 != 0)
