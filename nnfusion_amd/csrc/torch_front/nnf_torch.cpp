@@ -9,6 +9,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 
@@ -365,7 +366,8 @@ namespace
     {
         if (given == Py_None)
         {
-            PyObject* const o = THPVariable_Wrap(at::empty(at::IntArrayRef(sizes.begin(), sizes.size()), like.options().dtype(type)));
+            // (on_device's, so a GPU's: straight from the allocator, 0.5 us sooner than through the dispatcher)
+            PyObject* const o = THPVariable_Wrap(Tensor(at::detail::empty_cuda(at::IntArrayRef(sizes.begin(), sizes.size()), type, like.device(), std::nullopt)));
             if (!o)
                 throw Raised();
             return o;
