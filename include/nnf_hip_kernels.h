@@ -572,7 +572,9 @@ enum nnf_fp8_variant
     NNF_FP8_TILE_64x64 = 5, /* the wavefronts share the tile */
     NNF_FP8_TILE_64x128 = 6,
     NNF_FP8_TILE_128x256 = 7,
-    NNF_FP8_TILE_256x256 = 8
+    NNF_FP8_TILE_256x256 = 8,
+    NNF_FP8_ROWS_16x16 = 9, /* weights straight into registers, not through LDS; four ranges of K.  With SiLU-gate 16 gate rows and their up rows */
+    NNF_FP8_ROWS_16x32 = 10 /* with SiLU-gate 32 and 32 */
 };
 NNF_API int nnf_fp8_gemm_variant(nnf_stream_t stream, const void* A, const void* a_scales, const void* W, const void* w_scales, void* Y, int type,
                          int M, int N, int K, const void* bias, const void* residual, int act, int variant);

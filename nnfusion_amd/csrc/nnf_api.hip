@@ -1086,7 +1086,7 @@ namespace
     int fp8_product(nnf_stream_t stream, const nnf::fp8::Operands& o, int type, int act, int variant)
     {
         using namespace nnf::fp8;
-        static_assert((int)NNF_FP8_TILE_256x256 == (int)KERNELS, "variants and kernels in one order, automatic choice first");
+        static_assert((int)NNF_FP8_ROWS_16x32 == (int)KERNELS, "variants and kernels in one order, automatic choice first");
         if (!o.A || !o.As || !o.W || !o.Ws || !o.Y || o.M <= 0 || o.N <= 0 || o.K <= 0 || o.experts <= 0 || !sixteen_bits(type))
             return NNF_ERR_INVALID_ARGUMENT;
         if ((act != NNF_ACT_NONE && act != NNF_ACT_SILU_GATE) || variant < 0 || variant > KERNELS)
@@ -1114,7 +1114,7 @@ namespace
         const int kernel = variant != NNF_FP8_AUTO ? variant - 1 : choose(o.M, o.N, o.K, gate, experts, dev.num_cu);
         if (!fits(FACTS[kernel], o.M, o.N, gate, experts))
             return NNF_ERR_UNSUPPORTED_SHAPE; // (of a variant that the caller names)
-        return (int)nnf::launch_fp8_tiles((hipStream_t)stream, o, kernel, gate);
+        return (int)(kernel <= TILE_256x256 ? nnf::launch_fp8_tiles((hipStream_t)stream, o, kernel, gate) : nnf::launch_fp8_rows((hipStream_t)stream, o, kernel, gate));
     }
 } // namespace
 

@@ -42,31 +42,37 @@ namespace nnf
             TILE_64x128,
             TILE_128x256,
             TILE_256x256,
+            ROWS_16x16, // operands straight into registers, a wavefront for each range of K: four; with SiLU-gate 16 gate rows and 16 up rows
+            ROWS_16x32, // four; with SiLU-gate 32 and 32
             KERNELS
         };
         // What is known of a kernel: its tile, ranges of K, workgroups that a CU holds at once, and the constants of its time in us,
         //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps * (1 + off), wait * rounds * steps * (1 + off), bytes / rate)
         // with steps of 128 values, the rounds of workgroups that a CU runs and `off` where rows do not start on lines of memory (K no multiple of
-        // 128).  They are chosen for the choice that comes of them, not for the times (which they give within 15 .. 20 %): fitted to 1194 products on one
-        // MI355X, each on every kernel with its weights from HBM (15 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 13 mixtures of 4 .. 256
-        // experts with 4 .. 16000 rows, even and uneven, each with and without SiLU-gate), what they choose takes 1.007 times as long as the best kernel on
-        // average (1.014 of matrices and mixtures that a fit to the others has not seen), more than 1.15 times at 8 of them and at most 1.27 times
-        // (8192 rows in 60 even groups by 2 x 2050 x 1376, SiLU-gate: 189 us on TILE_128x256, 149 on TILE_256x256).  Without any one of the kernels the best
-        // of the others would take 1.003 .. 1.020 times as long on average, 1.13 .. 1.45 times at worst.
+        // 128); a step of the kernels without LDS goes by the lines that it loads, of weights and of the activation rows there are.  They are chosen for
+        // the choice that comes of them, not for the times (which they give within 12 .. 20 %): fitted to 1194 products on one MI355X, each on every kernel
+        // with its weights from HBM (15 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 13 mixtures of 4 .. 256
+        // experts with 4 .. 16000 rows, even and uneven, each with and without SiLU-gate), what they choose takes 1.009 times as long as the best kernel on
+        // average (1.014 of matrices and mixtures that a fit to the others has not seen), more than 1.15 times at 9 of them and at most 1.22 times
+        // (128 rows in 16 uneven groups by 2 x 2880 x 2880, SiLU-gate: 52.6 us on TILE_64x128).  Without any one of the kernels the best
+        // of the others would take 1.001 .. 1.019 times as long on average, 1.08 .. 1.42 times at worst.
         struct KernelFacts
         {
-            int rows, cols, ranges, per_cu;
+            int rows, cols, gate_cols, ranges, per_cu; // (gate_cols: with SiLU-gate, where that differs: the kernels without LDS)
             float start, turn, step, wait, off, rate;
         };
+        constexpr int tiles_of_columns(const KernelFacts& k, int N, bool gate) { return column_tiles(N, gate ? k.gate_cols : k.cols, gate); }
         constexpr KernelFacts FACTS[KERNELS] = {
-            {16, 32, 1, 6, 3.193f, 1.089f, 0.118f, 0.367f, 0.025f, 6.159f},
-            {16, 32, 2, 3, 3.665f, 1.442f, 0.188f, 0.229f, 0.099f, 6.615f},
-            {16, 32, 4, 1, 4.276f, 3.490f, 0.292f, 0.292f, 0.328f, 8.216f},
-            {32, 64, 4, 1, 3.356f, 5.162f, 0.768f, 0.768f, 0.186f, 3.829f},
-            {64, 64, 1, 2, 3.551f, 1.428f, 0.308f, 0.176f, 0.198f, 6.267f},
-            {64, 128, 1, 2, 3.505f, 0.765f, 0.459f, 0.015f, 0.122f, 5.912f},
-            {128, 256, 1, 1, 3.154f, 4.626f, 1.015f, 1.015f, 0.198f, 5.430f},
-            {256, 256, 1, 1, 3.727f, 6.209f, 1.674f, 1.674f, 0.187f, 4.144f},
+            {16, 32, 32, 1, 6, 3.970f, 0.797f, 0.123f, 0.288f, 0.055f, 6.590f},
+            {16, 32, 32, 2, 3, 3.356f, 0.984f, 0.209f, 0.276f, 0.535f, 6.682f},
+            {16, 32, 32, 4, 1, 4.590f, 3.822f, 0.254f, 0.294f, 0.504f, 8.090f},
+            {32, 64, 64, 4, 1, 3.345f, 2.858f, 0.033f, 0.836f, 0.409f, 4.530f},
+            {64, 64, 64, 1, 2, 4.164f, 1.052f, 0.288f, 0.274f, 0.284f, 6.613f},
+            {64, 128, 128, 1, 2, 4.436f, 0.618f, 0.426f, 0.020f, 0.342f, 6.409f},
+            {128, 256, 256, 1, 1, 4.128f, 3.464f, 0.945f, 0.945f, 0.259f, 6.195f},
+            {256, 256, 256, 1, 1, 2.958f, 5.072f, 0.020f, 1.475f, 0.150f, 4.430f},
+            {16, 16, 32, 4, 4, 2.699f, 0.679f, 0.420f, 0.466f, 0.020f, 6.586f},
+            {16, 32, 64, 4, 4, 2.388f, 0.410f, 0.441f, 0.529f, 0.019f, 6.016f},
         };
 
         // bytes of weights (every group's), activations and results
@@ -79,25 +85,29 @@ namespace nnf
         inline float estimate(const KernelFacts& k, int M, int N, int K, bool gate, int experts, int num_cu, float bytes)
         {
             // blocks of rows: a group ends in a block that is half full on average, and groups are of about one size
-            float blocks = (float)((M + k.rows - 1) / k.rows);
+            float blocks = (float)((M + k.rows - 1) / k.rows), of_group = (float)M;
             if (experts > 0)
             {
                 const int groups = experts < M ? experts : M;
-                blocks = groups * ((float)M / groups / k.rows + 0.5f);
+                of_group = (float)M / groups;
+                blocks = groups * (of_group / k.rows + 0.5f);
                 if (blocks < groups)
                     blocks = (float)groups;
             }
+            float lines = 1;
+            if (k.gate_cols != k.cols)
+                lines = ((gate ? k.gate_cols : k.cols) + (of_group < k.rows ? of_group : k.rows)) * (1 / 32.f);
             const int steps = (blocks_of(K) + k.ranges - 1) / k.ranges;
-            const float most = (float)(int)(blocks * column_tiles(N, k.cols, gate) / num_cu + 0.99999f); // workgroups of a CU
+            const float most = (float)(int)(blocks * tiles_of_columns(k, N, gate) / num_cu + 0.99999f); // workgroups of a CU
             const float rounds = (float)(((int)most + k.per_cu - 1) / k.per_cu);
-            const float work = most * steps * k.step, wait = rounds * steps * k.wait, stream = bytes * 1e-6f / k.rate;
+            const float work = most * steps * k.step * lines, wait = rounds * steps * k.wait * lines, stream = bytes * 1e-6f / k.rate;
             const float steady = (work > wait ? work : wait) * (K % BLOCK ? 1 + k.off : 1);
             return k.start + k.turn * (rounds - 1) + (steady > stream ? steady : stream);
         }
 
         constexpr bool fits(const KernelFacts& k, int M, int N, bool gate, int experts)
         {
-            return most_row_blocks(M, experts, k.rows) * column_tiles(N, k.cols, gate) <= MAX_WORKGROUPS;
+            return most_row_blocks(M, experts, k.rows) * tiles_of_columns(k, N, gate) <= MAX_WORKGROUPS;
         }
         // whether the library has a kernel for a product (experts == 0: one weight matrix): it takes these sizes, and some kernel's grid holds
         // their tiles
@@ -117,7 +127,7 @@ namespace nnf
             int best = KERNELS;
             float time = 0;
             // (unrolled: divisions by constants)
-#pragma GCC unroll 8
+#pragma GCC unroll 16
             for (int k = 0; k < KERNELS; ++k)
             {
                 if (!fits(FACTS[k], M, N, gate, experts))

@@ -360,7 +360,8 @@ def fp8_quantize_weights(w, codes=None, scales=None):
     return _native.fp8_quantize_weights(w, codes, scales)
 
 
-FP8_VARIANTS = {name: i for i, name in enumerate(("auto", "tile_16x32", "tile_16x32_2", "tile_16x32_4", "tile_32x64", "tile_64x64", "tile_64x128", "tile_128x256", "tile_256x256"))}
+FP8_VARIANTS = {name: i for i, name in enumerate(("auto", "tile_16x32", "tile_16x32_2", "tile_16x32_4", "tile_32x64", "tile_64x64", "tile_64x128", "tile_128x256", "tile_256x256",
+                                                       "rows_16x16", "rows_16x32"))}
 
 
 def fp8_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, dtype=None, variant="auto"):

@@ -104,7 +104,7 @@ def test_products_refuse_bad_arguments_at_the_c_entry():
     _no_device()
     assert _gemm() == NO_DEVICE and _grouped() == NO_DEVICE
     for change in ({"a": None}, {"a_s": None}, {"w": None}, {"w_s": None}, {"y": None}, {"m": 0}, {"n": 0}, {"k": 0}, {"m": -1}, {"act": 2}, {"act": -1}, {"type": 2}, {"type": -1},
-                   {"variant": -1}, {"variant": 9}, {"a": A + 8}, {"w": W + 1}, {"a_s": AS + 2}, {"w_s": WS + 1}, {"y": Y + 2}):
+                   {"variant": -1}, {"variant": 11}, {"a": A + 8}, {"w": W + 1}, {"a_s": AS + 2}, {"w_s": WS + 1}, {"y": Y + 2}):
         assert _gemm(**change) == INVALID, change
         assert _grouped(**change) == INVALID, change
     for change in ({"bias": B + 2}, {"residual": R + 8}):
@@ -118,10 +118,10 @@ def test_products_refuse_bad_arguments_at_the_c_entry():
     for good in ({"a_s": AS + 4, "w_s": WS + 8}, {"k": 16, "m": 1, "n": 1}, {"n": 1 << 16, "k": 1 << 15}, {"m": 1 << 26}, {"act": 1, "k": 1 << 22, "n": 511}):
         assert _gemm(**good) == NO_DEVICE, good
         assert _grouped(**good) == NO_DEVICE, good
-    for variant in range(1, 9):
+    for variant in range(1, 11):
         assert _gemm(variant=variant) == NO_DEVICE and _grouped(variant=variant, act=1) == NO_DEVICE
     # sizes whose tiles no grid holds, whichever kernel is asked for
-    for variant in range(9):
+    for variant in range(11):
         assert _gemm(m=1 << 28, n=1 << 12, k=32, variant=variant) == UNSUPPORTED
         assert _grouped(m=1 << 20, experts=1 << 20, n=4096, k=32, variant=variant) == UNSUPPORTED
     for experts in (2**31 - 1, 2**31 - 64, (1 << 30) + 1):
