@@ -8,7 +8,11 @@
 // fp32 and any other one is 2^-17 away from a tie.  Powers of two are kept out of it until the conversion, which takes them for nothing, so that no
 // number leaves fp32's range.  A block with an infinity or NaN: scale NaN, codes 0.
 //
-// One pass over memory, two bytes read and one written a value.
+// One pass over memory, two bytes read and one written a value: bound by HBM where there are enough of them -- 22016 x 4096 in 46 us as rows (5.9 TB/s; a copy
+// of 1 GiB runs at 5.2) and in 46 .. 52 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 11.5 us, 6.5 of them bytes: 44000 short
+// wavefronts of one load each (two or four units a wavefront changed nothing), and scales of 4 bytes a line, which lie as the products want them.  16 rows
+// of 4096 in 2.1 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096 behind
+// takes 2 us longer.
 #include "fp8_launch.h"
 #include "nnf_launch.h"
 

@@ -10,6 +10,11 @@
 // The order is a counting sort.  A pair's place among those of its expert comes from a ballot for each bit of the expert's number inside a
 // wavefront, then from the counts of the wavefronts ahead in LDS, then, in a launch of its own, from those of the workgroups ahead (16 bits
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
+//
+// Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
+// before -- 5.4, 6.3, 7.1 us for 8 of 64, 128, 256 experts in a graph, of which a launch is 1.8, and 9.4 for 256 with sigmoid, bias and groups, in one
+// wavefront; two launches cost 8.9 .. 13.1 us for 512 tokens over as many; many tokens are bound by the instructions of the rounds, 13.1, 17.9, 27.0, 40.7 and
+// 72.9 us for 16384 over 64, 128, 256, 512 and 1024 (128: 11.5 us choose, 5.6 sort).
 #include "moe_launch.h"
 #include "nnf_device.h"
 
