@@ -8,11 +8,12 @@
 // fp32 and any other one is 2^-17 away from a tie.  Powers of two are kept out of it until the conversion, which takes them for nothing, so that no
 // number leaves fp32's range.  A block with an infinity or NaN: scale NaN, codes 0.
 //
-// One pass over memory, two bytes read and one written a value: bound by HBM where there are enough of them -- 22016 x 4096 in 46 us as rows (5.9 TB/s; a copy
-// of 1 GiB runs at 5.2) and in 46 .. 52 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 11.5 us, 6.5 of them bytes: 44000 short
-// wavefronts of one load each (two or four units a wavefront changed nothing), and scales of 4 bytes a line, which lie as the products want them.  16 rows
-// of 4096 in 2.1 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096 behind
-// takes 2 us longer.
+// One pass over memory, two bytes read and one written a value: bound by HBM where there are enough of them -- 22016 x 4096 in 42 us as rows (6.4 TB/s; a copy
+// of 1 GiB runs at 5.2, a read at 6.2) and in 46 .. 52 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 10.7 us, 6.5 of them bytes.  A lane takes 16
+// values, so that a block's scale is made by eight lanes in place of 16, and a workgroup four rows at one place, whose scales lie side by side: with
+// eight values and four places of one row 47, 12.2 us, and 17.4 in place of 10.8 for 32768 x 528; eight rows are as fast, 16 slower.  16 rows of
+// 4096 in 2.3 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096
+// behind takes 2 us longer.
 #include "fp8_launch.h"
 #include "nnf_launch.h"
 
@@ -24,7 +25,7 @@ namespace nnf
 
         constexpr int CONVERT_THREADS = 256;
         constexpr int WAVES = CONVERT_THREADS / WAVE;
-        constexpr int ROWS_OF_GRID = 1 << 15; // in y; the others in z
+        constexpr int ROWS = WAVES, ROWS_OF_GRID = 1 << 15; // rows of a workgroup; so many times that in y, the others in z
 
         __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b)
         {
@@ -42,6 +43,14 @@ namespace nnf
             top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x124, 0xF, 0xF, false)); // row_ror:4
             top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x122, 0xF, 0xF, false)); // row_ror:2
             top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x121, 0xF, 0xF, false)); // row_ror:1
+            return max(top >> 16, top & 0xFFFFu);
+        }
+        // of eight lanes in the low half
+        __device__ __forceinline__ uint32_t top_of_8_lanes(uint32_t top)
+        {
+            top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));  // quad_perm 1,0,3,2
+            top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));  // 2,3,0,1
+            top = max_u16x2(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, false)); // row_half_mirror
             return max(top >> 16, top & 0xFFFFu);
         }
         template <bool BF16>
@@ -95,25 +104,40 @@ namespace nnf
             return c;
         }
 
-        // A wavefront takes 512 values of a row, eight to a lane; a workgroup up to four such units of the same row
-        template <bool BF16>
+        // A wavefront takes 512 or 1024 values of a row, EACH = 8 or 16 to a lane; a workgroup the same of four rows
+        template <bool BF16, int EACH>
         __global__ __launch_bounds__(CONVERT_THREADS) void fp8_quantize_kernel(const uint16_t* __restrict__ x, const int* __restrict__ index, uint8_t* __restrict__ codes,
                                                                                float* __restrict__ scales, int rows, int source_rows, int K)
         {
-            const int lane = threadIdx.x & (WAVE - 1), row = (int)(blockIdx.z * ROWS_OF_GRID + blockIdx.y);
-            const int unit = (int)(blockIdx.x * (blockDim.x / WAVE)) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), k = unit * 512 + lane * 8;
+            constexpr int PIECES = EACH / 8;
+            const int lane = threadIdx.x & (WAVE - 1), row = (int)(blockIdx.z * ROWS_OF_GRID + blockIdx.y) * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+            const int k = ((int)blockIdx.x * WAVE + lane) * EACH;
             if (row >= rows)
                 return;
             const int from = index ? index[row] : row;
-            uintx4 v = {0, 0, 0, 0}; // (a row that is not there is a row of zeros)
+            uintx4 v[PIECES] = {}; // (a row that is not there is a row of zeros)
             if (k < K && from >= 0 && from < source_rows)
-                v = *reinterpret_cast<const uintx4*>(x + (size_t)from * K + k);
-            const Quotient by = quotient_of<BF16>(top_of_16_lanes(top_of(v)));
-            const uintx2 c = codes_of<BF16>(v, by);
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    v[i] = *reinterpret_cast<const uintx4*>(x + (size_t)from * K + k + i * 8);
+            uint32_t top = top_of(v[0]);
+            if constexpr (PIECES == 2)
+                top = top_of_8_lanes(max_u16x2(top, top_of(v[1])));
+            else
+                top = top_of_16_lanes(top);
+            const Quotient by = quotient_of<BF16>(top);
+            uintx2 c[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                c[i] = codes_of<BF16>(v[i], by);
             if (k < K)
             {
-                *reinterpret_cast<uintx2*>(codes + (size_t)row * K + k) = c;
-                if ((lane & 15) == 0)
+                uint8_t* const to = codes + (size_t)row * K + k;
+                if constexpr (PIECES == 2)
+                    *reinterpret_cast<uintx4*>(to) = uintx4{c[0].x, c[0].y, c[1].x, c[1].y};
+                else
+                    *reinterpret_cast<uintx2*>(to) = c[0];
+                if (lane % (BLOCK / EACH) == 0)
                     scales[(size_t)(k >> 7) * rows + row] = by.scale;
             }
         }
@@ -160,12 +184,12 @@ namespace nnf
                     *reinterpret_cast<uintx2*>(codes + (base + n0 + i * 4) * K + k) = codes_of<BF16>(v[i], by);
         }
 
-        template <bool BF16>
+        template <bool BF16, int EACH>
         hipError_t launch_rows(hipStream_t s, const void* x, const void* index, void* codes, float* scales, int rows, int source_rows, int K)
         {
-            const int units = row_units(K), waves = units < WAVES ? units : WAVES;
-            const dim3 grid((units + waves - 1) / waves, rows < ROWS_OF_GRID ? rows : ROWS_OF_GRID, (rows + ROWS_OF_GRID - 1) / ROWS_OF_GRID);
-            fp8_quantize_kernel<BF16><<<grid, waves * WAVE, 0, s>>>((const uint16_t*)x, (const int*)index, (uint8_t*)codes, scales, rows, source_rows, K);
+            const int units = (K + WAVE * EACH - 1) / (WAVE * EACH), of_rows = (rows + ROWS - 1) / ROWS;
+            const dim3 grid(units, of_rows < ROWS_OF_GRID ? of_rows : ROWS_OF_GRID, (of_rows + ROWS_OF_GRID - 1) / ROWS_OF_GRID);
+            fp8_quantize_kernel<BF16, EACH><<<grid, CONVERT_THREADS, 0, s>>>((const uint16_t*)x, (const int*)index, (uint8_t*)codes, scales, rows, source_rows, K);
             return hipGetLastError();
         }
         template <bool BF16>
@@ -178,7 +202,10 @@ namespace nnf
 
     hipError_t launch_fp8_quantize(hipStream_t s, const void* x, bool bf16, const void* index, void* codes, float* scales, int rows, int source_rows, int K)
     {
-        return bf16 ? launch_rows<true>(s, x, index, codes, scales, rows, source_rows, K) : launch_rows<false>(s, x, index, codes, scales, rows, source_rows, K);
+        // (up to 512 a lane of 16 would leave half of the wavefront without any)
+        if (K <= 512)
+            return bf16 ? launch_rows<true, 8>(s, x, index, codes, scales, rows, source_rows, K) : launch_rows<false, 8>(s, x, index, codes, scales, rows, source_rows, K);
+        return bf16 ? launch_rows<true, 16>(s, x, index, codes, scales, rows, source_rows, K) : launch_rows<false, 16>(s, x, index, codes, scales, rows, source_rows, K);
     }
 
     hipError_t launch_fp8_quantize_weights(hipStream_t s, const void* w, bool bf16, void* codes, float* scales, int matrices, int N, int K)

@@ -15,7 +15,7 @@ namespace nnf
         constexpr int MAX_K = 1 << 22; // byte offsets inside a tile of 256 rows stay below 2^31
         // rows of codes start on 16 bytes
         constexpr bool supported(int K) { return K > 0 && K % 16 == 0 && K <= MAX_K; }
-        // quantising takes units of 512 values of a row, up to four to a workgroup, or blocks of 128 x 128; a grid has fewer than 2^32 threads
+        // quantising takes units of 512 values of a row or more, or blocks of 128 x 128; a grid has fewer than 2^32 threads
         constexpr int row_units(int K) { return (K + 511) / 512; }
         constexpr bool convertible(int rows, int K) { return supported(K) && (long long)rows * row_units(K) <= 1 << 24; }
         constexpr long long MAX_WORKGROUPS = (1 << 23) - 1; // a grid has fewer than 2^32 threads, and none of these kernels more than 512 in a workgroup
