@@ -9,7 +9,7 @@
 // number leaves fp32's range.  A block with an infinity or NaN: scale NaN, codes 0.
 //
 // One pass over memory, two bytes read and one written a value: bound by HBM where there are enough of them -- 22016 x 4096 in 42 us as rows (6.4 TB/s; a copy
-// of 1 GiB runs at 5.2, a read at 6.2) and in 46 .. 52 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 10.7 us, 6.5 of them bytes.  A lane takes 16
+// of 1 GiB runs at 5.2, a read at 6.2) and in 48 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 10.7 us, 6.5 of them bytes.  A lane takes 16
 // values, so that a block's scale is made by eight lanes in place of 16, and a workgroup four rows at one place, whose scales lie side by side: with
 // eight values and four places of one row 47, 12.2 us, and 17.4 in place of 10.8 for 32768 x 528; eight rows are as fast, 16 slower.  16 rows of
 // 4096 in 2.3 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096
@@ -142,18 +142,20 @@ namespace nnf
             }
         }
 
-        // A workgroup has a block of 128 x 128, a wavefront 32 rows of it, four rows to a load
+        // A workgroup has a block of 128 x 128, a wavefront 16 rows of it, four rows to a load (32 rows each of four wavefronts: 52 us in place of 48 for
+        // 22016 x 4096; 16 wavefronts 50)
+        constexpr int BLOCK_WAVES = 8;
         template <bool BF16>
-        __global__ __launch_bounds__(CONVERT_THREADS) void fp8_quantize_weights_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ codes,
+        __global__ __launch_bounds__(BLOCK_WAVES* WAVE) void fp8_quantize_weights_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ codes,
                                                                                        float* __restrict__ scales, int row_blocks, int N, int K)
         {
-            __shared__ uint32_t tops[WAVES];
+            constexpr int LOADS = BLOCK / 4 / BLOCK_WAVES;
+            __shared__ uint32_t tops[BLOCK_WAVES];
             const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE, blocks = blocks_of(K);
             const int block = (int)blockIdx.x / blocks, kb = (int)blockIdx.x - block * blocks; // block of rows, of all matrices'
             const int matrix = block / row_blocks;
-            const int n0 = (block - matrix * row_blocks) * BLOCK + wave * 32 + (lane >> 4), k = kb * BLOCK + (lane & 15) * 8;
+            const int n0 = (block - matrix * row_blocks) * BLOCK + wave * (LOADS * 4) + (lane >> 4), k = kb * BLOCK + (lane & 15) * 8;
             const size_t base = (size_t)matrix * N;
-            constexpr int LOADS = 8;
             uintx4 v[LOADS];
             uint32_t top = 0;
 #pragma unroll
@@ -173,7 +175,7 @@ namespace nnf
                 tops[wave] = top;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < WAVES; ++i)
+            for (int i = 0; i < BLOCK_WAVES; ++i)
                 top = max(top, tops[i]);
             const Quotient by = quotient_of<BF16>(top);
             if (threadIdx.x == 0)
@@ -195,7 +197,7 @@ namespace nnf
         template <bool BF16>
         hipError_t launch_weights(hipStream_t s, const void* w, void* codes, float* scales, int matrices, int N, int K)
         {
-            fp8_quantize_weights_kernel<BF16><<<matrices * blocks_of(N) * blocks_of(K), CONVERT_THREADS, 0, s>>>((const uint16_t*)w, (uint8_t*)codes, scales, blocks_of(N), N, K);
+            fp8_quantize_weights_kernel<BF16><<<matrices * blocks_of(N) * blocks_of(K), BLOCK_WAVES * WAVE, 0, s>>>((const uint16_t*)w, (uint8_t*)codes, scales, blocks_of(N), N, K);
             return hipGetLastError();
         }
     } // namespace
