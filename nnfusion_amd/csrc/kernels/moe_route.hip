@@ -12,9 +12,9 @@
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 //
 // Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
-// before -- 5.4, 6.3, 7.1 us for 8 of 64, 128, 256 experts in a graph, of which a launch is 1.8, and 9.4 for 256 with sigmoid, bias and groups, in one
-// wavefront; two launches cost 8.9 .. 13.1 us for 512 tokens over as many; many tokens are bound by the instructions of the rounds, 13.1, 17.9, 27.0, 40.7 and
-// 72.9 us for 16384 over 64, 128, 256, 512 and 1024 (128: 11.5 us choose, 5.6 sort).
+// before -- 5.4, 6.3, 7.0 us for 8 of 64, 128, 256 experts in a graph, of which a launch is 1.8, and 9.3 for 256 with sigmoid, bias and groups, in one
+// wavefront; two launches cost 9.4 .. 13.2 us for 512 tokens over as many; many tokens are bound by the instructions of the rounds, 15.0, 17.9, 26.2, 41 and
+// 98 us for 16384 over 64, 128, 256, 512 and 1024 (128: 11 us choose, 5.6 sort).
 #include "moe_launch.h"
 #include "nnf_device.h"
 
@@ -176,6 +176,17 @@ namespace nnf
         __device__ __forceinline__ float inverse_of(float v) { return __builtin_amdgcn_rcpf(v); }
         __device__ __forceinline__ double inverse_of(double v) { return 1 / v; }
 
+        // f(0) .. f(V - 1), four at a time (all of them at once would be registers that there are not)
+        template <int V, class F>
+        __device__ __forceinline__ void each(F f)
+        {
+            unroll_for<0, V>([&](auto j) {
+                f((int)j);
+                if constexpr (j % 4 == 3)
+                    __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+
         // The experts of the token whose logits begin `from` behind `row`: its lane p < k gets the p-th, and its score (0 of one that is masked).  room: a place
         // in LDS for E + groups values.  false: numbers that decide lie closer than Real can tell
         template <int LANES, int V, class Real, class Key>
@@ -183,7 +194,8 @@ namespace nnf
         {
             constexpr bool APPROXIMATE = sizeof(Real) == 4;
             constexpr Real UNIT = (Real)(1.0 / (1 << 23));
-            const int lane = threadIdx.x & (LANES - 1);
+            int lane = threadIdx.x & (LANES - 1);
+            asm volatile("" : "+v"(lane)); // (what comes of it would be kept from turn to turn, for each of the lane's experts)
             float v[V];
             logits_of<LANES>(r, row, from, v);
             // whether a comes ahead of b whatever their errors are, of sums of `terms` scores each.  fp32: exp and the inverse are off by 2^-23 of themselves, exp's
@@ -203,13 +215,7 @@ namespace nnf
                 most = over_lanes<LANES>(most, [](float a, float b) { return fmaxf(a, b); });
                 top = most == LOWEST ? 0 : (Real)most;
                 double all = 0; // (so that the sum adds nothing to the errors of the terms)
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                {
-                    all += (double)exp_of((Real)v[j] - top);
-                    if (j % 4 == 3)
-                        __builtin_amdgcn_sched_barrier(0); // (all of them at once would be registers that there are not)
-                }
+                each<V>([&](int j) { all += (double)exp_of((Real)v[j] - top); });
                 all = over_lanes<LANES>(all, [](double a, double b) { return a + b; });
                 over = all > 0 ? inverse_of((Real)all) : 0;
             }
@@ -220,23 +226,35 @@ namespace nnf
             const uint32_t inverse = ((1u << 22) + size - 1) / size; // i / size = i inverse >> 22 for i below 1024: the excess stays below 1 / size
             int E = r.E;
             asm volatile("" : "+s"(E));
-            Key key[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j)
+            // (one question after the other, each for all of the lane's experts: asked for each expert they are branches for each)
+            Real c[V];
+            if (exact)
             {
-                const int i = j * LANES + lane;
-                Real c = v[j];
-                if (!exact)
-                {
-                    c = score_of(v[j]) + (r.bias ? (Real)r.bias[min(i, E - 1)] : 0);
-                    c = c != c || v[j] == LOWEST ? (Real)LOWEST : c > (Real)LARGEST ? (Real)LARGEST : c;
-                }
-                key[j] = i < E ? key_of(by_logit ? (Real)v[j] : c) : 0;
-                if (restricted && i < E)
-                    room[i + (i * inverse >> 22)] = c; // (a group's values behind each other, a group a value further: other banks)
-                if (j % 4 == 3)
-                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    c[j] = v[j];
             }
+            else
+            {
+                if (r.sigmoid)
+                    each<V>([&](int j) { c[j] = inverse_of(1 + exp_of(-(Real)v[j])); });
+                else
+                    each<V>([&](int j) { c[j] = exp_of((Real)v[j] - top) * over; });
+                if (r.bias)
+                    each<V>([&](int j) { c[j] += (Real)r.bias[min(j * LANES + lane, E - 1)]; });
+                each<V>([&](int j) { c[j] = c[j] != c[j] || v[j] == LOWEST ? (Real)LOWEST : c[j] > (Real)LARGEST ? (Real)LARGEST : c[j]; });
+            }
+            if (restricted)
+                each<V>([&](int j) {
+                    const int i = j * LANES + lane;
+                    if (i < E)
+                        room[i + (i * inverse >> 22)] = c[j]; // (a group's values behind each other, a group a value further: other banks)
+                });
+            Key key[V];
+            if (by_logit)
+                each<V>([&](int j) { key[j] = j * LANES + lane < E ? key_of((Real)v[j]) : 0; });
+            else
+                each<V>([&](int j) { key[j] = j * LANES + lane < E ? key_of(c[j]) : 0; });
             if (restricted)
             {
                 constexpr int PARTS = LANES / MAX_GROUPS; // lanes to a group
@@ -642,8 +660,12 @@ namespace nnf
         if (r.E <= 256)
             return launch_any<16>(s, r);
         // (registers for more experts of a lane, and LDS for their counts, there are of fewer wavefronts)
-        if (r.E <= 512)
-            return r.tokens <= ONE_LAUNCH_WIDE ? launch<64, 8, 8, true>(s, r) : launch_both<64, 8, 8>(s, r);
-        return r.tokens <= ONE_LAUNCH_WIDE ? launch<64, 16, 8, true>(s, r) : launch_both<64, 16, 8>(s, r);
+        if (r.E > 512)
+            return r.tokens <= ONE_LAUNCH_WIDE ? launch<64, 16, 8, true>(s, r) : launch_both<64, 16, 8>(s, r);
+        if (r.tokens <= ONE_LAUNCH_WIDE)
+            return launch<64, 8, 8, true>(s, r);
+        // (16384 tokens over 512: 41 us, and 71 with a token to a wavefront; over 1024 four would have 64 experts to a lane: 86 and 98, with bias and groups 196 and
+        // 198, but 90 and 86 for 4096)
+        return tokens_of_workgroup(r.tokens) <= 8 ? launch_both<64, 8, 8>(s, r) : launch_both<16, 32, 8>(s, r);
     }
 } // namespace nnf

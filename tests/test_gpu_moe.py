@@ -137,6 +137,17 @@ def test_the_order_of_many(gpu, tokens, n, k):
     assert bool((weights.double().sum(1) - 1).abs().max() < 2.0 ** -18)  # 16 of them, each rounded twice
 
 
+@pytest.mark.parametrize("tokens", [9, 2048, 2049, 4500])
+@pytest.mark.parametrize("n,k,groups,top_groups,group_top,score,with_bias", [(257, 8, 1, 1, 1, "softmax", False), (300, 16, 3, 2, 2, "softmax", True), (512, 10, 16, 4, 2, "sigmoid", True),
+                                                                             (480, 5, 8, 3, 1, "softmax", False), (513, 7, 1, 1, 1, "sigmoid", True)])
+def test_more_than_256_experts(gpu, tokens, n, k, groups, top_groups, group_top, score, with_bias):
+    gen = _gen(tokens + n)
+    x = 1.5 * torch.randn((tokens, n), generator=gen)
+    x[::7, ::5] = float("-inf")
+    bias = 0.05 * torch.randn((n,), generator=gen) if with_bias else None
+    _check_route(gpu, x, k, score=score, bias=bias, groups=groups, top_groups=top_groups, group_top=group_top)
+
+
 def test_skewed_to_one_expert(gpu):
     logits = torch.zeros((3000, 256))
     logits[:, 200] = 5
