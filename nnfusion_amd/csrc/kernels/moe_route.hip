@@ -12,9 +12,10 @@
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 //
 // Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
-// before -- 5.4, 6.3, 7.0 us for 8 of 64, 128, 256 experts in a graph, of which a launch is 1.8, and 9.3 for 256 with sigmoid, bias and groups, in one
-// wavefront; two launches cost 9.4 .. 13.2 us for 512 tokens over as many; many tokens are bound by the instructions of the rounds, 15.0, 17.9, 26.2, 41 and
-// 98 us for 16384 over 64, 128, 256, 512 and 1024 (128: 11 us choose, 5.6 sort).
+// before -- 6.4 and 6.9 us for 8 of 128 and 256 experts in a graph (5.4 for 4 of 60), of which a launch is 1.8, and 8.9 for 256 with sigmoid, bias and groups, in
+// one wavefront: 500 cycles a round of choosing, 3500 for the groups; two launches cost 9.1, 10.9 and 12.8 us for 512 tokens over 60, 128 and 256; many
+// tokens are bound by the instructions of the rounds, 13.0, 17.4, 25.4, 41 and 97 us for 16384 over 60, 128, 256, 512 and 1024 (128: 11 us choose, 5.6 sort).
+#include "grouped_tiles.h"
 #include "moe_launch.h"
 #include "nnf_device.h"
 
@@ -366,13 +367,7 @@ namespace nnf
 #pragma unroll
             for (int i = 0; i < EACH; ++i)
                 all += own[i];
-            uint32_t before = all;
-#pragma unroll
-            for (int step = 1; step < WAVE; step *= 2)
-            {
-                const uint32_t other = __shfl_up(before, step);
-                before += lane >= step ? other : 0;
-            }
+            uint32_t before = (uint32_t)sum_up_to_lane((int)all);
             if (lane == WAVE - 1)
                 sums[wave] = before;
             __syncthreads();
@@ -412,9 +407,10 @@ namespace nnf
             uint32_t so_far[EACH] = {}; // pairs of the thread's experts in the turns before
             for (int turn = first; turn < end; turn += TURN * WAVES)
             {
-                for (int i = threadIdx.x; i < WAVES * r.E; i += WAVES * WAVE)
-                    counts[i] = 0;
-                __syncthreads();
+                // (its own wavefront's: read by others behind the next barrier)
+                for (int i = threadIdx.x & (WAVE - 1); i < r.E; i += WAVE)
+                    counts[wave * r.E + i] = 0;
+                lanes_meet();
                 const int t0 = turn + wave * TURN, t = t0 + slot;
                 const bool there = t < end && t < live;
                 int expert = 0;
