@@ -12,8 +12,8 @@
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 //
 // Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
-// before -- 6.4 and 6.9 us for 8 of 128 and 256 experts in a graph (5.4 for 4 of 60), of which a launch is 1.8, and 8.9 for 256 with sigmoid, bias and groups, in
-// one wavefront: 500 cycles a round of choosing, 3500 for the groups; two launches cost 9.1, 10.9 and 12.8 us for 512 tokens over 60, 128 and 256; many
+// before -- 6.4 and 6.9 us for 8 of 128 and 256 experts in a graph (5.4 for 4 of 60), of which a launch is 1.8, and 8.6 for 256 with sigmoid, bias and groups, in
+// one wavefront: 500 cycles a round of choosing, as much as six rounds for the groups; two launches cost 9.1, 10.9 and 12.8 us for 512 tokens over 60, 128 and 256; many
 // tokens are bound by the instructions of the rounds, 13.0, 17.4, 25.4, 41 and 97 us for 16384 over 60, 128, 256, 512 and 1024 (128: 11 us choose, 5.6 sort).
 #include "grouped_tiles.h"
 #include "moe_launch.h"
@@ -122,6 +122,8 @@ namespace nnf
             else
                 return most;
         }
+        __device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+        __device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) { return (uint64_t)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane); }
         __device__ __forceinline__ uint32_t least_of_16_lanes(uint32_t v)
         {
             return over_16_lanes(v, [](uint32_t a, uint32_t b) { return min(a, b); });
@@ -263,11 +265,19 @@ namespace nnf
                 const int group = lane / PARTS;
                 Real first = LOWEST, second = LOWEST;
                 if (group < r.groups)
-                    for (int i = lane % PARTS; i < size; i += PARTS)
+                    for (int i0 = lane % PARTS; i0 < size; i0 += 4 * PARTS)
                     {
-                        const Real c = room[group * (size + 1) + i];
-                        second = c > first ? first : c > second ? c : second;
-                        first = c > first ? c : first;
+                        Real some[4]; // (four reads under way at once)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            some[u] = room[group * (size + 1) + min(i0 + u * PARTS, size - 1)];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                        {
+                            const Real x = i0 + u * PARTS < size ? some[u] : (Real)LOWEST;
+                            second = x > first ? first : x > second ? x : second;
+                            first = x > first ? x : first;
+                        }
                     }
                 if constexpr (PARTS > 1)
                 {
@@ -285,29 +295,45 @@ namespace nnf
                 // (large biases that cancel in a group's sum: their rounding is not in the sum's size)
                 if (APPROXIMATE && r.group_top == 2)
                     certain = !__any(__builtin_fabs(first) + __builtin_fabs(second) > 4 + 2 * __builtin_fabs(first + second));
-                Key group_key = group < r.groups ? key_of(r.group_top == 1 ? first : first + second) : 0;
-                uint32_t kept = 0;
-                Key last = 0;
-                for (int g = 0; g <= r.top_groups; ++g)
+                // a group's place: how many are ahead of it, each compared with all others (a few instructions each that do not wait for one another)
+                const Key group_key = group < r.groups ? key_of(r.group_top == 1 ? first : first + second) : 0;
+                int place = 0;
+                if constexpr (LANES == 64)
                 {
-                    const Key best = largest<LANES>(group_key);
-                    if (APPROXIMATE && !exact && g > 0)
-                        certain = certain && sure(value_of(last), value_of(best), 2);
-                    last = best;
-                    int at;
-                    if constexpr (LANES == 64)
-                        at = __builtin_ctzll(__ballot(group_key == best)) / PARTS;
-                    else
-                        at = (int)least_of_16_lanes(group_key == best ? (uint32_t)group : ~0u);
-                    if (g < r.top_groups)
-                        kept |= 1u << at;
-                    if (group == at)
-                        group_key = 0;
-                }
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (!(kept >> ((uint32_t)(j * LANES + lane) * inverse >> 22 & 31) & 1))
+                    for (int g = 0; g < MAX_GROUPS; ++g)
+                    {
+                        const Key other = of_lane(group_key, g * PARTS);
+                        place += other > group_key || (other == group_key && g < group);
+                    }
+                }
+                else
+                {
+                    Key other = group_key;
+                    uint32_t whose = (uint32_t)group;
+#pragma unroll
+                    for (int g = 1; g < MAX_GROUPS; ++g)
+                    {
+                        other = moved<0x121>(other), whose = moved<0x121>(whose); // row_ror:1
+                        place += other > group_key || (other == group_key && (int)whose < group);
+                    }
+                }
+                const bool used = group < r.groups && place < r.top_groups;
+                const int first_lane = threadIdx.x & (WAVE - LANES); // of the token
+                using Lanes = std::conditional_t<LANES == 64, uint64_t, uint32_t>;
+                const Lanes kept = (Lanes)(__ballot(used) >> first_lane);
+                if (APPROXIMATE && !exact)
+                {
+                    // (the last that is used and any that is not: their order among themselves changes nothing)
+                    const Key last = over_lanes<LANES>(used ? group_key : ~(Key)0, [](Key a, Key b) { return a < b ? a : b; });
+                    const uint64_t close = __ballot(group < r.groups && !used && !sure(value_of(last), value_of(group_key), 2));
+                    certain = certain && (close >> first_lane & (LANES == 64 ? ~0ull : (1ull << (LANES & 63)) - 1)) == 0;
+                }
+                asm volatile("" : "+v"(lane)); // (an expert's group is computed again, in the place of V registers)
+                each<V>([&](int j) {
+                    if (!(kept >> ((uint32_t)(j * LANES + lane) * inverse >> 22 & 15) * PARTS & 1))
                         key[j] = 0;
+                });
             }
 
             const int turns = r.k + (APPROXIMATE && !by_logit ? 1 : 0);
