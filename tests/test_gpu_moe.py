@@ -148,6 +148,16 @@ def test_more_than_256_experts(gpu, tokens, n, k, groups, top_groups, group_top,
     _check_route(gpu, x, k, score=score, bias=bias, groups=groups, top_groups=top_groups, group_top=group_top)
 
 
+@pytest.mark.parametrize("tokens,n,k,groups,top_groups,group_top,score,type", [
+    (8192, 256, 8, 8, 4, 2, "sigmoid", torch.float32), (8192, 128, 6, 16, 3, 2, "softmax", torch.float16), (6000, 512, 10, 16, 4, 1, "sigmoid", torch.bfloat16)])
+def test_groups_of_many_tokens(gpu, tokens, n, k, groups, top_groups, group_top, score, type):
+    """So many that some groups' sums and some experts' lie closer than fp32 can tell"""
+    gen = _gen(n)
+    logits = (1.5 * torch.randn((tokens, n), generator=gen)).to(type)
+    bias = 0.05 * torch.randn((n,), generator=gen) if score == "sigmoid" else None
+    _check_route(gpu, logits, k, score=score, bias=bias, groups=groups, top_groups=top_groups, group_top=group_top)
+
+
 def test_skewed_to_one_expert(gpu):
     logits = torch.zeros((3000, 256))
     logits[:, 200] = 5
