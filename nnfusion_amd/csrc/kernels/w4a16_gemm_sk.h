@@ -1413,7 +1413,9 @@ namespace nnf
                     for (int i = 0; i < 4; ++i)
                         workgroup_barrier();
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the fragments read ahead for a step that does not exist
+            // the fragments read ahead for a step that does not exist: their registers are others' from here on, and no sooner
+            lds_wait<0>(af[0][0]);
+            unroll_for<1, TM>([&](auto f_c) { lds_wait_also(af[0][decltype(f_c)::value]); });
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));          // nothing may land in LDS or in registers any more ...
             __syncthreads();                                   // ... from any wavefront: the ring is free
             // ---- KH = 2: the two wavefronts of a strip trade sums through LDS: each finishes OWN blocks of 32 rows, the

@@ -1,6 +1,6 @@
 """The tile kernels ask for operands in LDS ahead of their use and wait for them by count, unseen by the compiler: along every path through the
-machine code of the library built here, no instruction touches a register while a read into it may be under way, and no scalar load, which returns
-when it likes, is counted among such reads."""
+machine code of the library built here, no instruction touches a register while a read into it may be under way.  (Scalar loads count in the same
+counter and return when they like: a wait for `n` still leaves no more than n reads.)"""
 import glob
 import os
 import re
@@ -33,7 +33,7 @@ def conflicts(code):
             _, text, target = code[i]
             op = text.split()[0]
             flying = frozenset().union(*reads)
-            if flying & registers(text) or (op.startswith("s_load") and reads):
+            if flying & registers(text):
                 bad.append(text)
             wait = re.search(r"lgkmcnt\((\d+)\)", text) if op == "s_waitcnt" else None
             if wait:
@@ -77,13 +77,14 @@ def test_what_counts_as_too_early():
     assert run(("ds_read_b32 v9, v1",), read, ("s_waitcnt lgkmcnt(1)",), use, end) == 1
     assert run(read, ("v_mov_b32 v6, v0",), end) == 1 and run(read, ("v_mov_b32 v8, v0",), end) == 0
     assert run(read, ("s_waitcnt vmcnt(0)",), use, end) == 1
-    assert run(read, ("s_load_dword s0, s[2:3], 0x0",), ("s_waitcnt lgkmcnt(0)",), end) == 1
+    assert run(read, ("s_load_dword s0, s[2:3], 0x0",), ("s_waitcnt lgkmcnt(1)",), use, end) == 1
+    assert run(read, ("s_load_dword s0, s[2:3], 0x0",), ("s_waitcnt lgkmcnt(0)",), use, end) == 0
     # around a loop: the read of one turn, the use of the next
     assert run(("s_nop 0",), use, ("s_waitcnt lgkmcnt(0)",), read, ("s_cbranch_scc1 65532", 4), end) == 1
     assert run(("s_nop 0",), ("s_waitcnt lgkmcnt(0)",), use, read, ("s_cbranch_scc1 65532", 4), end) == 0
 
 
-@pytest.mark.parametrize("kernel", ["fp8_tile_kernel", "mxfp4_tile_kernel"])
+@pytest.mark.parametrize("kernel", ["fp8_tile_kernel", "mxfp4_tile_kernel", "w8a8_gemm_dl_kernel", "w4a16_gemm_sk_kernel"])
 def test_nothing_touches_an_operand_on_its_way(tmp_path, kernel):
     if not os.path.exists(os.path.join(LLVM, "llvm-objdump")) or not os.path.exists(LIBRARY):
         pytest.skip("needs the built library and the ROCm LLVM tools")
