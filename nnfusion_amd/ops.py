@@ -367,14 +367,15 @@ FP8_VARIANTS = {name: i for i, name in enumerate(("auto", "tile_16x32", "tile_16
 def fp8_gemm(a, a_scales, w, w_scales, bias=None, residual=None, act=0, out=None, dtype=None, variant="auto"):
     """Y [M,N] = A . W^T (+ bias + residual) of block-scaled 8-bit operands: a [M,K] and a_scales [ceil(K/128), M] as fp8_quantize gives them, w [N,K] and
     w_scales [ceil(N/128), ceil(K/128)] as fp8_quantize_weights does; with act=1 SiLU(gate) * up, where w holds the gate rows, then the up
-    rows, and w_scales the gate's blocks, then the up matrix's.  Sums in fp32, one rounding to dtype: that of out, residual or bias where
-    given, else fp16 unless named.  out may be the residual.  variant: one kernel (a key of FP8_VARIANTS) instead of the library's choice."""
+    rows, and w_scales the gate's blocks, then the up matrix's.  Sums in fp32, of products of which the 8-bit matrix instructions keep what lies within
+    2^-13 of the largest of eight neighbours along K (2^-16 of the sums' root mean square for normal data); one rounding to dtype: that of out,
+    residual or bias where given, else fp16 unless named.  out may be the residual.  variant: one kernel (a key of FP8_VARIANTS) instead of the library's choice."""
     return _native.fp8_gemm(a, a_scales, w, w_scales, bias, residual, act, out, dtype, FP8_VARIANTS[variant])
 
 
 def fp8_grouped_gemm(a, a_scales, w, w_scales, offsets, act=0, out=None, dtype=None, variant="auto"):
     """The product of a mixture's experts: rows of a sorted by expert, w [experts, N, K] (2N rows with act=1, SiLU-gate), w_scales f32 [experts,
     ceil(N/128), ceil(K/128)] (twice the blocks with act=1); group e is the rows offsets[e] .. offsets[e+1] (offsets i32 [experts+1], on the device, not
-    decreasing).  Rows of out that belong to no group are left as they are (undefined where out is allocated here).  The library chooses a
-    kernel for all rows of a; where the groups fill little of them, name a variant for the rows there are."""
+    decreasing).  Sums as fp8_gemm's.  Rows of out that belong to no group are left as they are (undefined where out is allocated here).  The library
+    chooses a kernel for all rows of a; where the groups fill little of them, name a variant for the rows there are."""
     return _native.fp8_grouped_gemm(a, a_scales, w, w_scales, offsets, act, out, dtype, FP8_VARIANTS[variant])
