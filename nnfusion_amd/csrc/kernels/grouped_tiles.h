@@ -193,8 +193,10 @@ namespace nnf
             {
                 const Eight v = {(T)y[i][0].x, (T)y[i][0].y, (T)y[i][0].z, (T)y[i][0].w, (T)y[i][1].x, (T)y[i][1].y, (T)y[i][1].z, (T)y[i][1].w};
                 uintx4* const to = reinterpret_cast<uintx4*>((T*)o.Y + (size_t)row(i) * o.N + n);
-                if (PASSING && o.offsets) // (of a builtin and a plain store the compiler makes one, plain; the no-op: what has been stored may be overwritten next)
-                    asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 0" ::"v"(to), "v"(__builtin_bit_cast(uintx4, v)) : "memory");
+                // (of a builtin and a plain store the compiler makes one, plain.  A store of 16 bytes reads its registers in the next two states: these pass
+                // here, as the compiler does not know of it and may have them written next)
+                if (PASSING && o.offsets)
+                    asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" ::"v"(to), "v"(__builtin_bit_cast(uintx4, v)) : "memory");
                 else
                     *to = __builtin_bit_cast(uintx4, v);
             }
