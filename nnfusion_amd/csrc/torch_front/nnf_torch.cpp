@@ -9,7 +9,6 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
-#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 
@@ -366,8 +365,8 @@ namespace
     {
         if (given == Py_None)
         {
-            // (on_device's, so a GPU's: straight from the allocator, 0.5 us sooner than through the dispatcher)
-            PyObject* const o = THPVariable_Wrap(Tensor(at::detail::empty_cuda(at::IntArrayRef(sizes.begin(), sizes.size()), type, like.device(), std::nullopt)));
+            // (through the dispatcher, 0.25 us: modes see it, and deterministic ones fill it)
+            PyObject* const o = THPVariable_Wrap(at::empty(at::IntArrayRef(sizes.begin(), sizes.size()), like.options().dtype(type)));
             if (!o)
                 throw Raised();
             return o;
