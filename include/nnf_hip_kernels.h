@@ -517,7 +517,8 @@ typedef struct nnf_moe_routing
  * -inf or NaN, or a sum that is -inf or NaN, masks its expert: it comes behind all others of the groups in use, with weight 0.  +inf counts as the
  * largest fp32 number.  live (i32, on the device; NULL: all): tokens from *live on (a padded batch) have experts -1, weights 0, positions -1.
  * E up to 1024 and a multiple of groups, k up to top_groups * E / groups, tokens * k up to 2^23 (NNF_ERR_UNSUPPORTED_SHAPE).  No
- * result may overlap an input, another result or the workspace.  Calls that may run at the same time need a workspace each. */
+ * result may overlap an input, another result or the workspace.  Calls that may run at the same time need a workspace each.  The query gives
+ * 0 for calls that want none and for sizes that are not served. */
 NNF_API size_t nnf_moe_route_workspace_bytes(int tokens, int E, int k);
 NNF_API int nnf_moe_route(nnf_stream_t stream, const void* logits, int type, const void* bias, const void* live, const nnf_moe_routing* routing,
                   void* weights, void* experts, void* rows, void* offsets, void* positions, int tokens, int E,

@@ -1014,7 +1014,7 @@ extern "C" {
 
 size_t nnf_moe_route_workspace_bytes(int tokens, int E, int k)
 {
-    return tokens > 0 && E > 0 && k > 0 ? nnf::moe::workspace_bytes(tokens, E) : 0;
+    return nnf::moe::countable(tokens, k) && k <= nnf::moe::MAX_K && E > 0 && E <= nnf::moe::MAX_EXPERTS ? nnf::moe::workspace_bytes(tokens, E) : 0;
 }
 
 int nnf_moe_route(nnf_stream_t stream, const void* logits, int type, const void* bias, const void* live, const nnf_moe_routing* routing, void* weights,

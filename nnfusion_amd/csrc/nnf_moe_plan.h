@@ -11,6 +11,7 @@ namespace nnf
         constexpr int MAX_EXPERTS = 1024, MAX_K = 16, MAX_GROUPS = 16;
         constexpr int MAX_PAIRS = 1 << 23; // (token, slot) pairs of a call: a workgroup's counts stay within 16 bits
 
+        constexpr bool countable(int tokens, int k) { return tokens > 0 && k > 0 && (long long)tokens * k <= MAX_PAIRS; }
         // whether k experts can be chosen among top_groups of `groups` equal groups of E
         constexpr bool choosable(int E, int k, int groups, int top_groups, int group_top)
         {
@@ -19,12 +20,13 @@ namespace nnf
         }
         constexpr bool routable(int tokens, int E, int k, int groups, int top_groups, int group_top)
         {
-            return choosable(E, k, groups, top_groups, group_top) && tokens > 0 && (long long)tokens * k <= MAX_PAIRS;
+            return choosable(E, k, groups, top_groups, group_top) && countable(tokens, k);
         }
 
         // up to so many tokens one workgroup scores and sorts; above, up to MANY workgroups score, and a second launch sorts
         constexpr int ONE_LAUNCH = 16, ONE_LAUNCH_WIDE = 8, MANY = 256;
         constexpr int one_launch(int E) { return E <= 256 ? ONE_LAUNCH : ONE_LAUNCH_WIDE; }
+        // (tokens up to MAX_PAIRS)
         constexpr int tokens_of_workgroup(int tokens)
         {
             const int each = (tokens + MANY - 1) / MANY;

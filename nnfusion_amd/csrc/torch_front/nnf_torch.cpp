@@ -12,6 +12,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 
+#include "../nnf_moe_plan.h"
 #include "nnf_hip_kernels.h"
 
 namespace
@@ -34,6 +35,15 @@ namespace
         if (!ok)
             raise(PyExc_AssertionError, text);
     }
+    // the library's error
+    [[noreturn]] void fail(const char* where, int status)
+    {
+        PyObject* const e = g_error ? PyObject_CallFunction(g_error, "is", status, where) : nullptr;
+        if (e)
+            PyErr_SetObject(g_error, e);
+        Py_XDECREF(e);
+        throw Raised();
+    }
     // one call of the library, the interpreter released meanwhile (a launch into a full queue waits)
     template <typename F, typename... Args>
     void call(const char* where, F* function, Args... args)
@@ -41,13 +51,8 @@ namespace
         PyThreadState* const thread = PyEval_SaveThread();
         const int status = function(args...);
         PyEval_RestoreThread(thread);
-        if (status == NNF_OK)
-            return;
-        PyObject* const e = g_error ? PyObject_CallFunction(g_error, "is", status, where) : nullptr;
-        if (e)
-            PyErr_SetObject(g_error, e);
-        Py_XDECREF(e);
-        throw Raised();
+        if (status != NNF_OK)
+            fail(where, status);
     }
 
     const Tensor& tensor(PyObject* o)
@@ -531,6 +536,8 @@ namespace
         const nnf_moe_routing routing = {integer(v[1]), integer(v[2]), integer(v[4]), integer(v[5]), integer(v[6]), truth(v[7]), real(v[8])};
         require(routing.k > 0 && routing.k <= E, "k: at least 1, at most the experts there are"); // (ahead of results of that size)
         const int64_t k = routing.k, pairs = tokens * k;
+        if (pairs > nnf::moe::MAX_PAIRS) // (likewise)
+            fail("nnf_moe_route", NNF_ERR_UNSUPPORTED_SHAPE);
         if (v[3] != Py_None)
             require(is(tensor(v[3]), at::kFloat, {E}), "bias: contiguous fp32 [experts]");
         if (v[9] != Py_None)
