@@ -17,10 +17,10 @@ namespace nnf
         // bytes of experts' rows from which on they are read past the caches
         constexpr long long PASSING = 256ll << 20;
 
-        // WIDE: all rows start on 16 bytes.  PASS: x is read past the caches
+        // WIDE: all rows start on 16 bytes.  PASS: x is read past the caches.  y may be the residual: a lane reads what it writes, ahead of that
         template <class T, bool WIDE, bool PASS>
         __global__ __launch_bounds__(WAVES* WAVE) void moe_combine_kernel(const T* __restrict__ x, const float* __restrict__ weights,
-                                                                         const int* __restrict__ positions, const T* __restrict__ residual, T* __restrict__ y,
+                                                                         const int* __restrict__ positions, const T* residual, T* y,
                                                                          int units, int row_units, int rows, int k, int N)
         {
             typedef T Eight __attribute__((ext_vector_type(8)));
