@@ -50,12 +50,12 @@ namespace nnf
         //   start + turn * (rounds - 1) + max(step * workgroups of a CU * steps * (1 + off), wait * rounds * steps * (1 + off), bytes / rate)
         // with steps of 128 values, the rounds of workgroups that a CU runs and `off` where rows do not start on lines of memory (K no multiple of
         // 128); a step of the kernels without LDS goes by the lines that it loads, of weights and of the activation rows there are.  They are chosen for
-        // the choice that comes of them, not for the times (which they give within 12 .. 20 %): fitted to 1194 products on one MI355X, each on every kernel
-        // with its weights from HBM (15 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 13 mixtures of 4 .. 256
-        // experts with 4 .. 16000 rows, even and uneven, each with and without SiLU-gate), what they choose takes 1.009 times as long as the best kernel on
-        // average (1.014 of matrices and mixtures that a fit to the others has not seen), more than 1.15 times at 9 of them and at most 1.22 times
-        // (128 rows in 16 uneven groups by 2 x 2880 x 2880, SiLU-gate: 52.6 us on TILE_64x128).  Without any one of the kernels the best
-        // of the others would take 1.001 .. 1.019 times as long on average, 1.08 .. 1.42 times at worst.
+        // the choice that comes of them, not for the times (which they give within 12 .. 20 %), by 1194 products, each on every kernel with its weights
+        // from HBM: 15 matrices from 512 x 2048 to 28672 x 8192 with 1 .. 4096 rows, 13 mixtures of 4 .. 256 experts with 4 .. 16000 rows, even and uneven,
+        // each with and without SiLU-gate.  Timed anew on other cards (profiles/fp8_product_timings.csv, by which a test holds the choice), what they choose
+        // takes 1.010 times as long as the best kernel on average, 1.004 with one matrix and 1.015 with many; 1.009 with 64 .. 2000 rows, and above.  More than
+        // 1.15 times at 9, at most 1.26 times (8192 rows in 60 even groups by 2 x 2050 x 1376, SiLU-gate: 186 us on TILE_128x256, 148 on
+        // TILE_256x256).  Without any one of the kernels the best of the others would take 1.001 .. 1.019 times as long on average, 1.09 .. 1.43 times at worst.
         struct KernelFacts
         {
             int rows, cols, gate_cols, ranges, per_cu; // (gate_cols: with SiLU-gate, where that differs: the kernels without LDS)
