@@ -9,10 +9,11 @@
 // number leaves fp32's range.  A block with an infinity or NaN: scale NaN, codes 0.
 //
 // One pass over memory, two bytes read and one written a value: bound by HBM where there are enough of them -- 22016 x 4096 in 42 us as rows (6.4 TB/s; a copy
-// of 1 GiB runs at 5.2, a read at 6.2) and in 48 as blocks of 128 x 128.  4000 of 1000 rows of 5504 take 10.7 us, 6.5 of them bytes.  A lane takes 16
+// of 1 GiB runs at 5.0 .. 5.2, a read at up to 7.0) and in 42 .. 44 as blocks of 128 x 128 (48 .. 50 where each call's results are new memory).  4000 of 1000
+// rows of 5504 take 10.3 us, 4.8 of them bytes at a read's rate.  A lane takes 16
 // values, so that a block's scale is made by eight lanes in place of 16, and a workgroup four rows at one place, whose scales lie side by side: with
 // eight values and four places of one row 47, 12.2 us, and 17.4 in place of 10.8 for 32768 x 528; eight rows are as fast, 16 slower.  16 rows of
-// 4096 in 2.3 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096
+// 4096 in 2.1 us, of which a launch is 1.8.  Results go through the caches, as a product reads them next: past them, a product of 256 x 4096 x 4096
 // behind takes 2 us longer.
 #include "fp8_launch.h"
 #include "nnf_launch.h"

@@ -7,9 +7,9 @@
 // the A operand: a lane has four consecutive columns of one row of Y, and their scale is one number a lane.  How exact the sums are: as in fp8_tile.hip.
 //
 // Bound by the latency of a batch of loads where a workgroup has few of them (one row by 4096 x 4096, 16.8 MB: 5.4 us, of which a launch takes
-// 1.8; through LDS 6.6), else by HBM: 64 rows in 32 groups by 2048 x 4096, 268 MB, in 46 us (5.8 TB/s; through LDS 52), with SiLU-gate 16 tokens of four
-// experts each, 439 MB, in 66 (6.7 TB/s of what is read at least, as some weights come from the cache at the memory; 76).  Every workgroup reads the activations
-// anew, a line of each row for every 16 or 32 of weights: 16 rows by 11008 x 4096 take 13.9 us, 11.8 through LDS, one row 11.3.  Eight ranges of K in the place of
+// 1.8; through LDS 6.6), else by HBM: 64 rows in 32 groups by 2048 x 4096, 268 MB, in 46 .. 47 us (5.7 TB/s; through LDS 52), with SiLU-gate, 537 MB, in 89
+// (6.0 TB/s; 98); where 23, 24 and 27 of the 32 groups have rows in 69, 71 .. 74 and 80 (5.6 TB/s).  Every workgroup reads the activations
+// anew, a line of each row for every 16 or 32 of weights: 16 rows by 11008 x 4096 take 13.7 us, 11.6 through LDS, one row 10.0.  Eight ranges of K in the place of
 // four: 5.3 us for the first, 1.001 times the time of the best kernel on average where they are missing, so they are.
 #include "fp8_launch.h"
 #include "nnf_launch.h"

@@ -13,11 +13,16 @@
 // bound by memory (fp8_rows.hip, 16 x 16) they took 5.72 in place of 5.45 us for one row by 4096 x 4096, 14.9 for 11.6 at K = 11008, with SiLU-gate 27.2 for
 // 22.6 (16 rows by 2 x 11008 x 4096) and 108 for 89 (64 rows in 32 groups by 2 x 2048 x 4096).
 //
-// What bounds them: 16 x 32 and 32 x 64, a range of K a wavefront, HBM (16 rows by 2 x 11008 x 4096 with SiLU-gate in 16.6 us, 5.4 TB/s) or, where there
-// are few workgroups, the latency of a load, 2 us for the first and 0.25 a step (32 rows by 1024 x 8192: 8.2 us); 64 x 64 and 64 x 128 the loads into LDS, 56
-// bytes a clock and CU (256 rows by 22016 x 4096: 33 us); 128 x 256 and 256 x 256 the matrix cores' clock, which power sets, and between tiles
-// the filling of the stages and the results (4096 x 8192 x 8192: 229 .. 240 us, 2.3 .. 2.4 PFLOP/s; of zeros, which take no power, 167; the library's product with
-// one scale a matrix 209).  64 groups of 256 rows by 4096 x 2048 take 168 us, 704 MB at 4.2 TB/s.
+// What bounds them: 16 x 32 and 32 x 64, a range of K a wavefront, HBM (16 rows by 2 x 11008 x 4096 with SiLU-gate in 20.4 us, 4.4 TB/s; in 17.3 where
+// the weights, 90 MB, are in the cache at the memory from the call before) or, where there are few workgroups, the latency of a load, 2 us for the first and 0.25 a
+// step (32 rows by 1024 x 8192: 8.1 us); 64 x 64 and 64 x 128 the loads into LDS, 56 bytes a clock and CU (256 rows by 22016 x 4096 on 64 x 128: 36 us with
+// the weights in that cache, 47 from HBM; 128 x 256, which is chosen, 33 and 39); 256 x 256 the matrix cores' clock, which power sets, and between tiles the
+// filling of the stages and the results (4096 x 8192 x 8192: 229 .. 243 us, 2.3 .. 2.4 PFLOP/s; of zeros, which take little power, 172; the library's product
+// with one scale a matrix 209; after a rest the first five launches take 238 us each, the next 15 287, those up to the hundredth 245, then 229: the clock).
+// 16000 rows in 64 uneven groups by 4096 x 2048 on 128 x 256 take 218 us: 155 blocks, four fifths full, by 16 columns are ten rounds of the CUs of 4 .. 5 us and
+// 1.1 a step.  A step's matrix work is half of that and its 48 KB are 0.4 us of loads into LDS; HBM gives 3.5 TB/s; what is left is the time until the later of
+// its loads, of which four in ten miss the L2, answer.  64 groups of 256 rows take 194 us, and 164 .. 168 (704 MB at 4.2 TB/s) on 256 x 256, which a caller can
+// name: the estimates do not know the groups and count half a block of each as empty.
 #include "fp8_launch.h"
 #include "nnf_launch.h"
 
@@ -566,7 +571,7 @@ namespace nnf
                 };
                 if (n < o.N)
                 {
-                    // (tall tiles of a mixture, which streams its weights from memory: 64 groups of 256 rows by 4096 x 2048 in
+                    // (tall tiles of a mixture, which streams its weights from memory: 64 groups of 256 rows by 4096 x 2048 on 256 x 256 in
                     // 168 us, 176 without; with combining behind 194 and 206.  One product's weights come from the caches, and its results may stay there)
                     if (o.bf16)
                         write_rows<bf16_t, MINE, (T::FM > 1)>(o, y, n, row);

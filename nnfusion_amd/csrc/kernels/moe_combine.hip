@@ -2,7 +2,7 @@
 //
 // One pass over memory, bound by HBM: a wavefront has 512 columns of a token, eight to a lane, and asks for up to eight experts' pieces
 // ahead of the first sum.  Experts' rows that would not stay in the 256 MB cache at the memory are read past the caches: 8 rows each of 8192 tokens, 4096
-// columns, onto a residual in 106 .. 114 us, 132 without (5.9 .. 6.3 TB/s; a copy of 1 GiB runs at 5.2, a read at 6.2); at 128 MB of rows it would be 30.0 in place of 29.2.
+// columns, onto a residual in 106 .. 114 us, 132 without (5.9 .. 6.3 TB/s; a copy of 1 GiB runs at 5.0 .. 5.2, a read at up to 7.0); at 128 MB of rows it would be 30.0 in place of 29.2.
 #include "moe_launch.h"
 #include "nnf_device.h"
 

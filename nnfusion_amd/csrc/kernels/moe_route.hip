@@ -12,9 +12,12 @@
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 //
 // Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
-// before -- 6.4 and 6.9 us for 8 of 128 and 256 experts in a graph (5.4 for 4 of 60), of which a launch is 1.8, and 8.6 for 256 with sigmoid, bias and groups, in
-// one wavefront: 500 cycles a round of choosing, as much as six rounds for the groups; two launches cost 9.1, 10.9 and 12.8 us for 512 tokens over 60, 128 and 256; many
-// tokens are bound by the instructions of the rounds, 13.0, 17.4, 25.4, 41 and 97 us for 16384 over 60, 128, 256, 512 and 1024 (128: 11 us choose, 5.6 sort).
+// before -- 5.4 and 6.1 us for 8 of 128 and 256 experts in a graph (4.4 for 4 of 60), of which a launch is 1.8, and 7.9 for 256 with sigmoid, bias and groups, in
+// one wavefront: 500 cycles a round of choosing, as much as six rounds for the groups; two launches cost 8.2, 9.9 and 12.1 us for 512 tokens over 60, 128 and 256; many
+// tokens are bound by the instructions of the rounds, 12.3, 16.9, 24.7, 36 and 98 us for 16384 over 60, 128, 256, 512 and 1024, bf16 (128: 11.6 us choose, 5.3 sort).
+//
+// Weights come of the hardware's exp and inverse: off by about 2^-24 of themselves, and by up to 1.5 2^-24 |l - largest| more where
+// logits lie far apart.
 #include "grouped_tiles.h"
 #include "moe_launch.h"
 #include "nnf_device.h"
