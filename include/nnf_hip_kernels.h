@@ -515,8 +515,8 @@ typedef struct nnf_moe_routing
  *   positions i32 [tokens, k]   where in that order a pair lies
  * Without a bias experts are compared by their logits, else (and group sums of two) score + bias as if computed in 64 bits.  A logit of
  * -inf or NaN, or a sum that is -inf or NaN, masks its expert: it comes behind all others of the groups in use, with weight 0.  +inf counts as the
- * largest fp32 number.  Weights are off by about 2^-24 of themselves, by less than 2^-16 for logits within 2^7 of the largest.  live (i32, on the
- * device; NULL: all): tokens from *live on (a padded batch) have experts -1, weights 0, positions -1.
+ * largest fp32 number.  Weights are within 2^-19 of themselves, but for scores below 2^-126, where fp32 has fewer bits.  live (i32, on the device;
+ * NULL: all): tokens from *live on (a padded batch) have experts -1, weights 0, positions -1.
  * E up to 1024 and a multiple of groups, k up to top_groups * E / groups, tokens * k up to 2^23 (NNF_ERR_UNSUPPORTED_SHAPE).  No
  * result may overlap an input, another result or the workspace.  Calls that may run at the same time need a workspace each.  The query gives
  * 0 for calls that want none and for sizes that are not served. */

@@ -12,12 +12,13 @@
 // each in the workspace).  Counts are sums of integers: the same call gives the same order, (expert, token, slot).
 //
 // Not bound by memory (16384 tokens over 128 experts read and write 6 MB, 1.2 us of HBM): one token is a chain of reductions, each waiting for the one
-// before -- 5.4 and 6.1 us for 8 of 128 and 256 experts in a graph (4.4 for 4 of 60), of which a launch is 1.8, and 7.9 for 256 with sigmoid, bias and groups, in
-// one wavefront: 500 cycles a round of choosing, as much as six rounds for the groups; two launches cost 8.2, 9.9 and 12.1 us for 512 tokens over 60, 128 and 256; many
-// tokens are bound by the instructions of the rounds, 12.3, 16.9, 24.7, 36 and 98 us for 16384 over 60, 128, 256, 512 and 1024, bf16 (128: 11.6 us choose, 5.3 sort).
+// before -- 4.9 and 5.7 us for 8 of 128 and 256 experts in a graph of 40 calls (4.0 for 4 of 60), of which a launch is 1.8, and 7.4 for 256 with sigmoid, bias and groups,
+// in one wavefront: 500 cycles a round of choosing, as much as six rounds for the groups; two launches cost 7.8, 9.5 and 11.7 us for 512 tokens over 60, 128 and 256; many
+// tokens are bound by the instructions of the rounds, 11.6, 16.0, 24.1, 36 and 98 us for 16384 over 60, 128, 256, 512 and 1024 (128: 11.6 us choose, 5.3 sort).
 //
-// Weights come of the hardware's exp and inverse: off by about 2^-24 of themselves, and by up to 1.5 2^-24 |l - largest| more where
-// logits lie far apart.
+// The scores that become weights are computed once more, to a step of fp32: by the hardware's exp and inverse, which choosing makes do with, they would be off by
+// 1.5 2^-24 |l - largest| (at most 4.3e-7 of themselves in place of 2.3e-7 for normal logits of 1.5, 2-norm 5.4e-8 either way; 1e-5 where they lie 100 apart), and
+// a call 0.1 .. 0.2 us shorter.
 #include "grouped_tiles.h"
 #include "moe_launch.h"
 #include "nnf_device.h"
@@ -182,6 +183,13 @@ namespace nnf
         __device__ __forceinline__ float inverse_of(float v) { return __builtin_amdgcn_rcpf(v); }
         __device__ __forceinline__ double inverse_of(double v) { return 1 / v; }
 
+        // exp(v - top) to a step of fp32 however far apart they are: what the rounded difference lacks, times its exp, is added.  (Beyond fp32 it is not finite, and exp 0.)
+        __device__ __forceinline__ float exp_of_difference(float v, float top)
+        {
+            const float d = v - top, t = d - v, rest = (v - (d - t)) - (top + t), e = expf(d);
+            return e > 0 ? __builtin_fmaf(e, rest, e) : 0.0f;
+        }
+
         // f(0) .. f(V - 1), four at a time (all of them at once would be registers that there are not)
         template <int V, class F>
         __device__ __forceinline__ void each(F f)
@@ -211,7 +219,7 @@ namespace nnf
             const auto sure = [&](Real a, Real b, Real terms) { return a - b > terms * (r.sigmoid ? 6 : 8) * UNIT + 2 * UNIT * (__builtin_fabs(a) + __builtin_fabs(b)); };
             bool certain = true;
 
-            Real top = 0, over = 0;
+            Real top = 0, sum = 1, over = 0;
             if (!r.sigmoid)
             {
                 float most = v[0];
@@ -223,7 +231,8 @@ namespace nnf
                 double all = 0; // (so that the sum adds nothing to the errors of the terms)
                 each<V>([&](int j) { all += (double)exp_of((Real)v[j] - top); });
                 all = over_lanes<LANES>(all, [](double a, double b) { return a + b; });
-                over = all > 0 ? inverse_of((Real)all) : 0;
+                sum = (Real)all;
+                over = all > 0 ? inverse_of(sum) : 0;
             }
             const auto score_of = [&](float x) -> Real { return r.sigmoid ? inverse_of(1 + exp_of(-(Real)x)) : exp_of((Real)x - top) * over; };
 
@@ -383,7 +392,14 @@ namespace nnf
             }
             score = 0;
             if (lane < r.k && own != key_of((Real)LOWEST))
-                score = score_of(by_logit ? (float)value_of(own) : logit(r, row, from + expert));
+            {
+                const float x = by_logit ? (float)value_of(own) : logit(r, row, from + expert);
+                // (once a token, so not by the hardware's exp and inverse, which the choice makes do with)
+                if constexpr (APPROXIMATE)
+                    score = r.sigmoid ? 1 / (1 + expf(-x)) : exp_of_difference(x, top) / sum;
+                else
+                    score = score_of(x);
+            }
             return certain;
         }
 
